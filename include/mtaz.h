@@ -94,6 +94,82 @@ int mtaz_replay_put(int device, int n, const uint32_t* d_pos, const int32_t* d_k
                     const uint16_t* d_codes, const uint32_t* d_visits, const float* d_reward, int64_t cap,
                     int64_t head, uint8_t* d_tokens, float* d_clocks, float* d_pi, float* d_reward_out, void* stream);
 
+/* ---- learner operators ---------------------------------------------------------------------
+ * Called on device pointers and enqueued on `stream` without a sync; every one may be captured in a
+ * HIP graph.  Scratch memory is the caller's (`d_work`, the size the matching _workspace entry
+ * returns, 256-byte aligned): a call owns it until its work on the stream has ended, so calls on
+ * two streams need two.  Nothing is kept between calls, results do not depend on the launch order of
+ * workgroups, and a refused call (MTAZ_E_FAIL) has enqueued nothing.  Element types: */
+#define MTAZ_F32 0
+#define MTAZ_F16 1
+#define MTAZ_BF16 2
+#define MTAZ_MAX_STEPS 32          /* Newton-Schulz steps of one call */
+
+/* Orthogonalisation of n matrices G [rows][cols] (contiguous, one pointer each in the host array
+ * d_grad), rows, cols <= 65536 and rows * cols <= 2^30: X = G / (|G|_F + eps), then `steps` times
+ * X <- a X + (b S + c S S) X with S = X X^T over the shorter side, coefficients = {a, b, c}.
+ * Computed to 32 bits whatever the type; d_out[i] may be d_grad[i]. */
+int64_t mtaz_orthogonalize_workspace(int n, int64_t rows, int64_t cols, int dtype);
+int mtaz_orthogonalize(int device, int n, int64_t rows, int64_t cols, int dtype, const void* const* d_grad,
+                       void* const* d_out, int steps, const double* coefficients, double eps, void* d_work,
+                       int64_t work_bytes, void* stream);
+/* One Muon step on n parameters of one shape and type, momenta float32:
+ *   m <- momentum m + (1 - momentum) g;  u = nesterov ? (1 - momentum) g + momentum m : m;
+ *   w <- (1 - lr weight_decay) w - lr scale orthogonalize(u).
+ * Same workspace and limits as mtaz_orthogonalize. */
+int mtaz_muon_step(int device, int n, int64_t rows, int64_t cols, int dtype, void* const* d_params,
+                   const void* const* d_grads, float* const* d_momenta, double lr, double momentum, int nesterov,
+                   double weight_decay, double scale, int steps, const double* coefficients, double eps, void* d_work,
+                   int64_t work_bytes, void* stream);
+
+/* What the logits operators share.  d_legal: packed masks (bit v & 31 of word v >> 5, the layout
+ * mtaz_legal_batch writes), one row per row of logits or legal_stride 0 for one shared row; NULL =
+ * everything is legal.  d_bias: float32, likewise (bias_stride 0 = shared).  d_actions: the actions
+ * taken so far, row b's first d_lengths[b] (NULL: `history`) entries count, entries outside
+ * [0, cols) do not.  Penalties {repetition, frequency, presence}: the host triple, or one triple per
+ * row in d_penalties.  Strides are in elements (words for d_legal); cols <= 2^24.
+ *
+ * Adjusted logits y (same type; d_out may be d_logits with the same stride): with c = how often v
+ * was taken in the row, x <- c ? (x > 0 ? x / repetition : x repetition) - c frequency - presence : x;
+ * y = x + bias where legal, -inf elsewhere whatever x holds there. */
+int mtaz_adjust_logits(int device, int64_t rows, int64_t cols, int dtype, const void* d_logits, int64_t logits_stride,
+                       void* d_out, int64_t out_stride, const uint32_t* d_legal, int64_t legal_stride,
+                       const float* d_bias, int64_t bias_stride, const int32_t* d_actions, int64_t actions_stride,
+                       int history, const int32_t* d_lengths, const double* penalties, const float* d_penalties,
+                       void* stream);
+/* Its backward pass: d_grad (NULL: not wanted) = d y / d x of the logits times d_grad_out, 0 where
+ * not legal; d_bias_grad (NULL: not wanted) float32, per row, or summed over the rows in a fixed order
+ * when bias_grad_stride is 0.  d_logits is read only where a repetition penalty applies. */
+int64_t mtaz_adjust_logits_grad_workspace(int64_t rows, int64_t cols);
+int mtaz_adjust_logits_grad(int device, int64_t rows, int64_t cols, int dtype, const void* d_grad_out,
+                            int64_t grad_out_stride, const void* d_logits, int64_t logits_stride, void* d_grad,
+                            int64_t grad_stride, float* d_bias_grad, int64_t bias_grad_stride, const uint32_t* d_legal,
+                            int64_t legal_stride, const int32_t* d_actions, int64_t actions_stride, int history,
+                            const int32_t* d_lengths, const double* penalties, const float* d_penalties, void* d_work,
+                            int64_t work_bytes, void* stream);
+
+/* Policy/value loss (exp/learner.py:86-87) over the legal moves: per row
+ *   (value - reward)^2 - sum_v target_v log softmax(logits)_v,   v legal,
+ * and its mean over the rows into *d_loss (float32).  target_dtype: MTAZ_F32 or dtype.  d_value and
+ * d_reward: [rows] float32, or both NULL (no value term).  Masked places are never read into a sum
+ * (infinities and NaN there do not matter), a target of 0 adds nothing, and a row with nothing
+ * legal, or with every legal logit -inf, adds its value term alone.  d_stats [rows][4] float32
+ * receives what mtaz_policy_loss_grad needs.  d_grad / d_value_grad (either may be NULL) receive
+ * the gradients of scale * loss in the same call. */
+int64_t mtaz_policy_loss_workspace(int64_t rows, int64_t cols);
+int mtaz_policy_loss(int device, int64_t rows, int64_t cols, int dtype, int target_dtype, const void* d_logits,
+                     int64_t logits_stride, const void* d_target, int64_t target_stride, const uint32_t* d_legal,
+                     int64_t legal_stride, const float* d_value, const float* d_reward, float* d_loss, float* d_stats,
+                     void* d_grad, int64_t grad_stride, float* d_value_grad, double scale, void* d_work,
+                     int64_t work_bytes, void* stream);
+/* The gradients of the mean loss times the device scalar *d_grad_out, from an earlier call's d_stats
+ * on the same inputs. */
+int mtaz_policy_loss_grad(int device, int64_t rows, int64_t cols, int dtype, int target_dtype, const void* d_logits,
+                          int64_t logits_stride, const void* d_target, int64_t target_stride, const uint32_t* d_legal,
+                          int64_t legal_stride, const float* d_value, const float* d_reward, const float* d_stats,
+                          const float* d_grad_out, void* d_grad, int64_t grad_stride, float* d_value_grad,
+                          void* stream);
+
 /* ---- engine ------------------------------------------------------------------------- */
 typedef struct mtaz_engine mtaz_engine;
 

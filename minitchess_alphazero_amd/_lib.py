@@ -43,6 +43,25 @@ SIGNATURES = {
     'mtaz_encode_batch': (c_int, [c_int, c_void_p, c_int, c_void_p, c_void_p, c_void_p]),
     'mtaz_replay_put': (c_int, [c_int, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int64,
                                   c_int64, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p]),
+    'mtaz_orthogonalize_workspace': (c_int64, [c_int, c_int64, c_int64, c_int]),
+    'mtaz_orthogonalize': (c_int, [c_int, c_int, c_int64, c_int64, c_int, POINTER(c_void_p), POINTER(c_void_p), c_int,
+                                   P_f64, c_double, c_void_p, c_int64, c_void_p]),
+    'mtaz_muon_step': (c_int, [c_int, c_int, c_int64, c_int64, c_int, POINTER(c_void_p), POINTER(c_void_p),
+                               POINTER(c_void_p), c_double, c_double, c_int, c_double, c_double, c_int, P_f64, c_double,
+                               c_void_p, c_int64, c_void_p]),
+    'mtaz_adjust_logits': (c_int, [c_int, c_int64, c_int64, c_int, c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int64,
+                                   c_void_p, c_int64, c_void_p, c_int64, c_int, c_void_p, P_f64, c_void_p, c_void_p]),
+    'mtaz_adjust_logits_grad_workspace': (c_int64, [c_int64, c_int64]),
+    'mtaz_adjust_logits_grad': (c_int, [c_int, c_int64, c_int64, c_int, c_void_p, c_int64, c_void_p, c_int64, c_void_p,
+                                        c_int64, c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int64, c_int, c_void_p,
+                                        P_f64, c_void_p, c_void_p, c_int64, c_void_p]),
+    'mtaz_policy_loss_workspace': (c_int64, [c_int64, c_int64]),
+    'mtaz_policy_loss': (c_int, [c_int, c_int64, c_int64, c_int, c_int, c_void_p, c_int64, c_void_p, c_int64, c_void_p,
+                                 c_int64, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_void_p, c_double,
+                                 c_void_p, c_int64, c_void_p]),
+    'mtaz_policy_loss_grad': (c_int, [c_int, c_int64, c_int64, c_int, c_int, c_void_p, c_int64, c_void_p, c_int64, c_void_p,
+                                      c_int64, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_void_p,
+                                      c_void_p]),
     'mtaz_create': (c_void_p, [c_int, c_int, c_int, c_double, c_int, c_double, c_double, c_uint64, c_int, c_uint32, c_int]),
     'mtaz_destroy': (None, [c_void_p]),
     'mtaz_set_weights': (c_int, [c_void_p, POINTER(c_void_p), P_i64, c_int]),

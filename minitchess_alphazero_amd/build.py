@@ -2,8 +2,8 @@
 
 Translation units: csrc/mtaz_device.hip (tree kernels + launchers), csrc/mtaz_net16.hip and
 csrc/mtaz_net8.hip (network kernels k_net_y, k_net_z), csrc/mtaz_host.cpp (C ABI, numpy-legacy
-RNG compiled with -ffp-contract=off, engine driver) and csrc/mtaz_wire.cpp (episode wire
-format).  The shared object lands next to this file so it travels to the GPU box with the repo
+RNG compiled with -ffp-contract=off, engine driver), csrc/mtaz_wire.cpp (episode wire
+format), csrc/mtaz_muon.hip and csrc/mtaz_logits.hip (the learner's operators).  The shared object lands next to this file so it travels to the GPU box with the repo
 snapshot.  build(diag=True) makes libmtaz_diag.so with -DMTAZ_NET_DIAG: the network kernels'
 A/B and timing-only variants and round 3's k_net_y (csrc/mtaz_net16_r3.hip, variant 3; the
 round-3 comparison tests load it in a child process), never loaded by the product path.
@@ -27,6 +27,8 @@ BUILD_DIAG = os.path.join(HERE, '_build_diag')
 INCLUDE = os.path.join(os.path.dirname(HERE), 'include')
 ARCH = os.environ.get('MTAZ_OFFLOAD_ARCH', 'gfx950')
 
+NO_PACKED_FP32 = ['-Xclang', '-target-feature', '-Xclang', '-packed-fp32-ops']
+
 SOURCES = [
     ('mtaz_device.hip', ['-O3']),
     # the network kernels' K loops are unrolled by pragma; above LLVM's default pragma threshold
@@ -40,10 +42,13 @@ SOURCES = [
     # numpy's legacy RNG on the device (k_noise, k_choose; glibc's log/pow ported in glibc_math.h,
     # every FMA explicit, no contraction)
     ('mtaz_rng.hip', ['-O3', '-ffp-contract=off', '-fno-fast-math']),
+    # the learner's operators; without the packed fp32 instructions, whose forms are not all reliable
+    ('mtaz_muon.hip', ['-O3'] + NO_PACKED_FP32),
+    ('mtaz_logits.hip', ['-O3'] + NO_PACKED_FP32),
     ('mtaz_host.cpp', ['-O2', '-ffp-contract=off', '-fno-fast-math']),
     ('mtaz_wire.cpp', ['-O2']),
 ]
-HEADERS = ['rules.h', 'engine.h', 'net_common.h', 'glibc_math.h', 'glibc_math_tables.h']
+HEADERS = ['rules.h', 'engine.h', 'ops.h', 'net_common.h', 'glibc_math.h', 'glibc_math_tables.h']
 
 
 def _hipcc():

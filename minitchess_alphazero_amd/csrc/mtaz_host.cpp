@@ -27,6 +27,7 @@
 
 #include "../../include/mtaz.h"
 #include "engine.h"
+#include "ops.h"
 
 using namespace mtaz;
 
@@ -42,6 +43,7 @@ static int set_err(int code, const char* fmt, ...) {
   g_err = buf;
   return code;
 }
+int mtaz::ops_error(int code, const char* what, const char* why) { return set_err(code, "%s: %s", what, why); }
 #define HIPCHK(x)                                                                            \
   do {                                                                                       \
     hipError_t e_ = (x);                                                                     \

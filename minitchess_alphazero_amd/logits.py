@@ -1,0 +1,276 @@
+"""Operators on action logits [rows, cols], on hand-written HIP kernels (csrc/mtaz_logits.hip).
+
+    adjust_logits           penalties for repeated actions, a bias and a legal-move mask; differentiable
+    policy_value_loss       the learner's loss (exp/learner.py:86-87) over the legal moves; differentiable
+    policy_value_loss_grad  that loss and its gradients in one call
+    legal_masks             the packed legal masks of positions (mtaz_legal_batch)
+
+A mask is packed 32 actions a word: action v is legal where bit v & 31 of word v >> 5 is set, int32
+[rows, ceil(cols / 32)], or [1, words] / [words] for one mask that all rows share.  Logits are float32,
+float16 or bfloat16, sums are float32, and the operators enqueue on the current stream without a
+synchronization; they may be captured in a HIP graph.  There is no CPU form: tensors elsewhere are refused.
+"""
+import ctypes
+
+import torch
+from torch.autograd.function import once_differentiable
+
+from . import _lib
+from .environment import MOVE_CAP, RULES_FLAGS
+from .optim import TYPES, _check_type, _stream
+
+
+def _ptr(t):
+    return None if t is None else t.data_ptr()
+
+
+def _unit(t):
+    """t with its last dimension dense (a copy where it is not)."""
+    return t if t is None or t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
+
+
+def _row_stride(t, shared=False):
+    """Elements from one row to the next; 0 where one row serves all."""
+    return 0 if t is None or shared or t.dim() == 1 or t.shape[0] == 1 else t.stride(0)
+
+
+def _check_rows(t, what, like, shapes, dtypes):
+    if t.device != like.device:
+        raise ValueError(f'{what} must be on {like.device}, not on {t.device}')
+    if t.dtype not in dtypes:
+        raise ValueError(f'{what} must be {" or ".join(str(d) for d in dtypes)}, not {t.dtype}')
+    if tuple(t.shape) not in shapes:
+        raise ValueError(f'{what} has shape {tuple(t.shape)}, expected {" or ".join(str(s) for s in shapes)}')
+
+
+def _check_logits(logits):
+    _check_type(logits, 'logits')
+    if logits.dim() != 2 or logits.shape[1] == 0:
+        raise ValueError(f'logits must be [rows, cols], got {tuple(logits.shape)}')
+
+
+def _check_legal(legal, logits):
+    if legal is not None:
+        rows, words = logits.shape[0], (logits.shape[1] + 31) // 32
+        _check_rows(legal, 'legal', logits, {(rows, words), (1, words), (words,)}, (torch.int32, torch.uint32))
+
+
+def legal_masks(positions, device, rules_flags=RULES_FLAGS, move_cap=MOVE_CAP):
+    """Packed legal masks [n, 18] int32 of packed positions [n, 5] (host uint32 or device int32): what
+    mtaz_legal_batch finds (it waits for the stream, unlike the other functions here).  A position with no
+    legal move has an empty mask."""
+    import numpy as np
+    dev = torch.device(device)
+    if not torch.is_tensor(positions):
+        positions = torch.from_numpy(np.ascontiguousarray(positions, np.uint32).view(np.int32)).to(dev)
+    if positions.dim() != 2 or positions.shape[1] != 5 or positions.dtype != torch.int32 or positions.device.type != 'cuda':
+        raise ValueError('positions must be [n, 5] 32-bit words')
+    pos = positions.contiguous()
+    n = pos.shape[0]
+    codes = torch.empty((n, _lib.KMAX), dtype=torch.int16, device=pos.device)
+    counts, outcomes = (torch.empty(n, dtype=torch.int32, device=pos.device) for _ in range(2))
+    masks = torch.zeros((n, 18), dtype=torch.int32, device=pos.device)
+    if n:
+        _lib.check(_lib.lib().mtaz_legal_batch(pos.device.index, pos.data_ptr(), n, rules_flags, move_cap, codes.data_ptr(),
+                                               counts.data_ptr(), masks.data_ptr(), outcomes.data_ptr(),
+                                               _stream(pos.device)))
+    return masks
+
+
+# ---- penalties, bias and mask ----------------------------------------------------------------------------
+class _Taken:
+    """The actions taken and their penalties, as the C entries take them."""
+
+    def __init__(self, logits, actions, lengths, repetition, frequency, presence):
+        rows = logits.shape[0]
+        given = (repetition, frequency, presence)
+        self.actions = self.lengths = self.per_row = None
+        self.history = 0
+        if lengths is not None and actions is None:
+            raise ValueError('lengths without actions')
+        tensors = [t for t in given if torch.is_tensor(t)]
+        for t in tensors:
+            _check_rows(t, 'a penalty', logits, {(rows,)}, (torch.float32,))
+            if t.requires_grad and torch.is_grad_enabled():
+                raise ValueError('penalties have no gradient')
+        if not torch.is_tensor(repetition) and not repetition > 0:
+            raise ValueError(f'repetition must be positive, got {repetition}')
+        self.host = (ctypes.c_double * 3)(*[1.0 if torch.is_tensor(t) else float(t) for t in given])
+        self.bends = torch.is_tensor(repetition) or repetition != 1.0   # the slope is not 1 everywhere
+        if actions is None:
+            return
+        if actions.dim() != 2:
+            raise ValueError(f'actions must be [rows, history], got {tuple(actions.shape)}')
+        _check_rows(actions, 'actions', logits, {(rows, actions.shape[1])}, (torch.int32,))
+        if lengths is not None:
+            _check_rows(lengths, 'lengths', logits, {(rows,)}, (torch.int32,))
+            self.lengths = lengths.contiguous()
+        self.actions, self.history = _unit(actions), actions.shape[1]
+        if tensors:
+            self.per_row = torch.stack([t if torch.is_tensor(t) else torch.full((rows,), float(t), device=logits.device)
+                                        for t in given], 1).contiguous()
+
+    def args(self):
+        return (_ptr(self.actions), 0 if self.actions is None else self.actions.stride(0), self.history,
+                _ptr(self.lengths), self.host, _ptr(self.per_row))
+
+
+def _adjust(logits, legal, bias, taken, out):
+    x = _unit(logits)
+    rows, cols = x.shape
+    legal, bias = _unit(legal), _unit(bias)
+    _lib.check(_lib.lib().mtaz_adjust_logits(
+        x.device.index, rows, cols, TYPES[x.dtype], x.data_ptr(), x.stride(0), out.data_ptr(), out.stride(0),
+        _ptr(legal), _row_stride(legal), _ptr(bias), _row_stride(bias), *taken.args(), _stream(x.device)))
+    return out
+
+
+class _Adjust(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logits, bias, legal, taken):
+        ctx.taken, ctx.shape, ctx.dtype = taken, logits.shape, logits.dtype
+        ctx.bias_shape = None if bias is None else bias.shape
+        keep = logits if taken.bends and taken.actions is not None else None
+        ctx.save_for_backward(keep, legal, taken.actions, taken.lengths)
+        return _adjust(logits, legal, bias, taken, torch.empty(logits.shape, dtype=logits.dtype, device=logits.device))
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, grad):
+        x, legal, _, _ = ctx.saved_tensors   # raises where actions or lengths were changed in between
+        g, x, legal = _unit(grad), _unit(x), _unit(legal)
+        rows, cols = ctx.shape
+        dx = db = work = None
+        shared = False
+        if ctx.needs_input_grad[0]:
+            dx = torch.empty(ctx.shape, dtype=ctx.dtype, device=g.device)
+        if ctx.needs_input_grad[1]:
+            db = torch.empty(ctx.bias_shape, dtype=torch.float32, device=g.device)
+            shared = len(ctx.bias_shape) == 1 or ctx.bias_shape[0] == 1
+            if shared:
+                size = _lib.check(_lib.lib().mtaz_adjust_logits_grad_workspace(rows, cols))
+                work = torch.empty(max(size, 1), dtype=torch.uint8, device=g.device)
+        t = ctx.taken
+        taken = t.args() if x is not None else (None, 0, 0, None, t.host, None)   # the slope is 1 everywhere
+        _lib.check(_lib.lib().mtaz_adjust_logits_grad(
+            g.device.index, rows, cols, TYPES[ctx.dtype], g.data_ptr(), g.stride(0), _ptr(x),
+            0 if x is None else x.stride(0), _ptr(dx), cols, _ptr(db), 0 if shared else cols, _ptr(legal),
+            _row_stride(legal), *taken, _ptr(work), 0 if work is None else work.numel(), _stream(g.device)))
+        return dx, db, None, None
+
+
+def adjust_logits(logits, legal=None, bias=None, actions=None, lengths=None, repetition=1.0, frequency=0.0,
+                  presence=0.0, out=None):
+    """Logits a policy is to answer with.  With c = how often the row has taken action v:
+
+        x <- x / repetition if x > 0 else x * repetition, then x - c frequency - presence   (where c > 0)
+        y  = x + bias where v is legal, -inf elsewhere (whatever x holds there)
+
+    legal: packed masks (see the module).  bias: float32 [cols], [1, cols] or [rows, cols].  actions: int32
+    [rows, history], of which the first lengths[row] (int32; None: all) count; entries outside [0, cols) (a
+    padding of -1, say) do not.  The penalties are numbers or float32 tensors [rows]; repetition must be
+    positive.  Where logits or bias require a gradient the result is differentiable; the gradient of a bias that the
+    rows share is summed over them in a fixed order.  out (logits itself is allowed): not with gradients."""
+    _check_logits(logits)
+    rows, cols = logits.shape
+    _check_legal(legal, logits)
+    if bias is not None:
+        _check_rows(bias, 'bias', logits, {(cols,), (1, cols), (rows, cols)}, (torch.float32,))
+    taken = _Taken(logits, actions, lengths, repetition, frequency, presence)
+    if torch.is_grad_enabled() and (logits.requires_grad or (bias is not None and bias.requires_grad)):
+        if out is not None:
+            raise ValueError('out is not supported where a gradient is required')
+        return _Adjust.apply(logits, bias, legal, taken)
+    if out is None:
+        out = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
+    else:
+        if out.shape != logits.shape or out.dtype != logits.dtype or out.device != logits.device:
+            raise ValueError('out must have the shape, type and device of logits')
+        if (cols > 1 and out.stride(1) != 1) or (rows > 1 and out.stride(0) < cols):
+            raise ValueError('out must have dense rows that do not overlap')
+        if torch.is_grad_enabled() and out.requires_grad:
+            raise ValueError('out must not require a gradient')
+    _adjust(logits.detach(), legal, bias, taken, out)
+    torch.autograd.graph.increment_version(out)
+    return out
+
+
+# ---- policy/value loss -------------------------------------------------------------------------------------
+def _check_loss(logits, target, value, reward, legal):
+    _check_logits(logits)
+    rows, cols = logits.shape
+    if rows == 0:
+        raise ValueError('the mean loss of no rows')
+    _check_rows(target, 'target', logits, {(rows, cols)}, (torch.float32, logits.dtype))
+    if (value is None) != (reward is None):
+        raise ValueError('value and reward come together')
+    for t, what in ((value, 'value'), (reward, 'reward')):
+        if t is not None:
+            _check_rows(t, what, logits, {(rows,), (rows, 1)}, (torch.float32,))
+    _check_legal(legal, logits)
+    if torch.is_grad_enabled() and (target.requires_grad or (reward is not None and reward.requires_grad)):
+        raise ValueError('target and reward have no gradient')
+
+
+def _loss(logits, target, value, reward, legal, grad, value_grad, scale):
+    z, t, legal = _unit(logits), _unit(target), _unit(legal)
+    rows, cols = z.shape
+    dev = z.device
+    value, reward = (None if x is None else x.reshape(-1).contiguous() for x in (value, reward))
+    loss = torch.empty((), dtype=torch.float32, device=dev)
+    stats = torch.empty((rows, 4), dtype=torch.float32, device=dev)
+    work = torch.empty(_lib.check(_lib.lib().mtaz_policy_loss_workspace(rows, cols)), dtype=torch.uint8, device=dev)
+    _lib.check(_lib.lib().mtaz_policy_loss(
+        dev.index, rows, cols, TYPES[z.dtype], TYPES[t.dtype], z.data_ptr(), z.stride(0), t.data_ptr(), t.stride(0),
+        _ptr(legal), _row_stride(legal), _ptr(value), _ptr(reward), loss.data_ptr(), stats.data_ptr(), _ptr(grad), cols,
+        _ptr(value_grad), float(scale), work.data_ptr(), work.numel(), _stream(dev)))
+    return loss, stats
+
+
+class _PolicyValueLoss(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logits, value, target, reward, legal):
+        loss, stats = _loss(logits, target, value, reward, legal, None, None, 1.0)
+        ctx.save_for_backward(logits, value, target, reward, legal, stats)
+        return loss
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, grad):
+        logits, value, target, reward, legal, stats = ctx.saved_tensors
+        z, t, legal = _unit(logits), _unit(target), _unit(legal)
+        rows, cols = z.shape
+        flat, reward = (None if x is None else x.reshape(-1).contiguous() for x in (value, reward))
+        dz = torch.empty(z.shape, dtype=z.dtype, device=z.device) if ctx.needs_input_grad[0] else None
+        dv = torch.empty(value.shape, device=z.device) if value is not None and ctx.needs_input_grad[1] else None
+        _lib.check(_lib.lib().mtaz_policy_loss_grad(
+            z.device.index, rows, cols, TYPES[z.dtype], TYPES[t.dtype], z.data_ptr(), z.stride(0), t.data_ptr(),
+            t.stride(0), _ptr(legal), _row_stride(legal), _ptr(flat), _ptr(reward), stats.data_ptr(), grad.data_ptr(),
+            _ptr(dz), cols, _ptr(dv), _stream(z.device)))
+        return dz, dv, None, None, None
+
+
+def policy_value_loss(logits, target, value=None, reward=None, legal=None):
+    """The mean over the rows of (value - reward)^2 - sum over the legal v of target_v log softmax(logits)_v
+    (exp/learner.py:86-87, where every action counts as legal), a float32 scalar.
+
+    target: float32 or of the logits' type; it need not sum to 1.  value, reward: float32 [rows] or [rows, 1],
+    or neither.  Masked places do not matter, whatever they hold (an output of adjust_logits needs no mask),
+    a target of 0 adds nothing, and a row with nothing legal, or with every legal logit at -inf, adds its value term
+    alone.  Differentiable in logits and value."""
+    _check_loss(logits, target, value, reward, legal)
+    if torch.is_grad_enabled() and (logits.requires_grad or (value is not None and value.requires_grad)):
+        return _PolicyValueLoss.apply(logits, value, target, reward, legal)
+    return _loss(logits, target, value, reward, legal, None, None, 1.0)[0]
+
+
+@torch.no_grad()
+def policy_value_loss_grad(logits, target, value=None, reward=None, legal=None, scale=1.0):
+    """policy_value_loss and the gradients of scale * loss, from one pass: (loss, d logits, d value or None),
+    for torch.autograd.backward((logits, value), (d logits, d value)).  With 16-bit logits a scale keeps
+    small gradients in range."""
+    _check_loss(logits, target, value, reward, legal)
+    dz = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
+    dv = None if value is None else torch.empty(value.shape, dtype=torch.float32, device=logits.device)
+    loss, _ = _loss(logits, target, value, reward, legal, dz, dv, scale)
+    return loss, dz, dv
