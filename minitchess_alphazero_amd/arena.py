@@ -52,6 +52,56 @@ def arena(engine, new_net, old_net, seed_base=0):
     return out
 
 
+def policy_match(new_net, old_net, games, device=0, seed=0, tau_change=6, repetition=1.0, frequency=0.0, presence=0.0):
+    """New against old without search: every move is the mover's policy over its legal moves, sampled before
+    fullmove tau_change and the likeliest one after (the schedule of exp/agent.py:114-118), in `games` games
+    per side at once.  The penalties (logits.adjust_logits) weigh down actions the player has already
+    taken in the game; 1, 0, 0 leave the policy as it is.  Returns arena()'s counts and score."""
+    import torch
+
+    from .engine import Engine
+    from .environment import STARTING_FEN
+    from .logits import adjust_logits, legal_masks
+    dev = torch.device('cuda', device)
+    rng = torch.Generator(device=dev).manual_seed(seed)
+    engines = [Engine(n_games=games, sims=1, device=device) for _ in range(2)]   # the new and the old network
+    out = {'new_wins': 0, 'old_wins': 0, 'draws': 0, 'games': 0}
+    try:
+        for eng, net in zip(engines, (new_net, old_net)):
+            eng.set_weights(net)
+        board = engines[0]                                        # which also holds the games
+        for side in range(2):                                     # new first, then new second
+            board.set_games([STARTING_FEN] * games)
+            taken = [torch.empty((games, 0), dtype=torch.int32, device=dev) for _ in range(2)]   # by player
+            pos, _, active, _ = board.games()
+            ply = 0
+            while active.any():
+                player = ply % 2
+                live = active.astype(bool)
+                logits, _ = engines[player ^ side].evaluate_tensors(pos)
+                adjust_logits(logits, legal=legal_masks(pos, dev), actions=taken[player], repetition=repetition,
+                              frequency=frequency, presence=presence, out=logits)
+                logits[torch.from_numpy(~live).to(dev)] = 0.0     # a finished game may have nothing legal
+                if int(pos[live][0][4]) >> 16 < tau_change:       # the games move in lockstep
+                    action = torch.multinomial(torch.softmax(logits, 1), 1, generator=rng)
+                else:
+                    action = logits.argmax(1, keepdim=True)
+                taken[player] = torch.cat([taken[player], action.to(torch.int32)], 1)
+                board.apply(action[:, 0].cpu().numpy())
+                pos, _, active, outcome = board.games()
+                ended = live & ~active.astype(bool)
+                won = int(np.sum(outcome[ended] == DECISIVE))
+                out['new_wins' if player == side else 'old_wins'] += won   # the last mover's (exp/callbacks.py:19-22)
+                out['draws'] += int(ended.sum()) - won
+                out['games'] += int(ended.sum())
+                ply += 1
+    finally:
+        for eng in engines:
+            eng.close()
+    out['score'] = out['new_wins'] / (out['new_wins'] + out['old_wins'] + 1e-8)
+    return out
+
+
 def gate(score, threshold=GATE):
     """Keep the new network when it scored above the threshold (app/base.py:195-196)."""
     return score > threshold

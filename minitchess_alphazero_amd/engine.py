@@ -84,6 +84,11 @@ class Engine:
 
     def evaluate(self, positions):
         """Network.forward on packed positions [n,5] -> (logits [n,554], values [n]) (numpy)."""
+        logits, values = self.evaluate_tensors(positions)
+        return logits.cpu().numpy(), values.cpu().numpy()
+
+    def evaluate_tensors(self, positions):
+        """evaluate, with the results left on the device."""
         import torch
         dev = torch.device('cuda', self.device)
         pos = torch.from_numpy(np.ascontiguousarray(positions, np.uint32).view(np.int32)).to(dev)
@@ -93,7 +98,7 @@ class Engine:
         torch.cuda.synchronize(dev)
         _lib.check(self.L.mtaz_evaluate(self.h, c_void_p(pos.data_ptr()), n, c_void_p(logits.data_ptr()),
                                         c_void_p(values.data_ptr())))
-        return logits.cpu().numpy(), values.cpu().numpy()
+        return logits, values
 
     def net_exponents(self, positions):
         """k_net_y's stored-units exponents on packed positions [n,5], from one launch of the

@@ -16,6 +16,10 @@ reference's signature and output for callers that use a DataLoader themselves.
 
 MQTT / HTTP transport (app/learner.py) is out of scope (SURVEY 8f: wire formats are rank 3);
 LearnPuppet keeps the state machine, the dataset and the versioned weights.
+
+Two options the reference does not have, both off by default and both on the GPU only: optimizer='muon'
+trains the trunk's convolutions with Muon (optim.py) and everything else with AdamW, and legal_mask=True
+takes the policy's softmax over the legal moves instead of all 554 (logits.policy_value_loss_grad).
 """
 import copy
 import ctypes
@@ -91,10 +95,17 @@ def encode_positions(pos, device):
     return tok.long().reshape(n, 2, 6, 5), clk.reshape(n, 1)
 
 
-class ResidentBatches:
-    """A dataset encoded once and kept on the device; batches are index gathers."""
+def _masks_of(pos, device):
+    """Packed legal masks [n, 18] int32 of packed positions (host or device)."""
+    from .logits import legal_masks
+    return legal_masks(pos, device)
 
-    def __init__(self, rows, device):
+
+class ResidentBatches:
+    """A dataset encoded once and kept on the device; batches are index gathers.  legal_masks (GPU
+    only): keep the positions' packed legal masks too."""
+
+    def __init__(self, rows, device, legal_masks=False):
         self.device = torch.device(device)
         if isinstance(rows, EpisodeRecords):
             pos, pi, reward = rows.pos, rows.pi_dense(), rows.reward
@@ -108,6 +119,7 @@ class ResidentBatches:
             enc = [pos_encode(p) for p in pos]
             self.tokens = torch.from_numpy(np.stack([t for t, _ in enc])).reshape(-1, 2, 6, 5)
             self.clock = torch.tensor(np.asarray([c for _, c in enc], np.float32)).reshape(-1, 1)
+        self.legal = _masks_of(pos, self.device) if legal_masks else None
         self.pi = torch.from_numpy(pi).to(self.device)
         self.reward = torch.from_numpy(np.ascontiguousarray(reward, np.float32)).reshape(-1, 1).to(self.device)
 
@@ -117,6 +129,10 @@ class ResidentBatches:
     def gather(self, i):
         """Rows at the device index tensor i (capturable in a HIP graph)."""
         return self.pi[i], self.tokens[i], self.clock[i], self.reward[i]
+
+    def gather_legal(self, i):
+        """The packed legal masks of rows i."""
+        return self.legal[i]
 
     def batch(self, idx):
         return self.gather(torch.as_tensor(idx, dtype=torch.long, device=self.device))
@@ -136,9 +152,12 @@ class ReplayBuffer:
 
     ROW_BYTES = 60 + 4 + 4 * NUM_ACTIONS + 4
 
-    def __init__(self, max_length, device, initial=1 << 16):
+    def __init__(self, max_length, device, initial=1 << 16, legal_masks=False):
+        """legal_masks: keep each row's packed legal mask as well (72 B a row)."""
         self.max_length = int(max_length)
         self.device = torch.device(device)
+        self.legal_masks = bool(legal_masks)
+        self._legal = None
         if self.device.type != 'cuda':
             raise RuntimeError('ReplayBuffer lives in GPU memory (HIP ingest kernel); use '
                                'SimpleAlphaZeroDataset / ResidentBatches on the host')
@@ -152,11 +171,15 @@ class ReplayBuffer:
         new = (torch.zeros((cap, 60), dtype=torch.uint8, device=dev), torch.zeros(cap, dtype=torch.float32, device=dev),
                torch.zeros((cap, NUM_ACTIONS), dtype=torch.float32, device=dev),
                torch.zeros(cap, dtype=torch.float32, device=dev))
+        legal = torch.zeros((cap, 18), dtype=torch.int32, device=dev) if self.legal_masks else None
         if self.size:
             order = (torch.arange(self.size, device=dev) + self.head) % self.cap
             for dst, src in zip(new, (self._tokens, self._clock, self._pi, self._reward)):
                 dst[:self.size] = src[order]
+            if legal is not None:
+                legal[:self.size] = self._legal[order]
         self._tokens, self._clock, self._pi, self._reward = new
+        self._legal = legal
         self.cap, self.head = cap, 0
 
     def __len__(self):
@@ -191,6 +214,8 @@ class ReplayBuffer:
         if self.size + n > self.cap and self.cap < self.max_length:
             self._alloc(min(self.max_length, max(2 * self.cap, self.size + n)))
         tail = (self.head + self.size) % self.cap
+        if self.legal_masks:
+            self._legal[(torch.arange(n, device=self.device) + tail) % self.cap] = _masks_of(pos, self.device)
         args = [c.contiguous() for c in (pos, k, e0, codes, visits, reward)]
         _lib.check(_lib.lib().mtaz_replay_put(
             self.device.index or 0, n, *[a.data_ptr() for a in args], self.cap, tail,
@@ -220,6 +245,8 @@ class ReplayBuffer:
         self._tokens[slots] = tok.reshape(n, 60).to(torch.uint8)
         self._clock[slots] = clk.reshape(n)
         self._pi[slots] = pi
+        if self.legal_masks:
+            self._legal[slots] = _masks_of(pos, dev)
         self._reward[slots] = rew
         over = max(0, self.size + n - self.cap)
         self.size = min(self.cap, self.size + n)
@@ -231,6 +258,10 @@ class ReplayBuffer:
         j = (i + self.head) % self.cap if self.head else i
         return (self._pi[j], self._tokens[j].long().reshape(-1, 2, 6, 5), self._clock[j].reshape(-1, 1),
                 self._reward[j].reshape(-1, 1))
+
+    def gather_legal(self, i):
+        """The packed legal masks of rows i."""
+        return self._legal[(i + self.head) % self.cap if self.head else i]
 
     def batch(self, idx):
         return self.gather(torch.as_tensor(idx, dtype=torch.long, device=self.device))
@@ -336,9 +367,23 @@ def alphazero_loss(model, pib, tokens, clock, reward):
     return ((v - reward) ** 2 - (pib * p.log_softmax(-1)).sum(1)).mean()
 
 
+def muon_split(network):
+    """(the weights Muon trains: the trunk's convolutions; all other parameters)"""
+    trunk = {id(p) for n, p in network.named_parameters() if n.startswith('resbody.') and p.dim() == 4}
+    params = list(network.parameters())
+    return [p for p in params if id(p) in trunk], [p for p in params if id(p) not in trunk]
+
+
 # ---- learner (exp/learner.py:62-91) ------------------------------------------------------------------
 class SimpleAlphaZeroLearner:
-    def __init__(self, env, num_simulations, network, batch_size, epochs, optim_params, device=None):
+    def __init__(self, env, num_simulations, network, batch_size, epochs, optim_params, device=None,
+                 optimizer='adamw', muon_params=None, legal_mask=False):
+        """optimizer: 'adamw' (the reference's) or 'muon' (optim.Muon(**muon_params) on muon_split's first
+        part, AdamW(**optim_params) on the rest); legal_mask: the policy loss over the legal moves."""
+        if optimizer not in ('adamw', 'muon'):
+            raise ValueError(f"optimizer must be 'adamw' or 'muon', not {optimizer!r}")
+        if muon_params is not None and optimizer != 'muon':
+            raise ValueError("muon_params without optimizer='muon'")
         self._env = env
         self._num_simulations = num_simulations
         self._network = network
@@ -347,7 +392,33 @@ class SimpleAlphaZeroLearner:
         self._optim_params = dict(optim_params)
         self._device = torch.device(device) if device is not None else \
             torch.device('cuda', torch.cuda.current_device()) if torch.cuda.is_available() else torch.device('cpu')
+        self._optimizer, self._muon_params = optimizer, dict(muon_params or {})
+        self._legal_mask = bool(legal_mask)
+        if self._device.type != 'cuda' and (optimizer == 'muon' or legal_mask):
+            raise RuntimeError("optimizer='muon' and legal_mask run on HIP kernels: they need a GPU")
         self.last_losses = []
+
+    def _optimizers(self, model, capturable):
+        params, out = model.parameters(), []
+        if self._optimizer == 'muon':
+            from .optim import Muon
+            matrices, params = muon_split(model)
+            out.append(Muon(matrices, **self._muon_params))
+        out.append(torch.optim.AdamW(params, **self._optim_params, **({'capturable': True} if capturable else {})))
+        return out
+
+    def _backward(self, model, data, idx):
+        """Forward, loss and backward on the rows at the device index tensor idx; the detached loss."""
+        pib, tok, clk, rew = data.gather(idx)
+        if not self._legal_mask:
+            loss = alphazero_loss(model, pib, tok, clk, rew)
+            loss.backward()
+            return loss.detach()
+        from .logits import policy_value_loss_grad
+        p, v = model((tok, clk))
+        loss, dp, dv = policy_value_loss_grad(p.detach(), pib, v.detach(), rew, legal=data.gather_legal(idx))
+        torch.autograd.backward((p, v), (dp, dv))
+        return loss
 
     def update(self, dataset):
         """One learner update over `dataset` (rows, SimpleAlphaZeroDataset or EpisodeRecords).
@@ -361,15 +432,16 @@ class SimpleAlphaZeroLearner:
         step count on the device).  A partial last batch runs eagerly."""
         model = self._network.train().to(self._device)
         if isinstance(dataset, ReplayBuffer):
+            if self._legal_mask and not dataset.legal_masks:
+                raise ValueError('legal_mask needs a ReplayBuffer with legal_masks=True')
             data = dataset
         else:
             rows = dataset if isinstance(dataset, EpisodeRecords) else \
                 dataset.get_memory() if hasattr(dataset, 'get_memory') else list(dataset)
-            data = ResidentBatches(rows, self._device)
+            data = ResidentBatches(rows, self._device, legal_masks=self._legal_mask)
         use_graph = self.graphs and self._device.type == 'cuda' and len(data) >= self._batch_size
-        optimizer = torch.optim.AdamW(model.parameters(), **self._optim_params,
-                                      **({'capturable': True} if use_graph else {}))
-        step = self._graph_step(model, optimizer, data) if use_graph else None
+        optimizers = self._optimizers(model, use_graph)
+        step = self._graph_step(model, optimizers, data) if use_graph else None
         metric = AvgSmoothLoss().reset()
         losses = []
         for epoch in range(self._epochs):
@@ -380,12 +452,12 @@ class SimpleAlphaZeroLearner:
                 if step is not None and len(idx) == self._batch_size:
                     pending.append(step(idx))
                     continue
-                pib, tok, clk, rew = data.batch(idx)
-                loss = alphazero_loss(model, pib, tok, clk, rew)
-                optimizer.zero_grad()
-                loss.backward()
-                pending.append(loss.detach().clone())
-                optimizer.step()
+                for o in optimizers:
+                    o.zero_grad()
+                loss = self._backward(model, data, torch.as_tensor(idx, dtype=torch.long, device=self._device))
+                pending.append(loss.clone())
+                for o in optimizers:
+                    o.step()
             for lt in torch.stack(pending).tolist() if pending else []:   # one sync per epoch
                 metric.accumulate(lt)
                 losses.append(lt)
@@ -396,19 +468,21 @@ class SimpleAlphaZeroLearner:
     graphs = True
 
     def _graph_step(self, model, optimizer, data):
-        """Capture one full-batch training step; returns step(idx) -> loss tensor (a copy)."""
+        """Capture one full-batch training step; returns step(idx) -> loss tensor (a copy).
+        optimizer: one, or a list of them."""
+        optimizers = optimizer if isinstance(optimizer, list) else [optimizer]
         dev = self._device
         static_idx = torch.zeros(self._batch_size, dtype=torch.long, device=dev)
         static_loss = torch.zeros((), dtype=torch.float32, device=dev)
         saved = {k: v.detach().clone() for k, v in model.state_dict().items()}
 
         def body():
-            pib, tok, clk, rew = data.gather(static_idx)
-            loss = alphazero_loss(model, pib, tok, clk, rew)
-            optimizer.zero_grad(set_to_none=False)
-            loss.backward()
-            optimizer.step()
-            static_loss.copy_(loss.detach())
+            for o in optimizers:
+                o.zero_grad(set_to_none=False)
+            loss = self._backward(model, data, static_idx)
+            for o in optimizers:
+                o.step()
+            static_loss.copy_(loss)
 
         static_idx.copy_(torch.arange(self._batch_size, device=dev) % len(data))
         side = torch.cuda.Stream(dev)
@@ -420,11 +494,11 @@ class SimpleAlphaZeroLearner:
         graph = torch.cuda.CUDAGraph()
         with torch.cuda.graph(graph):
             body()
-        # undo the warm-up and capture steps: weights, BN buffers, AdamW moments and step count
+        # undo the warm-up and capture steps: weights, BN buffers, AdamW moments and step count, Muon momenta
         with torch.no_grad():
             for k, v in model.state_dict().items():
                 v.copy_(saved[k])
-            for st in optimizer.state.values():
+            for st in (st for o in optimizers for st in o.state.values()):
                 for t in st.values():
                     if torch.is_tensor(t):
                         t.zero_()
@@ -441,14 +515,16 @@ class SimpleAlphaZeroLearner:
 
 # ---- LearnPuppet (app/base.py:137-205, transport excluded) --------------------------------------------
 class LearnPuppet:
-    def __init__(self, userid, batch_size, epochs, optim_params, device=None, max_length=1_000_000):
+    def __init__(self, userid, batch_size, epochs, optim_params, device=None, max_length=1_000_000, optimizer='adamw',
+                 muon_params=None, legal_mask=False):
         self._userid = userid
         self._max_length = max_length
         self._replay = None
         self._dataset = None
         self._init_dataset()
         self._network = Network()
-        self._learner = SimpleAlphaZeroLearner(None, 36, self._network, batch_size, epochs, optim_params, device)
+        self._learner = SimpleAlphaZeroLearner(None, 36, self._network, batch_size, epochs, optim_params, device,
+                                               optimizer, muon_params, legal_mask)
         self._episode_counter = 0
         self._weights_version = None
         self._weights = None
@@ -495,7 +571,7 @@ class LearnPuppet:
         if self._learner._device.type != 'cuda':
             return None
         if self._replay is None:
-            self._replay = ReplayBuffer(self._max_length, self._learner._device)
+            self._replay = ReplayBuffer(self._max_length, self._learner._device, legal_masks=self._learner._legal_mask)
         return self._replay
 
     def push_data(self, data):

@@ -99,20 +99,26 @@ def arena_round(new_net, old_net, games, sims, dist, device, seed_base, gate_thr
 
 
 def run_loop(iterations, games, sims, batch_size=32, epochs=1, lr=0.2, dist=None, device=0, seed=0,
-             log=print, arena_games=0, gate_threshold=0.55, on_iteration=None, starts=None):
+             log=print, arena_games=0, gate_threshold=0.55, on_iteration=None, starts=None, optimizer='adamw',
+             muon_lr=0.02, legal_mask=False, policy_games=0):
     """C5 on this node.  Returns rank 0's per-iteration history (other ranks: []).
     on_iteration(it, net, records, history_entry), rank 0 only, after the weights of
     iteration `it` are in place (tools/train_stress.py measures the network there).
     starts(it, rank, games) -> None (every game from STARTING_FEN, the reference's puppet) or a list
     of `games` FENs to start this iteration's games from (tools/train_stress.py mixes endgame
-    starts in, so that the value targets are not all draws)."""
+    starts in, so that the value targets are not all draws).
+    optimizer / muon_lr / legal_mask: the learner's options (learner.SimpleAlphaZeroLearner).
+    policy_games > 0: rank 0 also plays that many games per side by the policies alone, new network
+    against previous (arena.policy_match); it reports, it does not gate."""
     from .engine import Engine
     rank = dist.get_rank() if dist is not None else 0
     world = dist.get_world_size() if dist is not None else 1
     dev = torch.device('cuda', device)
     torch.manual_seed(seed)
     net = Network()                                   # identical random init on every rank
-    learner = LearnPuppet('learner', batch_size, epochs, {'lr': lr}, device=dev) if rank == 0 else None
+    learner = LearnPuppet('learner', batch_size, epochs, {'lr': lr}, device=dev, optimizer=optimizer,
+                          muon_params={'lr': muon_lr} if optimizer == 'muon' else None,
+                          legal_mask=legal_mask) if rank == 0 else None
     if learner is not None:
         learner.weights = net.state_dict()
     broadcast_weights(net, dist, dev)
@@ -169,6 +175,9 @@ def run_loop(iterations, games, sims, batch_size=32, epochs=1, lr=0.2, dist=None
                  'plies_per_game': st['plies'] / games, 'decisive_frac': st['decisive'] / games}
             if verdict is not None:
                 h['arena'] = verdict
+            if policy_games > 0:
+                from .arena import policy_match
+                h['policy_match'] = policy_match(out['weights'], old_sd, policy_games, device=device, seed=it)
             if on_iteration is not None:
                 on_iteration(it, net, EpisodeRecords.concat(parts), h)
             history.append(h)
@@ -186,6 +195,12 @@ def main(argv=None):
     ap.add_argument('--lr', type=float, default=0.2)
     ap.add_argument('--seed', type=int, default=0)
     ap.add_argument('--arena-games', type=int, default=0, help='arena games per side per GPU (0: no gating)')
+    ap.add_argument('--optimizer', choices=('adamw', 'muon'), default='adamw',
+                    help="muon: the trunk's convolutions with Muon, the rest with AdamW")
+    ap.add_argument('--muon-lr', type=float, default=0.02)
+    ap.add_argument('--legal-mask', action='store_true', help='policy loss over the legal moves only')
+    ap.add_argument('--policy-games', type=int, default=0,
+                    help='games per side of new against previous policy, without search (0: none)')
     ap.add_argument('--gate', type=float, default=0.55)
     ap.add_argument('--save', default='', help='write the final state_dict here (torch.save)')
     args = ap.parse_args(argv)
@@ -200,7 +215,8 @@ def main(argv=None):
         torch.cuda.set_device(local)
         dist.init_process_group('nccl', device_id=torch.device('cuda', local))
     hist, net = run_loop(args.iterations, args.games, args.sims, args.batch, args.epochs, args.lr, dist, local,
-                         args.seed, arena_games=args.arena_games, gate_threshold=args.gate)
+                         args.seed, arena_games=args.arena_games, gate_threshold=args.gate, optimizer=args.optimizer,
+                         muon_lr=args.muon_lr, legal_mask=args.legal_mask, policy_games=args.policy_games)
     if (dist is None or dist.get_rank() == 0) and args.save:
         torch.save(net.state_dict(), args.save)
     if dist is not None:
