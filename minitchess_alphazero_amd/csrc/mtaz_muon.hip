@@ -10,8 +10,10 @@
 // coefficients alone, since the first X has norm at most 1 (bounds()).  Against the f32 matrix instruction
 // (157 TFLOP/s) the split has a third of the f16 rate, about 5 times as much.
 //
-// X, S and B lie in the workspace as hi and lo planes, padded with zeros to whole tiles, so that the product
-// kernel checks no bounds; a padded row or column stays zero through every step.
+// X, S and B lie in the workspace as such pairs: a row is a run of 128-byte lines, each the hi and then the lo
+// halves of 32 consecutive elements, so that one line is what a product reads of a row at a time.  They are padded
+// with zeros to whole tiles, so that the product kernel checks no bounds; a padded row or column stays zero through
+// every step.
 #include "ops.h"
 
 #include <math.h>
@@ -26,8 +28,7 @@ typedef float f32x16 __attribute__((ext_vector_type(16)));
 
 constexpr int NT = 256;
 constexpr int MOST = 64;      // matrices per launch: their pointers travel as kernel arguments
-constexpr int PAD = 64;       // rows and columns of the planes are multiples of it
-constexpr int PARTS = 64;     // workgroups per matrix for the sum of squares
+constexpr int PARTS = 256;    // most workgroups per matrix for the sum of squares
 
 struct Matrices {
   const void* grad[MOST];
@@ -37,20 +38,26 @@ struct Matrices {
 struct Shape {
   int rows, cols;             // of the matrix as it lies in memory
   int r, L;                   // short and long side
-  int rp, Lp;                 // padded
+  int rp, Lp;                 // padded to whole tiles
+  int tile_r, tile_L;         // tile of the products over r x r and over r x L: 64 or 128
+  int parts;                  // workgroups for the sum of squares
 };
 struct Update {
   float momentum, keep, step;   // m <- momentum m + (1 - momentum) g;  w <- keep w - step O
   int nesterov;
 };
-// hi and lo planes of n matrices [rows][pitch], one after the other
-struct Planes {
-  _Float16 *hi, *lo;
-  int64_t each;               // elements of one matrix
-  int pitch;
+// n matrices of pairs, one after the other
+struct Pairs {
+  _Float16* at;
+  int64_t each;               // halves of one matrix
+  int pitch;                  // halves of one row: twice the padded columns
+  // the hi half of (row, col); its lo half lies 32 behind it
+  __device__ __forceinline__ _Float16* hi(int i, int row, int col) const {
+    return at + i * each + (int64_t)row * pitch + (col >> 5) * 64 + (col & 31);
+  }
 };
 
-// ---- the matrix to orthogonalise: sum of squares, then the planes of X -----------------------------------------
+// ---- the matrix to orthogonalise: sum of squares, then the pairs of X -----------------------------------------
 template <int DT, bool MUON>
 __device__ __forceinline__ float update_of(float g, float m, const Update& u) {
   return MUON ? (u.nesterov ? fmaf(u.momentum, m, (1.f - u.momentum) * g) : m) : g;
@@ -60,12 +67,13 @@ __device__ __forceinline__ float update_of(float g, float m, const Update& u) {
 // pass also brings it up to date.
 template <int DT, bool MUON>
 __global__ __launch_bounds__(NT) void k_squares(Matrices ms, int64_t count, Update u, double* part) {
+  const int parts = gridDim.x;
   typedef Elem<DT> E;
   const int i = blockIdx.y;
   const typename E::T* g = (const typename E::T*)ms.grad[i];
   float* mom = ms.momentum[i];
   double s = 0.;
-  for (int64_t k = 4 * ((int64_t)blockIdx.x * NT + threadIdx.x); k < count; k += 4 * NT * PARTS) {
+  for (int64_t k = 4 * ((int64_t)blockIdx.x * NT + threadIdx.x); k < count; k += 4ll * NT * parts) {
     const int n = (int)min((int64_t)4, count - k);
     for (int j = 0; j < n; ++j) {
       const float gv = E::get(g[k + j]);
@@ -82,7 +90,7 @@ __global__ __launch_bounds__(NT) void k_squares(Matrices ms, int64_t count, Upda
   for (int o = 32; o; o >>= 1) s += __shfl_xor(s, o);
   if (threadIdx.x % 64 == 0) ws[threadIdx.x / 64] = s;
   __syncthreads();
-  if (threadIdx.x == 0) part[i * PARTS + blockIdx.x] = (ws[0] + ws[1]) + (ws[2] + ws[3]);
+  if (threadIdx.x == 0) part[i * parts + blockIdx.x] = (ws[0] + ws[1]) + (ws[2] + ws[3]);
 }
 
 __device__ __forceinline__ void split(float x, _Float16& hi, _Float16& lo) {
@@ -90,17 +98,31 @@ __device__ __forceinline__ void split(float x, _Float16& hi, _Float16& lo) {
   lo = (_Float16)(x - (float)hi);
 }
 
-// X = matrix * 2^e / (norm + eps) in planes, transposed where the matrix is tall; 64 x 64 elements per workgroup
+// eight consecutive elements (a multiple of 8 into the row) as pairs
+__device__ __forceinline__ void store_pairs(_Float16* to, const float* x) {
+  f16x8 h, l;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    _Float16 hj, lj;
+    split(x[j], hj, lj);
+    h[j] = hj, l[j] = lj;
+  }
+  *reinterpret_cast<f16x8*>(to) = h;
+  *reinterpret_cast<f16x8*>(to + 32) = l;
+}
+
+// X = matrix * 2^e / (norm + eps) in pairs, transposed where the matrix is tall; 64 x 64 elements per workgroup
 template <int DT, bool MUON>
-__global__ __launch_bounds__(NT) void k_planes(Matrices ms, Shape sh, Update u, const double* part, double eps,
-                                               double unit, Planes X) {
+__global__ __launch_bounds__(NT) void k_pairs(Matrices ms, Shape sh, Update u, const double* part, double eps,
+                                               double unit, Pairs X) {
   typedef Elem<DT> E;
   const int i = blockIdx.z;
   const int r0 = blockIdx.y * 64, c0 = blockIdx.x * 64;   // of X
   __shared__ double inv;
   __shared__ float tile[64][65];
   if (threadIdx.x < 64) {
-    double s = part[i * PARTS + threadIdx.x];
+    double s = 0.;
+    for (int p = threadIdx.x; p < sh.parts; p += 64) s += part[i * sh.parts + p];
     for (int o = 32; o; o >>= 1) s += __shfl_xor(s, o);
     if (threadIdx.x == 0) inv = unit / (sqrt(s) + eps);
   }
@@ -121,73 +143,68 @@ __global__ __launch_bounds__(NT) void k_planes(Matrices ms, Shape sh, Update u, 
   __syncthreads();
   for (int k = threadIdx.x; k < 64 * 8; k += NT) {
     const int a = k >> 3, b = (k & 7) * 8;
-    f16x8 h, l;
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      _Float16 hj, lj;
-      split(tile[a][b + j], hj, lj);
-      h[j] = hj, l[j] = lj;
-    }
-    const int64_t at = i * X.each + (int64_t)(r0 + a) * X.pitch + c0 + b;
-    *reinterpret_cast<f16x8*>(X.hi + at) = h;
-    *reinterpret_cast<f16x8*>(X.lo + at) = l;
+    store_pairs(X.hi(i, r0 + a, c0 + b), &tile[a][b]);
   }
 }
 
 // ---- products --------------------------------------------------------------------------------------------------
-// One workgroup: D[m][n] = sum_k P[m][k] Q[n][k] for a T x T tile, 4 waves of T/2 x T/2 on the 32x32x16 instruction.
+// One workgroup: D[m][n] = sum_k P[m][k] Q[n][k] for a tile of T x T, 4 waves of T/2 x T/2 on the 32x32x16 instruction.
 //   GRAM    P = Q = X:  S, the tiles on and below the diagonal, each written twice
 //   POLY    P = Q = S:  B = b S + c S S, likewise
 //   APPLY   P = X transposed while it is read from LDS, Q = B:  X <- a X + B X (m runs along X's rows in memory)
-//   LAST_*  APPLY whose result leaves the planes: orthogonalised, or subtracted from the parameter
+//   LAST_*  APPLY whose result leaves the pairs: orthogonalised, or subtracted from the parameter
+//
+// A stage is one line of 32 elements deep.  It goes straight from memory into LDS; STAGES - 1 of them are under way
+// while one is multiplied, and a stage costs one barrier.
 enum Kind { GRAM, POLY, APPLY, LAST_OUT, LAST_MUON };
 constexpr int BK = 32;
 
 struct Product {
-  Planes P, Q, D;
+  Pairs P, Q, D;
   int k;                // depth, a multiple of BK
-  int tiles_m;          // tiles along m (APPLY)
+  int n;                // matrices
+  int tiles, tiles_m;   // tiles of one matrix, and along m (APPLY)
   float self, acc;      // D = self * (the element of S or X) + acc * sum
 };
+struct Leave {          // what LAST_* needs besides
+  Matrices ms;
+  Shape sh;
+  Update u;
+};
+struct Stay {};
 
 // 16 bytes a lane straight into LDS; the wave's 64 pieces lie there in lane order
-__device__ __forceinline__ void to_lds(const _Float16* from, _Float16* lds) {
-  __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)from,
+__device__ __forceinline__ void to_lds(const char* from, uint32_t lane_offset, _Float16* lds) {
+  __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(from + lane_offset),
                                    (__attribute__((address_space(3))) void*)lds, 16, 0, 0);
 }
-// T rows of BK elements (64 B): 4 pieces a row, piece p of row m at p ^ (m >> 2 & 3), so that the 16 lanes that
-// read one piece of 16 rows meet 16 different bank groups
-template <int T>
-__device__ __forceinline__ void load_rows(const _Float16* g, int pitch, int k0, _Float16* lds, int wave, int lane) {
-  for (int c = wave; c < T / 16; c += 4) {
-    const int m = c * 16 + (lane >> 2), p = (lane & 3) ^ ((m >> 2) & 3);
-    to_lds(g + (int64_t)m * pitch + k0 + p * 8, lds + c * 512);
-  }
+// Waits until at most PENDING of the wave's loads are under way (and all its LDS reads are done), then for the
+// workgroup: after it every wave's older pieces are in LDS, and nobody reads the stage before any more.
+template <int PENDING> __device__ __forceinline__ void stage_ready() {
+  __builtin_amdgcn_s_waitcnt((PENDING & 15) | ((PENDING >> 4) << 14) | 0x0070);   // vmcnt(PENDING) lgkmcnt(0)
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
 }
-template <int T>
+// A stage of rows: T lines, 8 pieces of 16 B each (hi 0-3, lo 4-7), piece p of row m at p ^ (m >> 1 & 7), so that the
+// 16 lanes that read one piece of 16 rows meet 16 different bank groups.
+__device__ __forceinline__ int row_piece(int m, int p) { return p ^ ((m >> 1) & 7); }
 __device__ __forceinline__ f16x8 read_rows(const _Float16* lds, int m, int p) {
-  return *reinterpret_cast<const f16x8*>(lds + m * BK + ((p ^ ((m >> 2) & 3)) * 8));
+  return *reinterpret_cast<const f16x8*>(lds + m * 64 + row_piece(m, p) * 8);
 }
-// BK rows of T elements; piece p of row k lies at p ^ swz(k): the four rows one transposing read touches lie in
-// different banks
-template <int T> __device__ __forceinline__ int swz(int k) { return T == 128 ? (k & 3) << 2 : ((k >> 1) & 1) << 2; }
-template <int T>
-__device__ __forceinline__ void load_cols(const _Float16* g, int pitch, int k0, _Float16* lds, int wave, int lane) {
-  constexpr int PR = T / 8, RW = 64 / PR;               // pieces a row, rows a wave
-  for (int c = wave; c < BK / RW; c += 4) {
-    const int k = c * RW + lane / PR, p = (lane % PR) ^ swz<T>(k);
-    to_lds(g + (int64_t)(k0 + k) * pitch + p * 8, lds + c * 512);
-  }
-}
+// A stage of columns: BK rows of T / 32 lines; piece p of row k at p ^ ((k & 3) << 2), so that the four rows that a
+// transposing read touches (64 B each) lie in different banks.
+__device__ __forceinline__ int col_piece(int k, int p) { return p ^ ((k & 3) << 2); }
 // elements k .. k + 7 of column m (k a multiple of 8, m = the lane's): two transposing reads of 4 rows x 16 columns
 template <int T>
-__device__ __forceinline__ f16x8 read_cols(const _Float16* lds, int m0, int k0, int lane) {
-  const int q = lane & 15, col = m0 + ((lane >> 4) & 1) * 16 + (q & 3) * 4;
+__device__ __forceinline__ f16x8 read_cols(const _Float16* lds, int m0, int k0, int lo, int lane) {
+  const int q = lane & 15, col = ((lane >> 4) & 1) * 16 + (q & 3) * 4;   // within the line of m0
+  const int p = (m0 >> 5) * 8 + lo * 4 + (col >> 3);
   f16x8 r;
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
     const int k = k0 + (lane >> 5) * 8 + h * 4 + (q >> 2);
-    const _Float16* at = lds + k * T + ((((col >> 3) ^ swz<T>(k)) << 3) | (col & 7));
+    const _Float16* at = lds + k * 2 * T + col_piece(k, p) * 8 + (col & 7);
     const s16x4 v = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
         (__attribute__((address_space(3))) s16x4*)const_cast<_Float16*>(at));
     const f16x4 f = __builtin_bit_cast(f16x4, v);
@@ -197,55 +214,107 @@ __device__ __forceinline__ f16x8 read_cols(const _Float16* lds, int m0, int k0, 
   return r;
 }
 
-template <int T, int KIND, int DT>
-__global__ __launch_bounds__(NT) void k_product(Product pr, Matrices ms, Shape sh, Update u) {
+__device__ __forceinline__ bool tall(const Stay&) { return false; }
+__device__ __forceinline__ bool tall(const Leave& l) { return l.sh.rows > l.sh.cols; }
+// up to eight consecutive results into the output or the parameter
+template <int DT, bool MUON>
+__device__ __forceinline__ void leave(typename Elem<DT>::T* o, const float* v, int n, const Update& u) {
+  typedef Elem<DT> E;
+  Pack<typename E::T, 8> q;
+  if (n >= 8) {
+    if (MUON) q = *reinterpret_cast<const Pack<typename E::T, 8>*>(o);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) q.v[j] = E::put(MUON ? fmaf(u.keep, E::get(q.v[j]), -u.step * v[j]) : v[j]);
+    *reinterpret_cast<Pack<typename E::T, 8>*>(o) = q;
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      if (j < n) o[j] = E::put(MUON ? fmaf(u.keep, E::get(o[j]), -u.step * v[j]) : v[j]);
+  }
+}
+
+template <int T, int STAGES, int KIND, int DT, typename Out>
+__global__ __launch_bounds__(NT, 160 * 1024 / (STAGES * T * 256)) void k_product(Product pr, Out out) {
   constexpr bool COLS = KIND >= APPLY;
   constexpr int W = T / 2, F = W / 32;
-  __shared__ __attribute__((aligned(16))) _Float16 lds[4 * T * BK];
-  _Float16 *ph = lds, *pl = lds + T * BK, *qh = lds + 2 * T * BK, *ql = lds + 3 * T * BK;
-  const int i = blockIdx.y, lane = threadIdx.x % 64, wave = threadIdx.x / 64;
+  constexpr int CH = T / 32;                            // pieces of 1 KiB a wave loads of P, and of Q, per stage
+  constexpr int HALF = T * 64;                          // halves of one operand's stage
+  constexpr int PITCH = W + 4;                          // floats of a row of the wave's result in LDS
+  constexpr int LOOP = STAGES * 2 * HALF * 2, END = 4 * W * PITCH * 4;
+  __shared__ __attribute__((aligned(1024))) char shared[LOOP > END ? LOOP : END];
+  _Float16* lds = reinterpret_cast<_Float16*>(shared);
+  const int lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
+  // Workgroups go round the 8 XCDs in turn; give each XCD one contiguous run of tiles, so that the tiles that share
+  // rows or columns share an L2.
+  const int total = pr.tiles * pr.n, xcd = blockIdx.x % 8, nth = blockIdx.x / 8;
+  const int id = xcd * (total / 8) + min(xcd, total % 8) + nth;
+  const int i = id / pr.tiles, t = id % pr.tiles;
   int bm, bn;
   if (COLS) {
-    bm = blockIdx.x % pr.tiles_m, bn = blockIdx.x / pr.tiles_m;
+    bm = t % pr.tiles_m, bn = t / pr.tiles_m;
   } else {                                              // lower triangle, row by row
-    bm = (int)((sqrtf(8.f * blockIdx.x + 1.f) - 1.f) * 0.5f);
-    if ((bm + 1) * (bm + 2) / 2 <= (int)blockIdx.x) ++bm;
-    if (bm * (bm + 1) / 2 > (int)blockIdx.x) --bm;
-    bn = blockIdx.x - bm * (bm + 1) / 2;
+    bm = (int)((sqrtf(8.f * t + 1.f) - 1.f) * 0.5f);
+    if ((bm + 1) * (bm + 2) / 2 <= t) ++bm;
+    if (bm * (bm + 1) / 2 > t) --bm;
+    bn = t - bm * (bm + 1) / 2;
   }
-  const _Float16* gph = pr.P.hi + i * pr.P.each + (COLS ? (int64_t)bm * T : (int64_t)bm * T * pr.P.pitch);
-  const _Float16* gpl = pr.P.lo + i * pr.P.each + (COLS ? (int64_t)bm * T : (int64_t)bm * T * pr.P.pitch);
-  const _Float16* gqh = pr.Q.hi + i * pr.Q.each + (int64_t)bn * T * pr.Q.pitch;
-  const _Float16* gql = pr.Q.lo + i * pr.Q.each + (int64_t)bn * T * pr.Q.pitch;
-  const int m0 = (wave & 1) * W, n0 = (wave >> 1) * W;
-
-  f32x16 acc[F][F] = {};
-  for (int k0 = 0; k0 < pr.k; k0 += BK) {
+  const char* const from_p = (const char*)(COLS ? pr.P.hi(i, 0, bm * T) : pr.P.hi(i, bm * T, 0));
+  const char* const from_q = (const char*)pr.Q.hi(i, bn * T, 0);
+  // where in a stage this lane's 16 bytes come from (bytes)
+  uint32_t at_p[CH], at_q[CH];
+#pragma unroll
+  for (int c = 0; c < CH; ++c) {
+    const int chunk = wave + 4 * c;
+    const int m = chunk * 8 + (lane >> 3);
+    const uint32_t in_row = (uint32_t)row_piece(m, lane & 7) * 16;
+    at_q[c] = (uint32_t)m * pr.Q.pitch * 2 + in_row;
     if (COLS) {
-      load_cols<T>(gph, pr.P.pitch, k0, ph, wave, lane);
-      load_cols<T>(gpl, pr.P.pitch, k0, pl, wave, lane);
+      constexpr int PR = T / 4, RW = 64 / PR;           // pieces a row, rows a wave
+      const int k = chunk * RW + lane / PR;
+      at_p[c] = (uint32_t)k * pr.P.pitch * 2 + (uint32_t)col_piece(k, lane % PR) * 16;
     } else {
-      load_rows<T>(gph, pr.P.pitch, k0, ph, wave, lane);
-      load_rows<T>(gpl, pr.P.pitch, k0, pl, wave, lane);
+      at_p[c] = (uint32_t)m * pr.P.pitch * 2 + in_row;
     }
-    load_rows<T>(gqh, pr.Q.pitch, k0, qh, wave, lane);
-    load_rows<T>(gql, pr.Q.pitch, k0, ql, wave, lane);
-    __builtin_amdgcn_s_waitcnt(0x0f70);                 // vmcnt(0): this wave's pieces are in LDS
-    __syncthreads();
+  }
+  const int64_t step_p = COLS ? (int64_t)BK * pr.P.pitch * 2 : 128, step_q = 128;
+  auto load = [&](int stage, int buf) {
+#pragma unroll
+    for (int c = 0; c < CH; ++c) {
+      const int chunk = wave + 4 * c;
+      to_lds(from_p + stage * step_p, at_p[c], lds + buf * 2 * HALF + chunk * 512);
+      to_lds(from_q + stage * step_q, at_q[c], lds + buf * 2 * HALF + HALF + chunk * 512);
+    }
+  };
+  const int m0 = (wave & 1) * W, n0 = (wave >> 1) * W;
+  const int stages = pr.k / BK;
+  constexpr int AHEAD = STAGES - 1;                     // stages under way while one is multiplied
+  f32x16 acc[F][F] = {};
+#pragma unroll
+  for (int st = 0; st < AHEAD; ++st)
+    if (st < stages) load(st, st);
+  int buf = 0;
+  for (int st = 0; st < stages; ++st) {
+    // of the stages loaded so far, all but the newest AHEAD - 1 have to be there; near the end fewer were loaded
+    if (st + AHEAD - 1 < stages) stage_ready<2 * CH * (AHEAD - 1)>();
+    else stage_ready<0>();
+    if (st + AHEAD < stages) load(st + AHEAD, buf == 0 ? STAGES - 1 : buf - 1);   // over the stage read last
+    const _Float16 *p = lds + buf * 2 * HALF, *q = p + HALF;
+    buf = buf + 1 == STAGES ? 0 : buf + 1;
 #pragma unroll
     for (int kk = 0; kk < BK; kk += 16) {
       f16x8 ah[F], al[F], bh[F], bl[F];
 #pragma unroll
       for (int f = 0; f < F; ++f) {
+        const int piece = kk / 8 + (lane >> 5), m = m0 + 32 * f, n = n0 + 32 * f + (lane & 31);
         if (COLS) {
-          ah[f] = read_cols<T>(ph, m0 + 32 * f, kk, lane);
-          al[f] = read_cols<T>(pl, m0 + 32 * f, kk, lane);
+          ah[f] = read_cols<T>(p, m, kk, 0, lane);
+          al[f] = read_cols<T>(p, m, kk, 1, lane);
         } else {
-          ah[f] = read_rows<T>(ph, m0 + 32 * f + (lane & 31), kk / 8 + (lane >> 5));
-          al[f] = read_rows<T>(pl, m0 + 32 * f + (lane & 31), kk / 8 + (lane >> 5));
+          ah[f] = read_rows(p, m + (lane & 31), piece);
+          al[f] = read_rows(p, m + (lane & 31), piece + 4);
         }
-        bh[f] = read_rows<T>(qh, n0 + 32 * f + (lane & 31), kk / 8 + (lane >> 5));
-        bl[f] = read_rows<T>(ql, n0 + 32 * f + (lane & 31), kk / 8 + (lane >> 5));
+        bh[f] = read_rows(q, n, piece);
+        bl[f] = read_rows(q, n, piece + 4);
       }
 #pragma unroll
       for (int f = 0; f < F; ++f)
@@ -256,58 +325,71 @@ __global__ __launch_bounds__(NT) void k_product(Product pr, Matrices ms, Shape s
           acc[f][g] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ah[f], bh[g], acc[f][g], 0, 0, 0);
         }
     }
-    __syncthreads();
   }
 
-  // a lane holds column n and, four at a time, consecutive rows m
+  // The wave's result through LDS as [n][m], so that memory is read and written along rows.  A lane holds column n
+  // and, four at a time, consecutive m.
+  stage_ready<0>();
+  float* mine = reinterpret_cast<float*>(shared) + wave * W * PITCH;
 #pragma unroll
   for (int f = 0; f < F; ++f)
 #pragma unroll
     for (int g = 0; g < F; ++g)
 #pragma unroll
       for (int q = 0; q < 4; ++q) {
-        const int m = bm * T + m0 + 32 * f + 8 * q + 4 * (lane >> 5);
-        const int n = bn * T + n0 + 32 * g + (lane & 31);
-        float v[4];
-#pragma unroll
-        for (int j = 0; j < 4; ++j) v[j] = pr.acc * acc[f][g][4 * q + j];
-        if (KIND != GRAM) {
-          const Planes& A = pr.P;                       // S, or X
-          const int64_t at = i * A.each + (int64_t)n * A.pitch + m;
-          const f16x4 h = *reinterpret_cast<const f16x4*>(A.hi + at), l = *reinterpret_cast<const f16x4*>(A.lo + at);
-#pragma unroll
-          for (int j = 0; j < 4; ++j) v[j] = fmaf(pr.self, (float)h[j] + (float)l[j], v[j]);
-        }
-        if (KIND <= APPLY) {
-          f16x4 h, l;
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            _Float16 hj, lj;
-            split(v[j], hj, lj);
-            h[j] = hj, l[j] = lj;
-          }
-          const int64_t at = i * pr.D.each + (int64_t)n * pr.D.pitch + m;
-          *reinterpret_cast<f16x4*>(pr.D.hi + at) = h;
-          *reinterpret_cast<f16x4*>(pr.D.lo + at) = l;
-          if (KIND != APPLY && bm != bn) {
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-              const int64_t to = i * pr.D.each + (int64_t)(m + j) * pr.D.pitch + n;
-              pr.D.hi[to] = h[j], pr.D.lo[to] = l[j];
-            }
-          }
-        } else {
-          typedef Elem<DT> E;
-          typename E::T* o = (typename E::T*)ms.out[i];
-          const bool tall = sh.rows > sh.cols;
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            if (n >= sh.r || m + j >= sh.L) continue;
-            const int64_t at = tall ? (int64_t)(m + j) * sh.cols + n : (int64_t)n * sh.cols + m + j;
-            o[at] = E::put(KIND == LAST_MUON ? fmaf(u.keep, E::get(o[at]), -u.step * v[j]) : v[j]);
-          }
-        }
+        float4 v;
+        v.x = pr.acc * acc[f][g][4 * q], v.y = pr.acc * acc[f][g][4 * q + 1];
+        v.z = pr.acc * acc[f][g][4 * q + 2], v.w = pr.acc * acc[f][g][4 * q + 3];
+        *reinterpret_cast<float4*>(mine + (32 * g + (lane & 31)) * PITCH + 32 * f + 8 * q + 4 * (lane >> 5)) = v;
       }
+  stage_ready<0>();
+  constexpr int PER_ROW = W / 8;                        // lanes a row, 8 elements each
+#pragma unroll 4
+  for (int row = lane / PER_ROW; row < W; row += 64 / PER_ROW) {
+    const int col = lane % PER_ROW * 8, n = bn * T + n0 + row, m = bm * T + m0 + col;
+    float* at = mine + row * PITCH + col;
+    float v[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = at[j];
+    if constexpr (KIND != GRAM) {
+      const _Float16* self = pr.P.hi(i, n, m);          // of S, or X
+      const f16x8 h = *reinterpret_cast<const f16x8*>(self), l = *reinterpret_cast<const f16x8*>(self + 32);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[j] = fmaf(pr.self, (float)h[j] + (float)l[j], v[j]);
+    }
+    if constexpr (KIND <= APPLY) store_pairs(pr.D.hi(i, n, m), v);
+    if constexpr (KIND == POLY) {                       // for the mirrored tile
+#pragma unroll
+      for (int j = 0; j < 8; ++j) at[j] = v[j];
+    }
+    if constexpr (KIND > APPLY) {
+      typedef Elem<DT> E;
+      const Shape& sh = out.sh;
+      if (sh.rows > sh.cols) {                          // leaves transposed, below
+#pragma unroll
+        for (int j = 0; j < 8; ++j) at[j] = v[j];
+      } else if (n < sh.r) {
+        typename E::T* o = (typename E::T*)out.ms.out[i] + (int64_t)n * sh.cols + m;
+        leave<DT, KIND == LAST_MUON>(o, v, sh.L - m, out.u);
+      }
+    }
+  }
+  const bool turn = KIND < APPLY ? bm != bn : KIND > APPLY && tall(out);
+  if (!turn) return;
+  stage_ready<0>();
+#pragma unroll 4
+  for (int row = lane / PER_ROW; row < W; row += 64 / PER_ROW) {
+    const int col = lane % PER_ROW * 8, m = bm * T + m0 + row, n = bn * T + n0 + col;
+    float v[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = mine[(col + j) * PITCH + row];
+    if constexpr (KIND < APPLY) store_pairs(pr.D.hi(i, m, n), v);
+    if constexpr (KIND > APPLY) {
+      const Shape& sh = out.sh;
+      if (m < sh.L)
+        leave<DT, KIND == LAST_MUON>((typename Elem<DT>::T*)out.ms.out[i] + (int64_t)m * sh.cols + n, v, sh.r - n, out.u);
+    }
+  }
 }
 
 // ---- host --------------------------------------------------------------------------------------------------------
@@ -315,7 +397,7 @@ int64_t up(int64_t x, int64_t m) { return (x + m - 1) / m * m; }
 
 struct Work {
   double* part;
-  Planes X[2], S, B;
+  Pairs X[2], S, B;
   int64_t bytes;
 };
 Work layout(int n, const Shape& sh, char* base) {
@@ -326,27 +408,33 @@ Work layout(int n, const Shape& sh, char* base) {
     at += up(bytes, 256);
     return p;
   };
-  auto planes = [&](int rows, int pitch) {
-    Planes p;
-    p.each = (int64_t)rows * pitch, p.pitch = pitch;
-    p.hi = (_Float16*)take(2 * p.each * n);
-    p.lo = (_Float16*)take(2 * p.each * n);
+  auto pairs = [&](int rows, int cols) {
+    Pairs p;
+    p.pitch = 2 * cols, p.each = (int64_t)rows * p.pitch;
+    p.at = (_Float16*)take(2 * p.each * n);
     return p;
   };
   w.part = (double*)take(8 * PARTS * n);
-  w.X[0] = planes(sh.rp, sh.Lp);
-  w.X[1] = planes(sh.rp, sh.Lp);
-  w.S = planes(sh.rp, sh.rp);
-  w.B = planes(sh.rp, sh.rp);
+  w.X[0] = pairs(sh.rp, sh.Lp);
+  w.X[1] = pairs(sh.rp, sh.Lp);
+  w.S = pairs(sh.rp, sh.rp);
+  w.B = pairs(sh.rp, sh.rp);
   w.bytes = at;
   return w;
 }
 
-Shape shape_of(int64_t rows, int64_t cols) {
+// Tiles of 128 where the matrices have enough of them to occupy the 256 CUs, else of 64
+Shape shape_of(int n, int64_t rows, int64_t cols) {
   Shape s;
   s.rows = (int)rows, s.cols = (int)cols;
   s.r = (int)(rows < cols ? rows : cols), s.L = (int)(rows < cols ? cols : rows);
-  s.rp = (int)up(s.r, PAD), s.Lp = (int)up(s.L, PAD);
+  const int64_t tr = up(s.r, 128) / 128, tL = up(s.L, 128) / 128;
+  s.tile_r = n * tr * (tr + 1) / 2 >= 256 ? 128 : 64;
+  s.tile_L = n * tr * tL >= 256 ? 128 : 64;
+  s.rp = (int)up(s.r, s.tile_r > s.tile_L ? s.tile_r : s.tile_L);
+  s.Lp = (int)up(s.L, s.tile_L);
+  const int64_t parts = up(rows * cols, 4 * NT * 4) / (4 * NT * 4);   // at least four rounds each
+  s.parts = (int)(parts < PARTS ? parts : PARTS);
   return s;
 }
 
@@ -393,33 +481,40 @@ int launched(const char* what) {
   return e == hipSuccess ? 0 : ops_error(MTAZ_E_DEVICE, what, hipGetErrorString(e));
 }
 
-template <int T, int KIND, int DT>
-void product(const Product& pr, int tiles, int n, const Matrices& ms, const Shape& sh, const Update& u, hipStream_t s) {
-  k_product<T, KIND, DT><<<dim3(tiles, n), NT, 0, s>>>(pr, ms, sh, u);
+template <int KIND, int DT, typename Out>
+void product(Product pr, int T, const Out& out, hipStream_t s) {
+  const unsigned grid = (unsigned)(pr.tiles * pr.n);
+  if (T == 128) k_product<128, 2, KIND, DT, Out><<<grid, NT, 0, s>>>(pr, out);
+  else if (grid <= 256) k_product<64, 8, KIND, DT, Out><<<grid, NT, 0, s>>>(pr, out);   // a CU each: deeper
+  else k_product<64, 4, KIND, DT, Out><<<grid, NT, 0, s>>>(pr, out);
 }
 
 template <int DT, bool MUON>
 void iterate(const Matrices& ms, int n, const Shape& sh, const Update& u, int steps, const double* co, double eps,
              const Exponents& e, char* base, hipStream_t s) {
-  constexpr int T = 64;
   const Work w = layout(n, sh, base);
   const int64_t count = (int64_t)sh.rows * sh.cols;
-  k_squares<DT, MUON><<<dim3(PARTS, n), NT, 0, s>>>(ms, count, u, w.part);
-  k_planes<DT, MUON><<<dim3(sh.Lp / 64, sh.rp / 64, n), NT, 0, s>>>(ms, sh, u, w.part, eps, ldexp(1., e.x[0]), w.X[0]);
-  const int tr = sh.rp / T, tL = sh.Lp / T, tri = tr * (tr + 1) / 2;
+  k_squares<DT, MUON><<<dim3(sh.parts, n), NT, 0, s>>>(ms, count, u, w.part);
+  k_pairs<DT, MUON><<<dim3(sh.Lp / 64, sh.rp / 64, n), NT, 0, s>>>(ms, sh, u, w.part, eps, ldexp(1., e.x[0]), w.X[0]);
+  const int tr = sh.rp / sh.tile_r, tri = tr * (tr + 1) / 2;
+  const int tL = sh.Lp / sh.tile_L, tall = sh.rp / sh.tile_L * tL;
   for (int t = 0; t < steps; ++t) {
-    const Planes &X = w.X[t & 1], &Y = w.X[(t + 1) & 1];
-    Product p = {X, X, w.S, sh.Lp, 0, 0.f, (float)ldexp(1., e.s[t] - 2 * e.x[t])};
-    product<T, GRAM, MTAZ_F32>(p, tri, n, ms, sh, u, s);
-    p = {w.S, w.S, w.B, sh.rp, 0, (float)ldexp(co[1], e.b[t] - e.s[t]), (float)ldexp(co[2], e.b[t] - 2 * e.s[t])};
-    product<T, POLY, MTAZ_F32>(p, tri, n, ms, sh, u, s);
+    const Pairs &X = w.X[t & 1], &Y = w.X[(t + 1) & 1];
+    product<GRAM, MTAZ_F32>({X, X, w.S, sh.Lp, n, tri, 0, 0.f, (float)ldexp(1., e.s[t] - 2 * e.x[t])}, sh.tile_r, Stay{}, s);
+    product<POLY, MTAZ_F32>({w.S, w.S, w.B, sh.rp, n, tri, 0, (float)ldexp(co[1], e.b[t] - e.s[t]),
+                             (float)ldexp(co[2], e.b[t] - 2 * e.s[t])}, sh.tile_r, Stay{}, s);
     const int ex = t + 1 < steps ? e.x[t + 1] : 0;
-    p = {X, w.B, Y, sh.rp, tL, (float)ldexp(co[0], ex - e.x[t]), (float)ldexp(1., ex - e.x[t] - e.b[t])};
-    if (t + 1 < steps)
-      product<T, APPLY, MTAZ_F32>(p, tr * tL, n, ms, sh, u, s);
-    else
-      product<T, MUON ? LAST_MUON : LAST_OUT, DT>(p, tr * tL, n, ms, sh, u, s);
+    const Product last = {X, w.B, Y, sh.rp, n, tall, tL, (float)ldexp(co[0], ex - e.x[t]),
+                          (float)ldexp(1., ex - e.x[t] - e.b[t])};
+    if (t + 1 < steps) product<APPLY, MTAZ_F32>(last, sh.tile_L, Stay{}, s);
+    else product<MUON ? LAST_MUON : LAST_OUT, DT>(last, sh.tile_L, Leave{ms, sh, u}, s);
   }
+}
+
+// of the largest group; a smaller last one may choose smaller tiles, never larger ones
+int64_t workspace(int n, int64_t rows, int64_t cols) {
+  const int m = n < MOST ? n : MOST;
+  return layout(m, shape_of(m, rows, cols), nullptr).bytes;
 }
 
 // All checks, then the matrices in groups of at most MOST over the same workspace
@@ -438,8 +533,7 @@ int run(const char* what, int device, int n, int64_t rows, int64_t cols, int dty
   for (int i = 0; i < n; ++i)
     if (!grad[i] || !out[i] || (MUON && !momenta[i])) return ops_error(MTAZ_E_FAIL, what, "a null matrix");
   if (n == 0) return 0;
-  const Shape sh = shape_of(rows, cols);
-  if (!work || ((uintptr_t)work & 255) || work_bytes < layout(n < MOST ? n : MOST, sh, nullptr).bytes)
+  if (!work || ((uintptr_t)work & 255) || work_bytes < workspace(n, rows, cols))
     return ops_error(MTAZ_E_FAIL, what, "workspace too small or not aligned to 256 bytes");
   DeviceScope on(device);
   if (on.status != hipSuccess) return ops_error(MTAZ_E_DEVICE, what, hipGetErrorString(on.status));
@@ -451,6 +545,7 @@ int run(const char* what, int device, int n, int64_t rows, int64_t cols, int dty
       if (MUON) ms.momentum[i] = momenta[first + i];
     }
     const hipStream_t s = (hipStream_t)stream;
+    const Shape sh = shape_of(m, rows, cols);
     if (dtype == MTAZ_F32) iterate<MTAZ_F32, MUON>(ms, m, sh, u, steps, co, eps, e, (char*)work, s);
     else if (dtype == MTAZ_F16) iterate<MTAZ_F16, MUON>(ms, m, sh, u, steps, co, eps, e, (char*)work, s);
     else iterate<MTAZ_BF16, MUON>(ms, m, sh, u, steps, co, eps, e, (char*)work, s);
@@ -465,7 +560,7 @@ using namespace mtaz;
 
 extern "C" int64_t mtaz_orthogonalize_workspace(int n, int64_t rows, int64_t cols, int dtype) {
   if (const char* bad = bad_shape(n, rows, cols, dtype)) return ops_error(MTAZ_E_FAIL, "orthogonalize", bad);
-  return layout(n < MOST ? n : MOST, shape_of(rows, cols), nullptr).bytes;
+  return workspace(n, rows, cols);
 }
 
 extern "C" int mtaz_orthogonalize(int device, int n, int64_t rows, int64_t cols, int dtype, const void* const* d_grad,
