@@ -1,7 +1,7 @@
 // Orthogonalisation of matrices by Newton-Schulz products, and the Muon step around it.
 //
 // With r the shorter and L the longer side, X [r][L] (a tall matrix transposed) and the coefficients a, b, c:
-//   X <- G / (|G|_F + eps);    steps times:  S = X X^T,  B = b S + c S S,  X <- a X + B X.
+//   X <- G / (|G|_F + eps);    steps times:  S = X X^T,  B = a I + b S + c S S,  X <- B X.
 //
 // The products run on the f16 matrix cores and keep 32-bit accuracy: a value x is held as two f16 numbers,
 // hi = f16(2^e x) and lo = f16(2^e x - hi), together 22 bits, and a product is hi hi + hi lo + lo hi with
@@ -73,17 +73,31 @@ __global__ __launch_bounds__(NT) void k_squares(Matrices ms, int64_t count, Upda
   const typename E::T* g = (const typename E::T*)ms.grad[i];
   float* mom = ms.momentum[i];
   double s = 0.;
-  for (int64_t k = 4 * ((int64_t)blockIdx.x * NT + threadIdx.x); k < count; k += 4ll * NT * parts) {
-    const int n = (int)min((int64_t)4, count - k);
-    for (int j = 0; j < n; ++j) {
-      const float gv = E::get(g[k + j]);
-      float mv = 0.f;
-      if (MUON) {
-        mv = fmaf(u.momentum, mom[k + j], (1.f - u.momentum) * gv);
-        mom[k + j] = mv;
-      }
-      const double x = (double)update_of<DT, MUON>(gv, mv, u);
-      s += x * x;
+  constexpr int N = 8;
+  for (int64_t k = N * ((int64_t)blockIdx.x * NT + threadIdx.x); k < count; k += (int64_t)N * NT * parts) {
+    const int n = (int)min((int64_t)N, count - k);
+    Pack<typename E::T, N> gv;
+    Pack<float, N> mv;
+    if (n == N) {
+      gv = *reinterpret_cast<const Pack<typename E::T, N>*>(g + k);
+      if (MUON) mv = *reinterpret_cast<const Pack<float, N>*>(mom + k);
+    } else {
+#pragma unroll
+      for (int j = 0; j < N; ++j) gv.v[j] = j < n ? g[k + j] : (typename E::T)0.f, mv.v[j] = MUON && j < n ? mom[k + j] : 0.f;
+    }
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+      const float x = E::get(gv.v[j]);
+      if (MUON) mv.v[j] = fmaf(u.momentum, mv.v[j], (1.f - u.momentum) * x);
+      const double y = (double)update_of<DT, MUON>(x, mv.v[j], u);
+      s = fma(y, y, s);
+    }
+    if (MUON) {
+      if (n == N) *reinterpret_cast<Pack<float, N>*>(mom + k) = mv;
+      else
+#pragma unroll
+        for (int j = 0; j < N; ++j)
+          if (j < n) mom[k + j] = mv.v[j];
     }
   }
   __shared__ double ws[NT / 64];
@@ -150,8 +164,8 @@ __global__ __launch_bounds__(NT) void k_pairs(Matrices ms, Shape sh, Update u, c
 // ---- products --------------------------------------------------------------------------------------------------
 // One workgroup: D[m][n] = sum_k P[m][k] Q[n][k] for a tile of T x T, 4 waves of T/2 x T/2 on the 32x32x16 instruction.
 //   GRAM    P = Q = X:  S, the tiles on and below the diagonal, each written twice
-//   POLY    P = Q = S:  B = b S + c S S, likewise
-//   APPLY   P = X transposed while it is read from LDS, Q = B:  X <- a X + B X (m runs along X's rows in memory)
+//   POLY    P = Q = S:  B = a I + b S + c S S, likewise (a in B and not in the next product: X is read once less there)
+//   APPLY   P = X transposed while it is read from LDS, Q = B:  X <- B X (m runs along X's rows in memory)
 //   LAST_*  APPLY whose result leaves the pairs: orthogonalised, or subtracted from the parameter
 //
 // A stage is one line of 32 elements deep.  It goes straight from memory into LDS; STAGES - 1 of them are under way
@@ -164,7 +178,7 @@ struct Product {
   int k;                // depth, a multiple of BK
   int n;                // matrices
   int tiles, tiles_m;   // tiles of one matrix, and along m (APPLY)
-  float self, acc;      // D = self * (the element of S or X) + acc * sum
+  float acc, self, one; // D = acc * sum, and in POLY + self * the element of S + one on the diagonal
 };
 struct Leave {          // what LAST_* needs besides
   Matrices ms;
@@ -351,11 +365,14 @@ __global__ __launch_bounds__(NT, 160 * 1024 / (STAGES * T * 256)) void k_product
     float v[8];
 #pragma unroll
     for (int j = 0; j < 8; ++j) v[j] = at[j];
-    if constexpr (KIND != GRAM) {
-      const _Float16* self = pr.P.hi(i, n, m);          // of S, or X
+    if constexpr (KIND == POLY) {
+      const _Float16* self = pr.P.hi(i, n, m);
       const f16x8 h = *reinterpret_cast<const f16x8*>(self), l = *reinterpret_cast<const f16x8*>(self + 32);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) v[j] = fmaf(pr.self, (float)h[j] + (float)l[j], v[j]);
+      for (int j = 0; j < 8; ++j) {
+        v[j] = fmaf(pr.self, (float)h[j] + (float)l[j], v[j]);
+        if (m + j == n) v[j] += pr.one;
+      }
     }
     if constexpr (KIND <= APPLY) store_pairs(pr.D.hi(i, n, m), v);
     if constexpr (KIND == POLY) {                       // for the mirrored tile
@@ -433,7 +450,7 @@ Shape shape_of(int n, int64_t rows, int64_t cols) {
   s.tile_L = n * tr * tL >= 256 ? 128 : 64;
   s.rp = (int)up(s.r, s.tile_r > s.tile_L ? s.tile_r : s.tile_L);
   s.Lp = (int)up(s.L, s.tile_L);
-  const int64_t parts = up(rows * cols, 4 * NT * 4) / (4 * NT * 4);   // at least four rounds each
+  const int64_t parts = up(rows * cols, 8 * NT * 2) / (8 * NT * 2);   // two rounds each at least
   s.parts = (int)(parts < PARTS ? parts : PARTS);
   return s;
 }
@@ -448,7 +465,7 @@ const char* bad_shape(int n, int64_t rows, int64_t cols, int dtype) {
 
 // Exponents that keep every entry below 2^14: of X before each step and after the last, of S and of B.
 // Singular values start in [0, 1]; after a step they lie below the largest |s (a + b s^2 + c s^4)| over the range
-// before it, S below its square and B below the largest |b s^2 + c s^4|.  The maxima are taken over a grid that holds
+// before it, S below its square and B below the largest |a + b s^2 + c s^4|.  The maxima are taken over a grid that holds
 // the range's end, where a polynomial between two of 4096 points exceeds the larger one by some 10^-7 of its
 // maximum, with a thousandth on top for that and for roundings; f16 has room for twice 2^14 besides.
 struct Exponents {
@@ -466,8 +483,8 @@ const char* bounds(int steps, const double* co, Exponents& e) {
     if (t == steps) break;
     double next = 0., poly = 0.;
     for (int k = 0; k <= 4096; ++k) {
-      const double s = top * k / 4096., q = co[1] * s * s + co[2] * s * s * s * s;
-      next = fmax(next, fabs(s * (co[0] + q))), poly = fmax(poly, fabs(q));
+      const double s = top * k / 4096., q = co[0] + co[1] * s * s + co[2] * s * s * s * s;
+      next = fmax(next, fabs(s * q)), poly = fmax(poly, fabs(q));
     }
     e.s[t] = unit(fmax(1.001 * top * top, 1e-9));
     e.b[t] = unit(fmax(1.001 * poly, 1e-9));
@@ -500,12 +517,12 @@ void iterate(const Matrices& ms, int n, const Shape& sh, const Update& u, int st
   const int tL = sh.Lp / sh.tile_L, tall = sh.rp / sh.tile_L * tL;
   for (int t = 0; t < steps; ++t) {
     const Pairs &X = w.X[t & 1], &Y = w.X[(t + 1) & 1];
-    product<GRAM, MTAZ_F32>({X, X, w.S, sh.Lp, n, tri, 0, 0.f, (float)ldexp(1., e.s[t] - 2 * e.x[t])}, sh.tile_r, Stay{}, s);
-    product<POLY, MTAZ_F32>({w.S, w.S, w.B, sh.rp, n, tri, 0, (float)ldexp(co[1], e.b[t] - e.s[t]),
-                             (float)ldexp(co[2], e.b[t] - 2 * e.s[t])}, sh.tile_r, Stay{}, s);
+    product<GRAM, MTAZ_F32>({X, X, w.S, sh.Lp, n, tri, 0, (float)ldexp(1., e.s[t] - 2 * e.x[t]), 0.f, 0.f}, sh.tile_r,
+                            Stay{}, s);
+    product<POLY, MTAZ_F32>({w.S, w.S, w.B, sh.rp, n, tri, 0, (float)ldexp(co[2], e.b[t] - 2 * e.s[t]),
+                             (float)ldexp(co[1], e.b[t] - e.s[t]), (float)ldexp(co[0], e.b[t])}, sh.tile_r, Stay{}, s);
     const int ex = t + 1 < steps ? e.x[t + 1] : 0;
-    const Product last = {X, w.B, Y, sh.rp, n, tall, tL, (float)ldexp(co[0], ex - e.x[t]),
-                          (float)ldexp(1., ex - e.x[t] - e.b[t])};
+    const Product last = {X, w.B, Y, sh.rp, n, tall, tL, (float)ldexp(1., ex - e.x[t] - e.b[t]), 0.f, 0.f};
     if (t + 1 < steps) product<APPLY, MTAZ_F32>(last, sh.tile_L, Stay{}, s);
     else product<MUON ? LAST_MUON : LAST_OUT, DT>(last, sh.tile_L, Leave{ms, sh, u}, s);
   }
