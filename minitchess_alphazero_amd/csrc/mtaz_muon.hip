@@ -162,20 +162,20 @@ __global__ __launch_bounds__(NT) void k_pairs(Matrices ms, Shape sh, Update u, c
 }
 
 // ---- products --------------------------------------------------------------------------------------------------
-// One workgroup: D[m][n] = sum_k P[m][k] Q[n][k] for a tile of T x T, 4 waves of T/2 x T/2 on the 32x32x16 instruction.
+// One workgroup: D[m][n] = sum_k P[m][k] Q[n][k] for a tile of T x T on the 32x32x16 instruction.
 //   GRAM    P = Q = X:  S, the tiles on and below the diagonal, each written twice
 //   POLY    P = Q = S:  B = a I + b S + c S S, likewise (a in B and not in the next product: X is read once less there)
 //   APPLY   P = X transposed while it is read from LDS, Q = B:  X <- B X (m runs along X's rows in memory)
 //   LAST_*  APPLY whose result leaves the pairs: orthogonalised, or subtracted from the parameter
 //
-// A stage is one line of 32 elements deep.  It goes straight from memory into LDS; STAGES - 1 of them are under way
-// while one is multiplied, and a stage costs one barrier.
+// A round is DEPTH elements deep.  It goes straight from memory into LDS, in a ring of RING rounds: all but one are
+// under way while one is multiplied, and a round costs one barrier.  SIDE x SIDE waves share the tile, GROUPS such
+// sets share the depth of a round, and their sums are added at the end in a fixed order.
 enum Kind { GRAM, POLY, APPLY, LAST_OUT, LAST_MUON };
-constexpr int BK = 32;
 
 struct Product {
   Pairs P, Q, D;
-  int k;                // depth, a multiple of BK
+  int k;                // depth, a multiple of 64
   int n;                // matrices
   int tiles, tiles_m;   // tiles of one matrix, and along m (APPLY)
   float acc, self, one; // D = acc * sum, and in POLY + self * the element of S + one on the diagonal
@@ -193,20 +193,20 @@ __device__ __forceinline__ void to_lds(const char* from, uint32_t lane_offset, _
                                    (__attribute__((address_space(3))) void*)lds, 16, 0, 0);
 }
 // Waits until at most PENDING of the wave's loads are under way (and all its LDS reads are done), then for the
-// workgroup: after it every wave's older pieces are in LDS, and nobody reads the stage before any more.
-template <int PENDING> __device__ __forceinline__ void stage_ready() {
+// workgroup: after it every wave's older pieces are in LDS, and nobody reads the round before any more.
+template <int PENDING> __device__ __forceinline__ void ready() {
   __builtin_amdgcn_s_waitcnt((PENDING & 15) | ((PENDING >> 4) << 14) | 0x0070);   // vmcnt(PENDING) lgkmcnt(0)
   asm volatile("" ::: "memory");
   __builtin_amdgcn_s_barrier();
   asm volatile("" ::: "memory");
 }
-// A stage of rows: T lines, 8 pieces of 16 B each (hi 0-3, lo 4-7), piece p of row m at p ^ (m >> 1 & 7), so that the
+// Rows in LDS: blocks of T lines, 8 pieces of 16 B each (hi 0-3, lo 4-7), piece p of row m at p ^ (m >> 1 & 7), so that the
 // 16 lanes that read one piece of 16 rows meet 16 different bank groups.
 __device__ __forceinline__ int row_piece(int m, int p) { return p ^ ((m >> 1) & 7); }
 __device__ __forceinline__ f16x8 read_rows(const _Float16* lds, int m, int p) {
   return *reinterpret_cast<const f16x8*>(lds + m * 64 + row_piece(m, p) * 8);
 }
-// A stage of columns: BK rows of T / 32 lines; piece p of row k at p ^ ((k & 3) << 2), so that the four rows that a
+// Columns in LDS: rows of T / 32 lines; piece p of row k at p ^ ((k & 3) << 2), so that the four rows that a
 // transposing read touches (64 B each) lie in different banks.
 __device__ __forceinline__ int col_piece(int k, int p) { return p ^ ((k & 3) << 2); }
 // elements k .. k + 7 of column m (k a multiple of 8, m = the lane's): two transposing reads of 4 rows x 16 columns
@@ -247,17 +247,22 @@ __device__ __forceinline__ void leave(typename Elem<DT>::T* o, const float* v, i
   }
 }
 
-template <int T, int STAGES, int KIND, int DT, typename Out>
-__global__ __launch_bounds__(NT, 160 * 1024 / (STAGES * T * 256)) void k_product(Product pr, Out out) {
+template <int T, int SIDE, int GROUPS, int DEPTH, int RING, int KIND, int DT, typename Out>
+__global__ __launch_bounds__(64 * SIDE * SIDE * GROUPS, 160 * 1024 / (RING * T * DEPTH * 8) * SIDE * SIDE * GROUPS / 4)
+void k_product(Product pr, Out out) {
   constexpr bool COLS = KIND >= APPLY;
-  constexpr int W = T / 2, F = W / 32;
-  constexpr int CH = T / 32;                            // pieces of 1 KiB a wave loads of P, and of Q, per stage
-  constexpr int HALF = T * 64;                          // halves of one operand's stage
-  constexpr int PITCH = W + 4;                          // floats of a row of the wave's result in LDS
-  constexpr int LOOP = STAGES * 2 * HALF * 2, END = 4 * W * PITCH * 4;
+  constexpr int WAVES = SIDE * SIDE * GROUPS;
+  constexpr int W = T / SIDE, F = W / 32;               // a wave's part of the tile, in 32 x 32 sums
+  constexpr int STEPS = DEPTH / 16 / GROUPS;            // instructions deep a wave goes per round
+  constexpr int CH = T * DEPTH / 256 / WAVES;           // pieces of 1 KiB a wave loads of P, and of Q, per round
+  constexpr int HALF = T * DEPTH * 2;                   // halves of one operand's round
+  constexpr int PITCH = W + 4, PART = W * PITCH;        // floats of a wave's sums in LDS
+  constexpr int LOOP = RING * 2 * HALF * 2, END = WAVES * PART * 4;
+  static_assert(T * DEPTH % (256 * WAVES) == 0 && DEPTH % (16 * GROUPS) == 0 && 64 % DEPTH == 0, "round");
   __shared__ __attribute__((aligned(1024))) char shared[LOOP > END ? LOOP : END];
   _Float16* lds = reinterpret_cast<_Float16*>(shared);
   const int lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
+  const int part = wave % (SIDE * SIDE), group = wave / (SIDE * SIDE);
   // Workgroups go round the 8 XCDs in turn; give each XCD one contiguous run of tiles, so that the tiles that share
   // rows or columns share an L2.
   const int total = pr.tiles * pr.n, xcd = blockIdx.x % 8, nth = blockIdx.x / 8;
@@ -274,13 +279,13 @@ __global__ __launch_bounds__(NT, 160 * 1024 / (STAGES * T * 256)) void k_product
   }
   const char* const from_p = (const char*)(COLS ? pr.P.hi(i, 0, bm * T) : pr.P.hi(i, bm * T, 0));
   const char* const from_q = (const char*)pr.Q.hi(i, bn * T, 0);
-  // where in a stage this lane's 16 bytes come from (bytes)
+  // where in a round this lane's 16 bytes come from (bytes)
   uint32_t at_p[CH], at_q[CH];
 #pragma unroll
   for (int c = 0; c < CH; ++c) {
-    const int chunk = wave + 4 * c;
-    const int m = chunk * 8 + (lane >> 3);
-    const uint32_t in_row = (uint32_t)row_piece(m, lane & 7) * 16;
+    const int chunk = wave + WAVES * c;
+    const int line = chunk / (T / 8), m = chunk % (T / 8) * 8 + (lane >> 3);
+    const uint32_t in_row = (uint32_t)(line * 128 + row_piece(m, lane & 7) * 16);
     at_q[c] = (uint32_t)m * pr.Q.pitch * 2 + in_row;
     if (COLS) {
       constexpr int PR = T / 4, RW = 64 / PR;           // pieces a row, rows a wave
@@ -290,45 +295,47 @@ __global__ __launch_bounds__(NT, 160 * 1024 / (STAGES * T * 256)) void k_product
       at_p[c] = (uint32_t)m * pr.P.pitch * 2 + in_row;
     }
   }
-  const int64_t step_p = COLS ? (int64_t)BK * pr.P.pitch * 2 : 128, step_q = 128;
-  auto load = [&](int stage, int buf) {
+  const int64_t step_p = COLS ? (int64_t)DEPTH * pr.P.pitch * 2 : DEPTH * 4, step_q = DEPTH * 4;
+  auto load = [&](int round, int buf) {
 #pragma unroll
     for (int c = 0; c < CH; ++c) {
-      const int chunk = wave + 4 * c;
-      to_lds(from_p + stage * step_p, at_p[c], lds + buf * 2 * HALF + chunk * 512);
-      to_lds(from_q + stage * step_q, at_q[c], lds + buf * 2 * HALF + HALF + chunk * 512);
+      const int chunk = wave + WAVES * c;
+      to_lds(from_p + round * step_p, at_p[c], lds + buf * 2 * HALF + chunk * 512);
+      to_lds(from_q + round * step_q, at_q[c], lds + buf * 2 * HALF + HALF + chunk * 512);
     }
   };
-  const int m0 = (wave & 1) * W, n0 = (wave >> 1) * W;
-  const int stages = pr.k / BK;
-  constexpr int AHEAD = STAGES - 1;                     // stages under way while one is multiplied
+  const int m0 = part % SIDE * W, n0 = part / SIDE * W;
+  const int rounds = pr.k / DEPTH;
+  constexpr int AHEAD = RING - 1;                       // rounds under way while one is multiplied
   f32x16 acc[F][F] = {};
 #pragma unroll
-  for (int st = 0; st < AHEAD; ++st)
-    if (st < stages) load(st, st);
+  for (int r = 0; r < AHEAD; ++r)
+    if (r < rounds) load(r, r);
   int buf = 0;
-  for (int st = 0; st < stages; ++st) {
-    // of the stages loaded so far, all but the newest AHEAD - 1 have to be there; near the end fewer were loaded
-    if (st + AHEAD - 1 < stages) stage_ready<2 * CH * (AHEAD - 1)>();
-    else stage_ready<0>();
-    if (st + AHEAD < stages) load(st + AHEAD, buf == 0 ? STAGES - 1 : buf - 1);   // over the stage read last
+  for (int r = 0; r < rounds; ++r) {
+    // of the rounds loaded so far, all but the newest AHEAD - 1 have to be there; near the end fewer were loaded
+    if (r + AHEAD - 1 < rounds) ready<2 * CH * (AHEAD - 1)>();
+    else ready<0>();
+    if (r + AHEAD < rounds) load(r + AHEAD, buf == 0 ? RING - 1 : buf - 1);   // over the round read last
     const _Float16 *p = lds + buf * 2 * HALF, *q = p + HALF;
-    buf = buf + 1 == STAGES ? 0 : buf + 1;
+    buf = buf + 1 == RING ? 0 : buf + 1;
 #pragma unroll
-    for (int kk = 0; kk < BK; kk += 16) {
+    for (int step = 0; step < STEPS; ++step) {
+      const int kk = (group * STEPS + step) * 16;
+      const int line = kk / 32 * T * 64, piece = kk % 32 / 8 + (lane >> 5);   // rows: block of lines, piece
       f16x8 ah[F], al[F], bh[F], bl[F];
 #pragma unroll
       for (int f = 0; f < F; ++f) {
-        const int piece = kk / 8 + (lane >> 5), m = m0 + 32 * f, n = n0 + 32 * f + (lane & 31);
+        const int m = m0 + 32 * f, n = n0 + 32 * f + (lane & 31);
         if (COLS) {
           ah[f] = read_cols<T>(p, m, kk, 0, lane);
           al[f] = read_cols<T>(p, m, kk, 1, lane);
         } else {
-          ah[f] = read_rows(p, m + (lane & 31), piece);
-          al[f] = read_rows(p, m + (lane & 31), piece + 4);
+          ah[f] = read_rows(p + line, m + (lane & 31), piece);
+          al[f] = read_rows(p + line, m + (lane & 31), piece + 4);
         }
-        bh[f] = read_rows(q, n, piece);
-        bl[f] = read_rows(q, n, piece + 4);
+        bh[f] = read_rows(q + line, n, piece);
+        bl[f] = read_rows(q + line, n, piece + 4);
       }
 #pragma unroll
       for (int f = 0; f < F; ++f)
@@ -341,10 +348,11 @@ __global__ __launch_bounds__(NT, 160 * 1024 / (STAGES * T * 256)) void k_product
     }
   }
 
-  // The wave's result through LDS as [n][m], so that memory is read and written along rows.  A lane holds column n
-  // and, four at a time, consecutive m.
-  stage_ready<0>();
-  float* mine = reinterpret_cast<float*>(shared) + wave * W * PITCH;
+  // The sums through LDS as [n][m], so that memory is read and written along rows: a lane holds column n and, four
+  // at a time, consecutive m.  Group g then finishes the g-th share of the rows.
+  ready<0>();
+  float* const sums = reinterpret_cast<float*>(shared) + part * PART;         // of group 0; the next lies SIDE^2 PART on
+  float* const mine = sums + group * SIDE * SIDE * PART;
 #pragma unroll
   for (int f = 0; f < F; ++f)
 #pragma unroll
@@ -352,19 +360,25 @@ __global__ __launch_bounds__(NT, 160 * 1024 / (STAGES * T * 256)) void k_product
 #pragma unroll
       for (int q = 0; q < 4; ++q) {
         float4 v;
-        v.x = pr.acc * acc[f][g][4 * q], v.y = pr.acc * acc[f][g][4 * q + 1];
-        v.z = pr.acc * acc[f][g][4 * q + 2], v.w = pr.acc * acc[f][g][4 * q + 3];
+        v.x = acc[f][g][4 * q], v.y = acc[f][g][4 * q + 1], v.z = acc[f][g][4 * q + 2], v.w = acc[f][g][4 * q + 3];
         *reinterpret_cast<float4*>(mine + (32 * g + (lane & 31)) * PITCH + 32 * f + 8 * q + 4 * (lane >> 5)) = v;
       }
-  stage_ready<0>();
-  constexpr int PER_ROW = W / 8;                        // lanes a row, 8 elements each
+  ready<0>();
+  constexpr int PER_ROW = W / 8, SHARE = W / GROUPS;    // lanes a row, 8 elements each; rows a wave
+  const bool turn = KIND < APPLY ? bm != bn : KIND > APPLY && tall(out);   // leaves transposed (too), below
 #pragma unroll 4
-  for (int row = lane / PER_ROW; row < W; row += 64 / PER_ROW) {
+  for (int row = group * SHARE + lane / PER_ROW; row < (group + 1) * SHARE; row += 64 / PER_ROW) {
     const int col = lane % PER_ROW * 8, n = bn * T + n0 + row, m = bm * T + m0 + col;
-    float* at = mine + row * PITCH + col;
+    float* at = sums + row * PITCH + col;
     float v[8];
 #pragma unroll
     for (int j = 0; j < 8; ++j) v[j] = at[j];
+#pragma unroll
+    for (int g = 1; g < GROUPS; ++g)
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[j] += at[g * SIDE * SIDE * PART + j];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] *= pr.acc;
     if constexpr (KIND == POLY) {
       const _Float16* self = pr.P.hi(i, n, m);
       const f16x8 h = *reinterpret_cast<const f16x8*>(self), l = *reinterpret_cast<const f16x8*>(self + 32);
@@ -374,32 +388,26 @@ __global__ __launch_bounds__(NT, 160 * 1024 / (STAGES * T * 256)) void k_product
         if (m + j == n) v[j] += pr.one;
       }
     }
-    if constexpr (KIND <= APPLY) store_pairs(pr.D.hi(i, n, m), v);
-    if constexpr (KIND == POLY) {                       // for the mirrored tile
+    if (turn) {
 #pragma unroll
       for (int j = 0; j < 8; ++j) at[j] = v[j];
     }
-    if constexpr (KIND > APPLY) {
-      typedef Elem<DT> E;
+    if constexpr (KIND <= APPLY) {
+      store_pairs(pr.D.hi(i, n, m), v);
+    } else {
       const Shape& sh = out.sh;
-      if (sh.rows > sh.cols) {                          // leaves transposed, below
-#pragma unroll
-        for (int j = 0; j < 8; ++j) at[j] = v[j];
-      } else if (n < sh.r) {
-        typename E::T* o = (typename E::T*)out.ms.out[i] + (int64_t)n * sh.cols + m;
-        leave<DT, KIND == LAST_MUON>(o, v, sh.L - m, out.u);
-      }
+      if (!turn && n < sh.r)
+        leave<DT, KIND == LAST_MUON>((typename Elem<DT>::T*)out.ms.out[i] + (int64_t)n * sh.cols + m, v, sh.L - m, out.u);
     }
   }
-  const bool turn = KIND < APPLY ? bm != bn : KIND > APPLY && tall(out);
   if (!turn) return;
-  stage_ready<0>();
+  ready<0>();
 #pragma unroll 4
-  for (int row = lane / PER_ROW; row < W; row += 64 / PER_ROW) {
+  for (int row = group * SHARE + lane / PER_ROW; row < (group + 1) * SHARE; row += 64 / PER_ROW) {
     const int col = lane % PER_ROW * 8, m = bm * T + m0 + row, n = bn * T + n0 + col;
     float v[8];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] = mine[(col + j) * PITCH + row];
+    for (int j = 0; j < 8; ++j) v[j] = sums[(col + j) * PITCH + row];
     if constexpr (KIND < APPLY) store_pairs(pr.D.hi(i, m, n), v);
     if constexpr (KIND > APPLY) {
       const Shape& sh = out.sh;
@@ -440,14 +448,14 @@ Work layout(int n, const Shape& sh, char* base) {
   return w;
 }
 
-// Tiles of 128 where the matrices have enough of them to occupy the 256 CUs, else of 64
+// Tiles of 128 where the matrices have enough of them to occupy half of the 256 CUs, else of 64
 Shape shape_of(int n, int64_t rows, int64_t cols) {
   Shape s;
   s.rows = (int)rows, s.cols = (int)cols;
   s.r = (int)(rows < cols ? rows : cols), s.L = (int)(rows < cols ? cols : rows);
   const int64_t tr = up(s.r, 128) / 128, tL = up(s.L, 128) / 128;
-  s.tile_r = n * tr * (tr + 1) / 2 >= 256 ? 128 : 64;
-  s.tile_L = n * tr * tL >= 256 ? 128 : 64;
+  s.tile_r = n * tr * (tr + 1) / 2 >= 128 ? 128 : 64;
+  s.tile_L = n * tr * tL >= 128 ? 128 : 64;
   s.rp = (int)up(s.r, s.tile_r > s.tile_L ? s.tile_r : s.tile_L);
   s.Lp = (int)up(s.L, s.tile_L);
   const int64_t parts = up(rows * cols, 8 * NT * 2) / (8 * NT * 2);   // two rounds each at least
@@ -498,12 +506,18 @@ int launched(const char* what) {
   return e == hipSuccess ? 0 : ops_error(MTAZ_E_DEVICE, what, hipGetErrorString(e));
 }
 
+// Up to one tile a CU: the whole LDS for the ring, and waves that share the depth, so that each SIMD has work while
+// another wave waits.  More tiles: two workgroups a CU.
 template <int KIND, int DT, typename Out>
 void product(Product pr, int T, const Out& out, hipStream_t s) {
   const unsigned grid = (unsigned)(pr.tiles * pr.n);
-  if (T == 128) k_product<128, 2, KIND, DT, Out><<<grid, NT, 0, s>>>(pr, out);
-  else if (grid <= 256) k_product<64, 8, KIND, DT, Out><<<grid, NT, 0, s>>>(pr, out);   // a CU each: deeper
-  else k_product<64, 4, KIND, DT, Out><<<grid, NT, 0, s>>>(pr, out);
+  if (T == 128) {
+    if (grid <= 256) k_product<128, 2, 2, 32, 4, KIND, DT, Out><<<grid, 512, 0, s>>>(pr, out);
+    else k_product<128, 2, 1, 32, 2, KIND, DT, Out><<<grid, 256, 0, s>>>(pr, out);
+  } else {
+    if (grid <= 256) k_product<64, 1, 4, 64, 4, KIND, DT, Out><<<grid, 256, 0, s>>>(pr, out);
+    else k_product<64, 1, 4, 64, 2, KIND, DT, Out><<<grid, 256, 0, s>>>(pr, out);
+  }
 }
 
 template <int DT, bool MUON>
