@@ -186,6 +186,8 @@ struct Leave {          // what LAST_* needs besides
   Update u;
 };
 struct Stay {};
+struct Yes { static constexpr bool value = true; };
+struct No { static constexpr bool value = false; };
 
 // 16 bytes a lane straight into LDS; the wave's 64 pieces lie there in lane order
 __device__ __forceinline__ void to_lds(const char* from, uint32_t lane_offset, _Float16* lds) {
@@ -209,25 +211,47 @@ __device__ __forceinline__ f16x8 read_rows(const _Float16* lds, int m, int p) {
 // Columns in LDS: rows of T / 32 lines; piece p of row k at p ^ ((k & 3) << 2), so that the four rows that a
 // transposing read touches (64 B each) lie in different banks.
 __device__ __forceinline__ int col_piece(int k, int p) { return p ^ ((k & 3) << 2); }
-// elements k .. k + 7 of column m (k a multiple of 8, m = the lane's): two transposing reads of 4 rows x 16 columns
-template <int T>
-__device__ __forceinline__ f16x8 read_cols(const _Float16* lds, int m0, int k0, int lo, int lane) {
-  const int q = lane & 15, col = ((lane >> 4) & 1) * 16 + (q & 3) * 4;   // within the line of m0
-  const int p = (m0 >> 5) * 8 + lo * 4 + (col >> 3);
-  f16x8 r;
+// For F groups of 32 columns from m0 on: elements k .. k + 7 (k = k0 + 8 for the upper half wave) of the lane's column,
+// their hi halves and their lo halves; each is two transposing reads of 4 rows x 16 columns.  In one block of
+// assembly that ends with its own wait, because the compiler would have every such read wait for all loads on
+// their way into LDS.
+template <int T, int F>
+__device__ __forceinline__ void read_cols(const _Float16* lds, int m0, int k0, int lane, f16x8* hi, f16x8* lo) {
+  const int q = lane & 15, col = ((lane >> 4) & 1) * 16 + (q & 3) * 4;   // within a group
+  const int k = k0 + (lane >> 5) * 8 + (q >> 2);                        // k & 3 is that of k + 4 too
+  const uint32_t base = (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) char*)lds +
+                        k * 4 * T + (col & 7) * 2;
+  f16x4 v[F][4];
 #pragma unroll
-  for (int h = 0; h < 2; ++h) {
-    const int k = k0 + (lane >> 5) * 8 + h * 4 + (q >> 2);
-    const _Float16* at = lds + k * 2 * T + col_piece(k, p) * 8 + (col & 7);
-    const s16x4 v = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-        (__attribute__((address_space(3))) s16x4*)const_cast<_Float16*>(at));
-    const f16x4 f = __builtin_bit_cast(f16x4, v);
-#pragma unroll
-    for (int j = 0; j < 4; ++j) r[4 * h + j] = f[j];
+  for (int f = 0; f < F; f += 2) {
+    const int p = ((m0 >> 5) + f) * 8 + (col >> 3);
+    const uint32_t h0 = base + col_piece(k, p) * 16, l0 = base + col_piece(k, p + 4) * 16;
+    const uint32_t h1 = base + col_piece(k, p + 8) * 16, l1 = base + col_piece(k, p + 12) * 16;
+    asm volatile(
+        "ds_read_b64_tr_b16 %0, %8\n\tds_read_b64_tr_b16 %1, %8 offset:%12\n\t"
+        "ds_read_b64_tr_b16 %2, %9\n\tds_read_b64_tr_b16 %3, %9 offset:%12\n\t"
+        "ds_read_b64_tr_b16 %4, %10\n\tds_read_b64_tr_b16 %5, %10 offset:%12\n\t"
+        "ds_read_b64_tr_b16 %6, %11\n\tds_read_b64_tr_b16 %7, %11 offset:%12\n\t"
+        "s_waitcnt lgkmcnt(0)"
+        : "=&v"(v[f][0]), "=&v"(v[f][1]), "=&v"(v[f][2]), "=&v"(v[f][3]), "=&v"(v[f + 1][0]), "=&v"(v[f + 1][1]),
+          "=&v"(v[f + 1][2]), "=&v"(v[f + 1][3])
+        : "v"(h0), "v"(l0), "v"(h1), "v"(l1), "n"(16 * T)
+        : "memory");
   }
-  return r;
+#pragma unroll
+  for (int f = 0; f < F; ++f) {
+    hi[f] = __builtin_shufflevector(v[f][0], v[f][1], 0, 1, 2, 3, 4, 5, 6, 7);
+    lo[f] = __builtin_shufflevector(v[f][2], v[f][3], 0, 1, 2, 3, 4, 5, 6, 7);
+  }
 }
 
+// the row of element t of a lower triangle, row by row
+__device__ __forceinline__ int triangle_row(int t) {
+  int row = (int)((sqrtf(8.f * t + 1.f) - 1.f) * 0.5f);
+  if ((row + 1) * (row + 2) / 2 <= t) ++row;
+  if (row * (row + 1) / 2 > t) --row;
+  return row;
+}
 __device__ __forceinline__ bool tall(const Stay&) { return false; }
 __device__ __forceinline__ bool tall(const Leave& l) { return l.sh.rows > l.sh.cols; }
 // up to eight consecutive results into the output or the parameter
@@ -259,23 +283,30 @@ void k_product(Product pr, Out out) {
   constexpr int PITCH = W + 4, PART = W * PITCH;        // floats of a wave's sums in LDS
   constexpr int LOOP = RING * 2 * HALF * 2, END = WAVES * PART * 4;
   static_assert(T * DEPTH % (256 * WAVES) == 0 && DEPTH % (16 * GROUPS) == 0 && 64 % DEPTH == 0, "round");
+  static_assert(F % 2 == 0, "read_cols");
   __shared__ __attribute__((aligned(1024))) char shared[LOOP > END ? LOOP : END];
   _Float16* lds = reinterpret_cast<_Float16*>(shared);
   const int lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
   const int part = wave % (SIDE * SIDE), group = wave / (SIDE * SIDE);
-  // Workgroups go round the 8 XCDs in turn; give each XCD one contiguous run of tiles, so that the tiles that share
-  // rows or columns share an L2.
+  // Workgroups go round the 8 XCDs in turn; give each XCD one contiguous run of tiles, and order the tiles in bands,
+  // so that those an XCD works on at a time share rows and columns in its L2.
   const int total = pr.tiles * pr.n, xcd = blockIdx.x % 8, nth = blockIdx.x / 8;
   const int id = xcd * (total / 8) + min(xcd, total % 8) + nth;
   const int i = id / pr.tiles, t = id % pr.tiles;
   int bm, bn;
-  if (COLS) {
-    bm = t % pr.tiles_m, bn = t / pr.tiles_m;
-  } else {                                              // lower triangle, row by row
-    bm = (int)((sqrtf(8.f * t + 1.f) - 1.f) * 0.5f);
-    if ((bm + 1) * (bm + 2) / 2 <= t) ++bm;
-    if (bm * (bm + 1) / 2 > t) --bm;
-    bn = t - bm * (bm + 1) / 2;
+  if (COLS) {                                           // bands of 8 tiles along n, n the faster within a band
+    const int band = t / (8 * pr.tiles_m), in = t - band * 8 * pr.tiles_m;
+    const int high = min(8, pr.tiles / pr.tiles_m - band * 8);
+    bm = in / high, bn = band * 8 + in % high;
+  } else {                                              // lower triangle in bands of 8 rows: a band's square columns,
+    const int first = triangle_row(t) & ~7, in = t - first * (first + 1) / 2;   // then its triangle
+    const int high = min(8, triangle_row(pr.tiles - 1) + 1 - first);
+    if (in < first * high) {
+      bm = first + in % high, bn = in / high;
+    } else {
+      const int rest = in - first * high, row = triangle_row(rest);
+      bm = first + row, bn = first + rest - row * (row + 1) / 2;
+    }
   }
   const char* const from_p = (const char*)(COLS ? pr.P.hi(i, 0, bm * T) : pr.P.hi(i, bm * T, 0));
   const char* const from_q = (const char*)pr.Q.hi(i, bn * T, 0);
@@ -296,13 +327,10 @@ void k_product(Product pr, Out out) {
     }
   }
   const int64_t step_p = COLS ? (int64_t)DEPTH * pr.P.pitch * 2 : DEPTH * 4, step_q = DEPTH * 4;
-  auto load = [&](int round, int buf) {
-#pragma unroll
-    for (int c = 0; c < CH; ++c) {
-      const int chunk = wave + WAVES * c;
-      to_lds(from_p + round * step_p, at_p[c], lds + buf * 2 * HALF + chunk * 512);
-      to_lds(from_q + round * step_q, at_q[c], lds + buf * 2 * HALF + HALF + chunk * 512);
-    }
+  auto load = [&](int round, int buf, int c) {          // one piece of P and one of Q
+    const int chunk = wave + WAVES * c;
+    to_lds(from_p + round * step_p, at_p[c], lds + buf * 2 * HALF + chunk * 512);
+    to_lds(from_q + round * step_q, at_q[c], lds + buf * 2 * HALF + HALF + chunk * 512);
   };
   const int m0 = part % SIDE * W, n0 = part / SIDE * W;
   const int rounds = pr.k / DEPTH;
@@ -310,13 +338,14 @@ void k_product(Product pr, Out out) {
   f32x16 acc[F][F] = {};
 #pragma unroll
   for (int r = 0; r < AHEAD; ++r)
-    if (r < rounds) load(r, r);
+    if (r < rounds)
+#pragma unroll
+      for (int c = 0; c < CH; ++c) load(r, r, c);
   int buf = 0;
-  for (int r = 0; r < rounds; ++r) {
-    // of the rounds loaded so far, all but the newest AHEAD - 1 have to be there; near the end fewer were loaded
-    if (r + AHEAD - 1 < rounds) ready<2 * CH * (AHEAD - 1)>();
-    else ready<0>();
-    if (r + AHEAD < rounds) load(r + AHEAD, buf == 0 ? RING - 1 : buf - 1);   // over the round read last
+  // One round's products.  Its loads (of the round AHEAD, over the one read last) are issued between the products:
+  // a wave issues in order, and the address path takes 1 KiB pieces too slowly to have them ahead of everything.
+  auto multiply = [&](int r, auto loads) {
+    const int over = buf == 0 ? RING - 1 : buf - 1;
     const _Float16 *p = lds + buf * 2 * HALF, *q = p + HALF;
     buf = buf + 1 == RING ? 0 : buf + 1;
 #pragma unroll
@@ -326,17 +355,15 @@ void k_product(Product pr, Out out) {
       f16x8 ah[F], al[F], bh[F], bl[F];
 #pragma unroll
       for (int f = 0; f < F; ++f) {
-        const int m = m0 + 32 * f, n = n0 + 32 * f + (lane & 31);
-        if (COLS) {
-          ah[f] = read_cols<T>(p, m, kk, 0, lane);
-          al[f] = read_cols<T>(p, m, kk, 1, lane);
-        } else {
-          ah[f] = read_rows(p + line, m + (lane & 31), piece);
-          al[f] = read_rows(p + line, m + (lane & 31), piece + 4);
+        const int m = m0 + 32 * f + (lane & 31), n = n0 + 32 * f + (lane & 31);
+        if (!COLS) {
+          ah[f] = read_rows(p + line, m, piece);
+          al[f] = read_rows(p + line, m, piece + 4);
         }
         bh[f] = read_rows(q + line, n, piece);
         bl[f] = read_rows(q + line, n, piece + 4);
       }
+      if (COLS) read_cols<T, F>(p, m0, kk, lane, ah, al);
 #pragma unroll
       for (int f = 0; f < F; ++f)
 #pragma unroll
@@ -344,8 +371,24 @@ void k_product(Product pr, Out out) {
           acc[f][g] = __builtin_amdgcn_mfma_f32_32x32x16_f16(al[f], bh[g], acc[f][g], 0, 0, 0);
           acc[f][g] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ah[f], bl[g], acc[f][g], 0, 0, 0);
           acc[f][g] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ah[f], bh[g], acc[f][g], 0, 0, 0);
+          if constexpr (decltype(loads)::value) {
+            constexpr int ALL = STEPS * F * F;
+            const int at = (step * F + f) * F + g;
+#pragma unroll
+            for (int c = at * CH / ALL; c < (at + 1) * CH / ALL; ++c) load(r + AHEAD, over, c);
+            __builtin_amdgcn_sched_barrier(0x7);        // arithmetic may move, products, loads and LDS reads not
+          }
         }
     }
+  };
+  int r = 0;
+  for (; r + AHEAD < rounds; ++r) {
+    ready<2 * CH * (AHEAD - 1)>();                      // all rounds loaded so far but the newest AHEAD - 1
+    multiply(r, Yes{});
+  }
+  for (; r < rounds; ++r) {
+    ready<0>();
+    multiply(r, No{});
   }
 
   // The sums through LDS as [n][m], so that memory is read and written along rows: a lane holds column n and, four
