@@ -460,6 +460,261 @@ void k_product(Product pr, Out out) {
   }
 }
 
+// ---- small matrices ------------------------------------------------------------------------------------------------
+// A matrix that fits into one CU's LDS together with its r x r products is taken through all steps there, by one
+// workgroup of 16 waves in one launch: memory is read once and the result written.  X lies in LDS as hi and lo planes
+// [r16][pitch], S and then B as [r16][pitch_s]; the 16-byte piece p of row m is at p ^ (m >> 1 & 7), and the pitches are
+// odd multiples of 128 bytes where there is room, so that the 16 rows of an operand lie in different banks.  Products
+// are 16 x 16 x 32: a wave takes whole tiles of S and B (on and below the diagonal, written twice) and whole strips of
+// 16 columns of X, which it reads before it overwrites them.
+constexpr int SMALL_WAVES = 16;
+constexpr int SMALL_LDS = 160 * 1024;
+constexpr int SMALL_ROWS = 128;                         // r at most: three tiles of S a wave
+struct Small {
+  int r16, strips, pitch, pitch_s;                      // padded short side, 16 columns each; halves from row to row
+};
+struct Factors {                                        // of GRAM, POLY (S S, S, diagonal) and APPLY, per step
+  float gram[MTAZ_MAX_STEPS], square[MTAZ_MAX_STEPS], self[MTAZ_MAX_STEPS], one[MTAZ_MAX_STEPS], apply[MTAZ_MAX_STEPS];
+};
+// where column c of row m lies in its row
+__device__ __forceinline__ int small_at(int m, int c) { return row_piece(m, c >> 3) * 8 + (c & 7); }
+
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+// 16 x 16 sums of hi hi, hi lo and lo hi over one instruction's depth
+struct Sums {
+  f32x4 main = {}, cross = {}, cross2 = {};
+  __device__ __forceinline__ void add(f16x8 ah, f16x8 al, f16x8 bh, f16x8 bl) {
+    main = __builtin_amdgcn_mfma_f32_16x16x32_f16(ah, bh, main, 0, 0, 0);
+    cross = __builtin_amdgcn_mfma_f32_16x16x32_f16(ah, bl, cross, 0, 0, 0);
+    cross2 = __builtin_amdgcn_mfma_f32_16x16x32_f16(al, bh, cross2, 0, 0, 0);
+  }
+  __device__ __forceinline__ f32x4 sum() const { return main + (cross + cross2); }
+};
+
+// P P^T for rows [16 a, +16) and [16 b, +16) of the planes at hi: k runs along the rows, `depth` a multiple of 32
+__device__ __forceinline__ f32x4 gram_tile(const _Float16* hi, int lo, int pitch, int depth, int a, int b, int lane) {
+  const int ma = 16 * a + (lane & 15), mb = 16 * b + (lane & 15), k = (lane >> 4) * 8;
+  const _Float16 *pa = hi + ma * pitch, *pb = hi + mb * pitch;
+  auto at = [&](const _Float16* p, int m, int k0) { return *reinterpret_cast<const f16x8*>(p + small_at(m, k0 + k)); };
+  Sums s;
+  if (a == b) {
+    for (int k0 = 0; k0 < depth; k0 += 32) {
+      const f16x8 ah = at(pa, ma, k0), al = at(pa + lo, ma, k0);
+      s.add(ah, al, ah, al);
+    }
+  } else {
+    for (int k0 = 0; k0 < depth; k0 += 32) s.add(at(pa, ma, k0), at(pa + lo, ma, k0), at(pb, mb, k0), at(pb + lo, mb, k0));
+  }
+  return s.sum();
+}
+
+__device__ __forceinline__ void split4(f32x4 v, f16x4& h, f16x4& l) {
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    _Float16 hj, lj;
+    split(v[j], hj, lj);
+    h[j] = hj, l[j] = lj;
+  }
+}
+// a tile's result into the symmetric planes: a lane holds column 16 b + (lane & 15), rows 16 a + 4 (lane >> 4) + j
+__device__ __forceinline__ void put_tile(_Float16* hi, int lo, int pitch, int a, int b, f32x4 v, int lane) {
+  f16x4 h, l;
+  split4(v, h, l);
+  const int m = 16 * a + 4 * (lane >> 4), n = 16 * b + (lane & 15);
+  _Float16* to = hi + n * pitch + small_at(n, m);
+  *reinterpret_cast<f16x4*>(to) = h;
+  *reinterpret_cast<f16x4*>(to + lo) = l;
+  if (a != b)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      to = hi + (m + j) * pitch + small_at(m + j, n);
+      to[0] = h[j], to[lo] = l[j];
+    }
+}
+
+// DEEP: instructions deep that B X goes at most, r16 / 32 rounded up to 1, 2 or 4; a wave takes up to WIDE strips of X at
+// a time, so that a part of B once read serves them all.
+template <int DT, bool MUON, int DEEP>
+__global__ __launch_bounds__(64 * SMALL_WAVES) void k_small(Matrices ms, Shape sh, Small sm, Update u, int steps,
+                                                            double eps, double unit, Factors fa) {
+  typedef Elem<DT> E;
+  constexpr int ALL = 64 * SMALL_WAVES;
+  __shared__ __attribute__((aligned(1024))) char shared[SMALL_LDS];
+  const int i = blockIdx.x, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
+  int lane = threadIdx.x % 64;
+  const typename E::T* g = (const typename E::T*)ms.grad[i];
+  float* mom = ms.momentum[i];
+  typename E::T* out = (typename E::T*)ms.out[i];
+  const bool tall = sh.rows > sh.cols;
+
+  // the steps' factors, lane t those of step t
+  const int mine = min(lane, MTAZ_MAX_STEPS - 1);
+  const float f_gram = fa.gram[mine], f_square = fa.square[mine], f_self = fa.self[mine], f_one = fa.one[mine],
+              f_apply = fa.apply[mine];
+
+  // The matrix, eight elements at a time: all of a thread's share (LDS holds 40 Ki pairs) is under way at once and
+  // stays in registers until the norm, summed in 64 bits, is known.  Momentum is brought up to date on the way.
+  constexpr int N = 8, PACKS = SMALL_LDS / 4 / (ALL * N);
+  const int count = sh.rows * sh.cols;
+  Pack<typename E::T, N> gv[PACKS];
+  Pack<float, N> mv[PACKS];
+#pragma unroll
+  for (int c = 0; c < PACKS; ++c) {
+    const int k = N * (threadIdx.x + ALL * c), n = count - k;
+    if (n >= N) {
+      gv[c] = *reinterpret_cast<const Pack<typename E::T, N>*>(g + k);
+      if (MUON) mv[c] = *reinterpret_cast<const Pack<float, N>*>(mom + k);
+    } else {
+#pragma unroll
+      for (int j = 0; j < N; ++j) gv[c].v[j] = j < n ? g[k + j] : (typename E::T)0.f, mv[c].v[j] = MUON && j < n ? mom[k + j] : 0.f;
+    }
+  }
+  _Float16* const X = reinterpret_cast<_Float16*>(shared);
+  const int lo = sm.r16 * sm.pitch, lo_s = sm.r16 * sm.pitch_s;
+  _Float16* const S = X + 2 * lo;
+  for (int k = threadIdx.x; k < (lo + lo_s) / 4; k += ALL) reinterpret_cast<f16x8*>(X)[k] = f16x8{};   // the padding
+  __syncthreads();
+  double sq = 0.;
+#pragma unroll
+  for (int c = 0; c < PACKS; ++c) {
+    const int k = N * (threadIdx.x + ALL * c), n = count - k;
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+      const float x = E::get(gv[c].v[j]);
+      float m = mv[c].v[j];
+      if (MUON) {
+        m = fmaf(u.momentum, m, (1.f - u.momentum) * x);
+        if (j < n) mom[k + j] = m;
+      }
+      mv[c].v[j] = update_of<DT, MUON>(x, m, u);
+      const double y = (double)mv[c].v[j];
+      sq = fma(y, y, sq);
+    }
+  }
+  double* sums = reinterpret_cast<double*>(S);
+  for (int o = 32; o; o >>= 1) sq += __shfl_xor(sq, o);
+  if (lane == 0) sums[wave] = sq;
+  __syncthreads();
+  double norm = 0.;
+  for (int w = 0; w < SMALL_WAVES; ++w) norm += sums[w];
+  const double inv = unit / (sqrt(norm) + eps);
+  __syncthreads();
+  if (threadIdx.x < SMALL_WAVES) sums[threadIdx.x] = 0.;
+#pragma unroll
+  for (int c = 0; c < PACKS; ++c) {
+    const int k = N * (threadIdx.x + ALL * c);
+    int row = k / sh.cols, col = k - row * sh.cols;     // in memory
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+      if (k + j < count) {
+        const int m = tall ? col : row, n = tall ? row : col, to = m * sm.pitch + small_at(m, n);
+        _Float16 h, l;
+        split((float)((double)mv[c].v[j] * inv), h, l);
+        X[to] = h, X[to + lo] = l;
+      }
+      if (++col == sh.cols) col = 0, ++row;
+    }
+  }
+  __syncthreads();
+
+  const int R = sm.r16 / 16, tiles = R * (R + 1) / 2;
+  constexpr int MINE = (SMALL_ROWS / 16) * (SMALL_ROWS / 16 + 1) / 2 / SMALL_WAVES + 1;   // tiles of S a wave
+  for (int step = 0; step < steps; ++step) {
+    asm volatile("" : "+v"(lane));                      // addresses are computed in each step, not kept (and spilled) over all
+    const float k_gram = __shfl(f_gram, step), k_square = __shfl(f_square, step), k_self = __shfl(f_self, step),
+                k_one = __shfl(f_one, step), k_apply = __shfl(f_apply, step);
+    for (int t = wave; t < tiles; t += SMALL_WAVES) {
+      const int a = triangle_row(t), b = t - a * (a + 1) / 2;
+      put_tile(S, lo_s, sm.pitch_s, a, b, k_gram * gram_tile(X, lo, sm.pitch, (16 * sm.strips + 31) & ~31, a, b, lane), lane);
+    }
+    __syncthreads();
+    f32x4 v[MINE];
+#pragma unroll
+    for (int c = 0; c < MINE; ++c) {
+      const int t = wave + SMALL_WAVES * c;
+      if (t >= tiles) continue;
+      const int a = triangle_row(t), b = t - a * (a + 1) / 2, m = 16 * a + 4 * (lane >> 4), n = 16 * b + (lane & 15);
+      const f32x4 ss = gram_tile(S, lo_s, sm.pitch_s, (sm.r16 + 31) & ~31, a, b, lane);
+      const _Float16* self = S + n * sm.pitch_s + small_at(n, m);
+      const f16x4 h = *reinterpret_cast<const f16x4*>(self), l = *reinterpret_cast<const f16x4*>(self + lo_s);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        v[c][j] = fmaf(k_self, (float)h[j] + (float)l[j], k_square * ss[j]);
+        if (m + j == n) v[c][j] += k_one;
+      }
+    }
+    __syncthreads();                                    // S is read; B takes its place
+#pragma unroll
+    for (int c = 0; c < MINE; ++c) {
+      const int t = wave + SMALL_WAVES * c;
+      if (t >= tiles) continue;
+      const int a = triangle_row(t), b = t - a * (a + 1) / 2;
+      put_tile(S, lo_s, sm.pitch_s, a, b, v[c], lane);
+    }
+    __syncthreads();
+    const bool last = step + 1 == steps;
+    constexpr int WIDE = DEEP == 4 ? 1 : 2;
+    const int q = lane & 15, g8 = (lane >> 4) * 8;
+    for (int strip = wave * WIDE; strip < sm.strips; strip += SMALL_WAVES * WIDE) {
+      // The strips' columns as the first operand, k = rows of X: two transposing reads of 4 rows x 16 columns for 8 rows
+      // a lane.  A transposing read runs in all lanes, whatever the mask: the lanes behind the last row read rows that are
+      // there (r16 is a multiple of 16) and drop what they got, and so do strips behind the last.
+      f16x8 ah[WIDE][DEEP], al[WIDE][DEEP];
+#pragma unroll
+      for (int w = 0; w < WIDE; ++w) {
+        const int first = 16 * min(strip + w, sm.strips - 1) + (q & 3) * 4;
+#pragma unroll
+        for (int d = 0; d < DEEP; ++d) {
+          const bool there = 32 * d + g8 < sm.r16;
+          const int row = there ? 32 * d + g8 + (q >> 2) : q >> 2;
+          f16x4 part[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e)                   // hi of rows row, row + 4; lo
+            part[e] = __builtin_bit_cast(f16x4, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                (__attribute__((address_space(3))) s16x4*)(X + (e >> 1) * lo + (row + 4 * (e & 1)) * sm.pitch +
+                                                          small_at(row + 4 * (e & 1), first))));
+          const f16x8 h = __builtin_shufflevector(part[0], part[1], 0, 1, 2, 3, 4, 5, 6, 7);
+          const f16x8 l = __builtin_shufflevector(part[2], part[3], 0, 1, 2, 3, 4, 5, 6, 7);
+          ah[w][d] = there ? h : f16x8{}, al[w][d] = there ? l : f16x8{};
+        }
+      }
+      for (int tile = 0; tile < R; ++tile) {
+        const int row = 16 * tile + q;
+        const _Float16* pb = S + row * sm.pitch_s;
+        Sums s[WIDE];
+#pragma unroll
+        for (int d = 0; d < DEEP; ++d) {                // behind r16 X is 0 here, and B in its padding
+          const _Float16* at = pb + (32 * d < sm.r16 ? small_at(row, 32 * d + g8) : 0);
+          const f16x8 bh = *reinterpret_cast<const f16x8*>(at), bl = *reinterpret_cast<const f16x8*>(at + lo_s);
+#pragma unroll
+          for (int w = 0; w < WIDE; ++w) s[w].add(ah[w][d], al[w][d], bh, bl);
+        }
+#pragma unroll
+        for (int w = 0; w < WIDE; ++w) {
+          const int col = 16 * (strip + w) + (lane >> 4) * 4;
+          if (strip + w >= sm.strips) continue;
+          const f32x4 x = k_apply * s[w].sum();
+          if (!last) {
+            f16x4 h, l;
+            split4(x, h, l);
+            _Float16* to = X + row * sm.pitch + small_at(row, col);
+            *reinterpret_cast<f16x4*>(to) = h;
+            *reinterpret_cast<f16x4*>(to + lo) = l;
+          } else if (row < sh.r) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              if (col + j >= sh.L) continue;
+              typename E::T* o = out + (tall ? (col + j) * sh.cols + row : row * sh.cols + col + j);
+              *o = E::put(MUON ? fmaf(u.keep, E::get(*o), -u.step * x[j]) : x[j]);
+            }
+          }
+        }
+      }
+    }
+    __syncthreads();
+  }
+}
+
 // ---- host --------------------------------------------------------------------------------------------------------
 int64_t up(int64_t x, int64_t m) { return (x + m - 1) / m * m; }
 
@@ -516,29 +771,33 @@ const char* bad_shape(int n, int64_t rows, int64_t cols, int dtype) {
 
 // Exponents that keep every entry below 2^14: of X before each step and after the last, of S and of B.
 // Singular values start in [0, 1]; after a step they lie below the largest |s (a + b s^2 + c s^4)| over the range
-// before it, S below its square and B below the largest |a + b s^2 + c s^4|.  The maxima are taken over a grid that holds
-// the range's end, where a polynomial between two of 4096 points exceeds the larger one by some 10^-7 of its
-// maximum, with a thousandth on top for that and for roundings; f16 has room for twice 2^14 besides.
+// before it, S below its square and B below the largest |a + b s^2 + c s^4|: both are taken at the range's ends and
+// where the derivative vanishes, with a thousandth on top for roundings; f16 has room for twice 2^14 besides.
 struct Exponents {
   int x[MTAZ_MAX_STEPS + 1], s[MTAZ_MAX_STEPS], b[MTAZ_MAX_STEPS];
 };
 const char* bounds(int steps, const double* co, Exponents& e) {
-  double top = 1.;
+  const double a = co[0], b = co[1], c = co[2];
+  auto q = [&](double t) { return fabs(a + t * (b + t * c)); };   // of t = s^2
   auto unit = [](double bound) {
-    const int k = 14 - (int)ceil(log2(bound));
+    const int k = 14 - (int)ceil(log2(1.001 * bound));
     return k > 40 ? 40 : k;
   };
+  // of s q(s^2): a + 3 b t + 5 c t^2 = 0 (one of the two forms of each root is exact where c is small or 0)
+  const double disc = 9. * b * b - 20. * a * c, root = disc > 0. ? sqrt(disc) : 0., z = -3. * b - copysign(root, b);
+  const double at[2] = {disc >= 0. && c != 0. ? z / (10. * c) : -1., disc >= 0. && z != 0. ? 2. * a / z : -1.};
+  double top = 1.;
   for (int t = 0; t <= steps; ++t) {
     if (!(top <= 1e6)) return "the coefficients let the singular values grow past 10^6";
-    e.x[t] = unit(top > 1e-9 ? top : 1e-9);
+    e.x[t] = unit(fmax(top, 1e-9));
     if (t == steps) break;
-    double next = 0., poly = 0.;
-    for (int k = 0; k <= 4096; ++k) {
-      const double s = top * k / 4096., q = co[0] + co[1] * s * s + co[2] * s * s * s * s;
-      next = fmax(next, fabs(s * q)), poly = fmax(poly, fabs(q));
-    }
-    e.s[t] = unit(fmax(1.001 * top * top, 1e-9));
-    e.b[t] = unit(fmax(1.001 * poly, 1e-9));
+    const double end = top * top;
+    double next = top * q(end), poly = fmax(q(0.), q(end));
+    for (double s2 : at)
+      if (s2 > 0. && s2 < end) next = fmax(next, sqrt(s2) * q(s2));
+    if (c != 0. && -b / (2. * c) > 0. && -b / (2. * c) < end) poly = fmax(poly, q(-b / (2. * c)));
+    e.s[t] = unit(fmax(end, 1e-9));
+    e.b[t] = unit(fmax(poly, 1e-9));
     top = 1.001 * next;
   }
   return nullptr;
@@ -547,6 +806,17 @@ const char* bounds(int steps, const double* co, Exponents& e) {
 int launched(const char* what) {
   const hipError_t e = hipGetLastError();
   return e == hipSuccess ? 0 : ops_error(MTAZ_E_DEVICE, what, hipGetErrorString(e));
+}
+
+bool small(const Shape& sh, Small& sm) {
+  sm.r16 = (int)up(sh.r, 16), sm.strips = (int)up(sh.L, 16) / 16;
+  if (sm.r16 > SMALL_ROWS) return false;
+  auto fits = [&](int a, int b) {
+    sm.pitch = a, sm.pitch_s = b;
+    return 4ll * sm.r16 * (a + b) <= SMALL_LDS;
+  };
+  const int a = (int)up(sh.L, 64), b = (int)up(sh.r, 64);
+  return fits(a | 64, b | 64) || fits(a | 64, b) || fits(a, b | 64) || fits(a, b);
 }
 
 // Up to one tile a CU: the whole LDS for the ring, and waves that share the depth, so that each SIMD has work while
@@ -566,6 +836,21 @@ void product(Product pr, int T, const Out& out, hipStream_t s) {
 template <int DT, bool MUON>
 void iterate(const Matrices& ms, int n, const Shape& sh, const Update& u, int steps, const double* co, double eps,
              const Exponents& e, char* base, hipStream_t s) {
+  Small sm;
+  if (small(sh, sm)) {
+    Factors fa = {};
+    for (int t = 0; t < steps; ++t) {
+      fa.gram[t] = (float)ldexp(1., e.s[t] - 2 * e.x[t]);
+      fa.square[t] = (float)ldexp(co[2], e.b[t] - 2 * e.s[t]), fa.self[t] = (float)ldexp(co[1], e.b[t] - e.s[t]);
+      fa.one[t] = (float)ldexp(co[0], e.b[t]);
+      fa.apply[t] = (float)ldexp(1., (t + 1 < steps ? e.x[t + 1] : 0) - e.x[t] - e.b[t]);
+    }
+    const double unit = ldexp(1., e.x[0]);
+    if (sm.r16 <= 32) k_small<DT, MUON, 1><<<n, 64 * SMALL_WAVES, 0, s>>>(ms, sh, sm, u, steps, eps, unit, fa);
+    else if (sm.r16 <= 64) k_small<DT, MUON, 2><<<n, 64 * SMALL_WAVES, 0, s>>>(ms, sh, sm, u, steps, eps, unit, fa);
+    else k_small<DT, MUON, 4><<<n, 64 * SMALL_WAVES, 0, s>>>(ms, sh, sm, u, steps, eps, unit, fa);
+    return;
+  }
   const Work w = layout(n, sh, base);
   const int64_t count = (int64_t)sh.rows * sh.cols;
   k_squares<DT, MUON><<<dim3(sh.parts, n), NT, 0, s>>>(ms, count, u, w.part);
@@ -588,7 +873,9 @@ void iterate(const Matrices& ms, int n, const Shape& sh, const Update& u, int st
 // of the largest group; a smaller last one may choose smaller tiles, never larger ones
 int64_t workspace(int n, int64_t rows, int64_t cols) {
   const int m = n < MOST ? n : MOST;
-  return layout(m, shape_of(m, rows, cols), nullptr).bytes;
+  const Shape sh = shape_of(m, rows, cols);
+  Small sm;
+  return small(sh, sm) ? 256 : layout(m, sh, nullptr).bytes;
 }
 
 // All checks, then the matrices in groups of at most MOST over the same workspace

@@ -88,6 +88,14 @@ def test_zeros_nan_and_neighbours():
         assert off(got[i], want[i]) <= TIGHT
 
 
+@pytest.mark.parametrize('shape', [(5, 24), (17, 40), (61, 300), (100, 130), (3, 2000), (200, 300)], ids=str)
+def test_nothing_is_left_from_another_matrix(shape):
+    """Matrices of NaN on every CU before: what they leave in LDS must not get into padded rows and columns."""
+    optim.orthogonalize(torch.full((1024, 96, 96), math.nan, device='cuda'))
+    g = randn(2, *shape, seed=12)
+    assert off(optim.orthogonalize(g), reference(g)) <= LOOSE
+
+
 def test_many_matrices_in_groups():
     g = randn(131, 5, 24, seed=8)           # two launches of 64 and one of 3
     got = optim.orthogonalize(g)
