@@ -24,6 +24,7 @@ namespace {
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
 typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef float f32x8 __attribute__((ext_vector_type(8)));
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 
 constexpr int NT = 256;
@@ -114,13 +115,11 @@ __device__ __forceinline__ void split(float x, _Float16& hi, _Float16& lo) {
 
 // eight consecutive elements (a multiple of 8 into the row) as pairs
 __device__ __forceinline__ void store_pairs(_Float16* to, const float* x) {
-  f16x8 h, l;
+  f32x8 v;
 #pragma unroll
-  for (int j = 0; j < 8; ++j) {
-    _Float16 hj, lj;
-    split(x[j], hj, lj);
-    h[j] = hj, l[j] = lj;
-  }
+  for (int j = 0; j < 8; ++j) v[j] = x[j];
+  const f16x8 h = __builtin_convertvector(v, f16x8);
+  const f16x8 l = __builtin_convertvector(v - __builtin_convertvector(h, f32x8), f16x8);
   *reinterpret_cast<f16x8*>(to) = h;
   *reinterpret_cast<f16x8*>(to + 32) = l;
 }
@@ -471,7 +470,8 @@ constexpr int SMALL_WAVES = 16;
 constexpr int SMALL_LDS = 160 * 1024;
 constexpr int SMALL_ROWS = 128;                         // r at most: three tiles of S a wave
 struct Small {
-  int r16, strips, pitch, pitch_s;                      // padded short side, 16 columns each; halves from row to row
+  int r16, strips;                                      // padded short side; 16 columns each of the long side
+  int depth, depth_s, pitch, pitch_s;                   // of X and of S: columns up to a multiple of 64; from row to row
 };
 struct Factors {                                        // of GRAM, POLY (S S, S, diagonal) and APPLY, per step
   float gram[MTAZ_MAX_STEPS], square[MTAZ_MAX_STEPS], self[MTAZ_MAX_STEPS], one[MTAZ_MAX_STEPS], apply[MTAZ_MAX_STEPS];
@@ -491,30 +491,35 @@ struct Sums {
   __device__ __forceinline__ f32x4 sum() const { return main + (cross + cross2); }
 };
 
-// P P^T for rows [16 a, +16) and [16 b, +16) of the planes at hi: k runs along the rows, `depth` a multiple of 32
+// P P^T for rows [16 a, +16) and [16 b, +16) of the planes at hi: k runs along the rows, `depth` a multiple of 64.
+// A lane's rows 16 a + j and 16 b + j are swizzled alike, and 64 columns are one full turn of the swizzle: the lane's
+// places for the two instructions of a turn stay the same from turn to turn.
 __device__ __forceinline__ f32x4 gram_tile(const _Float16* hi, int lo, int pitch, int depth, int a, int b, int lane) {
-  const int ma = 16 * a + (lane & 15), mb = 16 * b + (lane & 15), k = (lane >> 4) * 8;
-  const _Float16 *pa = hi + ma * pitch, *pb = hi + mb * pitch;
-  auto at = [&](const _Float16* p, int m, int k0) { return *reinterpret_cast<const f16x8*>(p + small_at(m, k0 + k)); };
+  const int j = lane & 15, first = small_at(j, (lane >> 4) * 8);
+  const _Float16 *pa = hi + (16 * a + j) * pitch + first, *pb = hi + (16 * b + j) * pitch + first;
+  const int second = first & 32 ? -32 : 32;
+  auto at = [](const _Float16* p) { return *reinterpret_cast<const f16x8*>(p); };
   Sums s;
   if (a == b) {
-    for (int k0 = 0; k0 < depth; k0 += 32) {
-      const f16x8 ah = at(pa, ma, k0), al = at(pa + lo, ma, k0);
+    for (int k = 0; k < depth; k += 64, pa += 64) {
+      const f16x8 ah = at(pa), al = at(pa + lo), ch = at(pa + second), cl = at(pa + lo + second);
       s.add(ah, al, ah, al);
+      s.add(ch, cl, ch, cl);
     }
   } else {
-    for (int k0 = 0; k0 < depth; k0 += 32) s.add(at(pa, ma, k0), at(pa + lo, ma, k0), at(pb, mb, k0), at(pb + lo, mb, k0));
+    for (int k = 0; k < depth; k += 64, pa += 64, pb += 64) {
+      const f16x8 ah = at(pa), al = at(pa + lo), bh = at(pb), bl = at(pb + lo);
+      const f16x8 ch = at(pa + second), cl = at(pa + lo + second), dh = at(pb + second), dl = at(pb + lo + second);
+      s.add(ah, al, bh, bl);
+      s.add(ch, cl, dh, dl);
+    }
   }
   return s.sum();
 }
 
 __device__ __forceinline__ void split4(f32x4 v, f16x4& h, f16x4& l) {
-#pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    _Float16 hj, lj;
-    split(v[j], hj, lj);
-    h[j] = hj, l[j] = lj;
-  }
+  h = __builtin_convertvector(v, f16x4);
+  l = __builtin_convertvector(v - __builtin_convertvector(h, f32x4), f16x4);
 }
 // a tile's result into the symmetric planes: a lane holds column 16 b + (lane & 15), rows 16 a + 4 (lane >> 4) + j
 __device__ __forceinline__ void put_tile(_Float16* hi, int lo, int pitch, int a, int b, f32x4 v, int lane) {
@@ -598,6 +603,8 @@ __global__ __launch_bounds__(64 * SMALL_WAVES) void k_small(Matrices ms, Shape s
   double norm = 0.;
   for (int w = 0; w < SMALL_WAVES; ++w) norm += sums[w];
   const double inv = unit / (sqrt(norm) + eps);
+  int twos;                                             // as a float below 1 and a power of two: in range for any norm
+  const float ones = (float)frexp(inv, &twos);
   __syncthreads();
   if (threadIdx.x < SMALL_WAVES) sums[threadIdx.x] = 0.;
 #pragma unroll
@@ -609,7 +616,7 @@ __global__ __launch_bounds__(64 * SMALL_WAVES) void k_small(Matrices ms, Shape s
       if (k + j < count) {
         const int m = tall ? col : row, n = tall ? row : col, to = m * sm.pitch + small_at(m, n);
         _Float16 h, l;
-        split((float)((double)mv[c].v[j] * inv), h, l);
+        split(ldexpf(mv[c].v[j] * ones, twos), h, l);
         X[to] = h, X[to + lo] = l;
       }
       if (++col == sh.cols) col = 0, ++row;
@@ -625,7 +632,7 @@ __global__ __launch_bounds__(64 * SMALL_WAVES) void k_small(Matrices ms, Shape s
                 k_one = __shfl(f_one, step), k_apply = __shfl(f_apply, step);
     for (int t = wave; t < tiles; t += SMALL_WAVES) {
       const int a = triangle_row(t), b = t - a * (a + 1) / 2;
-      put_tile(S, lo_s, sm.pitch_s, a, b, k_gram * gram_tile(X, lo, sm.pitch, (16 * sm.strips + 31) & ~31, a, b, lane), lane);
+      put_tile(S, lo_s, sm.pitch_s, a, b, k_gram * gram_tile(X, lo, sm.pitch, sm.depth, a, b, lane), lane);
     }
     __syncthreads();
     f32x4 v[MINE];
@@ -634,7 +641,7 @@ __global__ __launch_bounds__(64 * SMALL_WAVES) void k_small(Matrices ms, Shape s
       const int t = wave + SMALL_WAVES * c;
       if (t >= tiles) continue;
       const int a = triangle_row(t), b = t - a * (a + 1) / 2, m = 16 * a + 4 * (lane >> 4), n = 16 * b + (lane & 15);
-      const f32x4 ss = gram_tile(S, lo_s, sm.pitch_s, (sm.r16 + 31) & ~31, a, b, lane);
+      const f32x4 ss = gram_tile(S, lo_s, sm.pitch_s, sm.depth_s, a, b, lane);
       const _Float16* self = S + n * sm.pitch_s + small_at(n, m);
       const f16x4 h = *reinterpret_cast<const f16x4*>(self), l = *reinterpret_cast<const f16x4*>(self + lo_s);
 #pragma unroll
@@ -663,16 +670,16 @@ __global__ __launch_bounds__(64 * SMALL_WAVES) void k_small(Matrices ms, Shape s
 #pragma unroll
       for (int w = 0; w < WIDE; ++w) {
         const int first = 16 * min(strip + w, sm.strips - 1) + (q & 3) * 4;
+        const int turn[2] = {small_at(g8 + (q >> 2), first), small_at(g8 + (q >> 2) + 4, first)};   // 32 rows on the same
 #pragma unroll
         for (int d = 0; d < DEEP; ++d) {
           const bool there = 32 * d + g8 < sm.r16;
-          const int row = there ? 32 * d + g8 + (q >> 2) : q >> 2;
+          const _Float16* at = X + (there ? 32 * d + g8 + (q >> 2) : q >> 2) * sm.pitch;
           f16x4 part[4];
 #pragma unroll
           for (int e = 0; e < 4; ++e)                   // hi of rows row, row + 4; lo
             part[e] = __builtin_bit_cast(f16x4, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                (__attribute__((address_space(3))) s16x4*)(X + (e >> 1) * lo + (row + 4 * (e & 1)) * sm.pitch +
-                                                          small_at(row + 4 * (e & 1), first))));
+                (__attribute__((address_space(3))) s16x4*)(at + (e >> 1) * lo + 4 * (e & 1) * sm.pitch + turn[e & 1])));
           const f16x8 h = __builtin_shufflevector(part[0], part[1], 0, 1, 2, 3, 4, 5, 6, 7);
           const f16x8 l = __builtin_shufflevector(part[2], part[3], 0, 1, 2, 3, 4, 5, 6, 7);
           ah[w][d] = there ? h : f16x8{}, al[w][d] = there ? l : f16x8{};
@@ -680,11 +687,12 @@ __global__ __launch_bounds__(64 * SMALL_WAVES) void k_small(Matrices ms, Shape s
       }
       for (int tile = 0; tile < R; ++tile) {
         const int row = 16 * tile + q;
+        const int first = small_at(q, g8);              // 16 rows on the same, 64 columns on too
         const _Float16* pb = S + row * sm.pitch_s;
         Sums s[WIDE];
 #pragma unroll
         for (int d = 0; d < DEEP; ++d) {                // behind r16 X is 0 here, and B in its padding
-          const _Float16* at = pb + (32 * d < sm.r16 ? small_at(row, 32 * d + g8) : 0);
+          const _Float16* at = pb + (32 * d < sm.r16 ? 64 * (d / 2) + (d & 1 ? first ^ 32 : first) : 0);
           const f16x8 bh = *reinterpret_cast<const f16x8*>(at), bl = *reinterpret_cast<const f16x8*>(at + lo_s);
 #pragma unroll
           for (int w = 0; w < WIDE; ++w) s[w].add(ah[w][d], al[w][d], bh, bl);
@@ -815,7 +823,7 @@ bool small(const Shape& sh, Small& sm) {
     sm.pitch = a, sm.pitch_s = b;
     return 4ll * sm.r16 * (a + b) <= SMALL_LDS;
   };
-  const int a = (int)up(sh.L, 64), b = (int)up(sh.r, 64);
+  const int a = sm.depth = (int)up(sh.L, 64), b = sm.depth_s = (int)up(sh.r, 64);
   return fits(a | 64, b | 64) || fits(a | 64, b) || fits(a, b | 64) || fits(a, b);
 }
 
