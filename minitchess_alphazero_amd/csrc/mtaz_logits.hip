@@ -1,13 +1,13 @@
 // Operators on logits [rows][cols]: the policy's answers and the learner's loss.
 //
-//   k_adjust        penalties for repeated actions, a bias, a legal-move mask
-//   k_adjust_grad   its backward pass (per row), k_bias_sum / k_bias_join for a shared bias
-//   k_loss_part, k_loss_row, k_loss_mean   the policy/value loss and its gradient
+//   k_adjust_wave, k_adjust   penalties for repeated actions, a bias, a legal-move mask
+//   k_adjust_grad             its backward pass; k_bias_join joins the gradient of a bias that rows share
+//   k_loss_wave, k_loss_block, k_loss_part + k_loss_row   the policy/value loss, with or without its gradient
+//   k_loss_grad               the gradient alone, from the rows' statistics
+//   k_loss_mean               the mean of the rows
 //
-// All are bound by memory: every element is read and written once with wide accesses, arithmetic is
-// in float.  A row is cut into tiles of TILE columns, one workgroup each, so that a single long row
-// fills the chip as well as many short ones do; what a tile needs of its row (the counts of the actions taken
-// in its columns, the softmax statistics of the other tiles) is rebuilt by its workgroup.
+// All are bound by memory or, for small calls, by latency: every element is read and written once, 16 bytes at a time
+// and before anything that does not need it, and arithmetic is in float.
 #include "ops.h"
 
 #include <math.h>
@@ -15,16 +15,16 @@
 namespace mtaz {
 namespace {
 
-constexpr int TILE = 4096;    // columns per workgroup
-constexpr int NT = 256;
-constexpr int PER = 4;        // elements per access (16 B of float, 8 B of a 16-bit type)
+// elements of 16 bytes
+template <int DT> constexpr int PER = DT == MTAZ_F32 ? 4 : 8;
 
 struct Legal {
   const uint32_t* bits;
   int64_t stride;
-  // bits of columns v .. v + 3 (v a multiple of 4)
-  __device__ __forceinline__ uint32_t four(int64_t row, int v) const {
-    return bits ? (bits[row * stride + (v >> 5)] >> (v & 31)) & 15u : 15u;
+  // bits of columns v .. v + N - 1 (v a multiple of N, N 4 or 8), 0 behind the last column (n of them are left)
+  template <int N> __device__ __forceinline__ uint32_t some(int64_t row, int v, int n) const {
+    const uint32_t all = n >= N ? (1u << N) - 1 : n > 0 ? (1u << n) - 1 : 0u;
+    return bits && n > 0 ? (bits[row * stride + (v >> 5)] >> (v & 31)) & all : all;
   }
 };
 
@@ -36,277 +36,468 @@ struct Taken {
   float repetition, frequency, presence;
   const float* per_row;
 };
-
 struct Penalty {
   float repetition, frequency, presence;
 };
-
 __device__ __forceinline__ Penalty penalty_of(const Taken& t, int64_t row) {
   if (t.per_row) return {t.per_row[3 * row], t.per_row[3 * row + 1], t.per_row[3 * row + 2]};
   return {t.repetition, t.frequency, t.presence};
 }
-
-// counts of the row's actions in columns [v0, v0 + nv) into cnt (LDS); integer adds, so their order does
-// not matter.  Entries outside [0, cols) fall outside every tile.
-__device__ __forceinline__ void count_taken(const Taken& t, int64_t row, int v0, int nv, uint32_t* cnt) {
-  for (int i = threadIdx.x; i < nv; i += NT) cnt[i] = 0;
-  __syncthreads();
+// calls f for every action that the row has taken, THREADS threads in steps of four entries.  Entries outside
+// [0, cols) lie outside every tile.
+template <int THREADS, typename F> __device__ __forceinline__ void each_taken(const Taken& t, int64_t row, int thread, F f) {
   const int len = t.lengths ? min(max(t.lengths[row], 0), t.history) : t.history;
   const int32_t* a = t.actions + row * t.stride;
-  for (int i = threadIdx.x; i < len; i += NT) {
-    const uint32_t v = (uint32_t)(a[i] - v0);
-    if (v < (uint32_t)nv) atomicAdd(&cnt[v], 1u);
+  for (int i = 4 * thread; i < len; i += 4 * THREADS) {
+    if (i + 4 <= len) {
+      const Pack<int32_t, 4> q = *reinterpret_cast<const Pack<int32_t, 4>*>(a + i);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) f(q.v[j]);
+    } else {
+      for (int j = i; j < len; ++j) f(a[j]);
+    }
   }
-  __syncthreads();
 }
 
-template <typename T> __device__ __forceinline__ Pack<T, PER> load4(const T* p, int n) {
-  Pack<T, PER> r;
-  if (n >= PER) return *reinterpret_cast<const Pack<T, PER>*>(p);
+// N elements, n of them there
+template <typename T, int N> __device__ __forceinline__ Pack<T, N> load(const T* p, int n) {
+  Pack<T, N> r;
+  if (n >= N) return *reinterpret_cast<const Pack<T, N>*>(p);
 #pragma unroll
-  for (int j = 0; j < PER; ++j) r.v[j] = j < n ? p[j] : (T)0.f;
+  for (int j = 0; j < N; ++j) r.v[j] = j < n ? p[j] : (T)0.f;
   return r;
 }
-template <typename T> __device__ __forceinline__ void store4(T* p, const Pack<T, PER>& r, int n) {
-  if (n >= PER) {
-    *reinterpret_cast<Pack<T, PER>*>(p) = r;
+template <typename T, int N> __device__ __forceinline__ void store(T* p, const Pack<T, N>& r, int n) {
+  if (n >= N) {
+    *reinterpret_cast<Pack<T, N>*>(p) = r;
     return;
   }
 #pragma unroll
-  for (int j = 0; j < PER; ++j)
+  for (int j = 0; j < N; ++j)
     if (j < n) p[j] = r.v[j];
 }
 
+// ---- penalties, bias, mask -----------------------------------------------------------------------------------
+__device__ __forceinline__ float adjusted(float x, uint32_t count, float bias, const Penalty& p) {
+  if (count) x = (x > 0.f ? x / p.repetition : x * p.repetition) - p.frequency * (float)count - p.presence;
+  return x + bias;
+}
+
+// Rows of up to WAVE_COLS columns: a wave each, with the counts of its actions in its own piece of LDS.
+constexpr int WAVE_COLS = 1024;
+template <int DT>
+__global__ __launch_bounds__(256) void k_adjust_wave(const typename Elem<DT>::T* x, int64_t x_stride,
+                                                     typename Elem<DT>::T* y, int64_t y_stride, int64_t rows, int cols,
+                                                     Legal legal, const float* bias, int64_t bias_stride, Taken taken) {
+  typedef Elem<DT> E;
+  constexpr int N = PER<DT>, REP = WAVE_COLS / (64 * N);
+  __shared__ __attribute__((aligned(16))) uint32_t counts[4][WAVE_COLS];
+  const int lane = threadIdx.x % 64, wave = threadIdx.x / 64;
+  const int64_t row = (int64_t)blockIdx.x * 4 + wave;
+  if (row >= rows) return;
+  Pack<typename E::T, N> q[REP];
+#pragma unroll
+  for (int k = 0; k < REP; ++k) {
+    const int v = N * (lane + 64 * k);
+    if (v < cols) q[k] = load<typename E::T, N>(x + row * x_stride + v, cols - v);
+  }
+  Penalty p = {1.f, 0.f, 0.f};
+  uint32_t* cnt = counts[wave];
+  const bool counted = taken.actions != nullptr;
+  if (counted) {                                        // LDS serves one wave's accesses in order
+    p = penalty_of(taken, row);
+#pragma unroll
+    for (int k = 0; k < WAVE_COLS / 256; ++k) *reinterpret_cast<uint4*>(cnt + 4 * (lane + 64 * k)) = make_uint4(0, 0, 0, 0);
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    each_taken<64>(taken, row, lane, [&](int v) {
+      if ((uint32_t)v < (uint32_t)cols) atomicAdd(&cnt[v], 1u);
+    });
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  }
+#pragma unroll
+  for (int k = 0; k < REP; ++k) {
+    const int v = N * (lane + 64 * k), n = cols - v;
+    if (n <= 0) continue;
+    const uint32_t ok = legal.some<N>(row, v, n);
+    Pack<float, N> b = {};
+    if (bias && ok) b = load<float, N>(bias + row * bias_stride + v, n);
+#pragma unroll
+    for (int j = 0; j < N; ++j)
+      q[k].v[j] = E::put((ok >> j) & 1u ? adjusted(E::get(q[k].v[j]), counted ? cnt[v + j] : 0u, b.v[j], p) : -INFINITY);
+    store(y + row * y_stride + v, q[k], n);
+  }
+}
+
+// Longer rows in tiles, so that one long row fills the chip as well as many: a workgroup per tile counts the actions
+// in its columns.  Integer adds, so their order does not matter.
+constexpr int NT = 512;
+template <int DT> constexpr int TILE = NT * PER<DT>;
 template <int DT>
 __global__ __launch_bounds__(NT) void k_adjust(const typename Elem<DT>::T* x, int64_t x_stride,
                                                typename Elem<DT>::T* y, int64_t y_stride, int cols, int tiles,
                                                Legal legal, const float* bias, int64_t bias_stride, Taken taken) {
   typedef Elem<DT> E;
-  __shared__ uint32_t cnt[TILE];
+  constexpr int N = PER<DT>;
+  __shared__ __attribute__((aligned(16))) uint32_t cnt[TILE<DT>];
   const int64_t row = blockIdx.x / tiles;
-  const int v0 = (int)(blockIdx.x % tiles) * TILE;
-  const int nv = min(TILE, cols - v0);
+  const int v0 = (int)(blockIdx.x % tiles) * TILE<DT>, i = N * threadIdx.x, v = v0 + i, n = cols - v;
   const bool counted = taken.actions != nullptr;
+  Pack<typename E::T, N> q;
+  Pack<float, N> b = {};
+  const uint32_t ok = legal.some<N>(row, v, n);
+  if (n > 0) q = load<typename E::T, N>(x + row * x_stride + v, n);
+  if (bias && ok) b = load<float, N>(bias + row * bias_stride + v, n);
   Penalty p = {1.f, 0.f, 0.f};
   if (counted) {
-    count_taken(taken, row, v0, nv, cnt);
     p = penalty_of(taken, row);
-  }
-  for (int i = PER * threadIdx.x; i < nv; i += PER * NT) {
-    const int v = v0 + i, n = nv - i;
-    const uint32_t ok = legal.four(row, v);
-    Pack<typename E::T, PER> q = load4(x + row * x_stride + v, n);
-    Pack<float, PER> b = {};
-    if (bias) b = load4(bias + row * bias_stride + v, n);
 #pragma unroll
-    for (int j = 0; j < PER; ++j) {
-      float s = E::get(q.v[j]);
-      const uint32_t c = counted && j < n ? cnt[i + j] : 0u;
-      if (c) s = (s > 0.f ? s / p.repetition : s * p.repetition) - p.frequency * (float)c - p.presence;
-      s += b.v[j];
-      q.v[j] = E::put((ok >> j) & 1u ? s : -INFINITY);
-    }
-    store4(y + row * y_stride + v, q, n);
+    for (int j = 0; j < N; j += 4) *reinterpret_cast<uint4*>(cnt + i + j) = make_uint4(0, 0, 0, 0);
+    __syncthreads();
+    each_taken<NT>(taken, row, threadIdx.x, [&](int a) {
+      const uint32_t at = (uint32_t)a - (uint32_t)v0;
+      if (at < (uint32_t)TILE<DT>) atomicAdd(&cnt[at], 1u);
+    });
+    __syncthreads();
   }
+  if (n <= 0) return;
+#pragma unroll
+  for (int j = 0; j < N; ++j)
+    q.v[j] = E::put((ok >> j) & 1u ? adjusted(E::get(q.v[j]), counted ? cnt[i + j] : 0u, b.v[j], p) : -INFINITY);
+  store(y + row * y_stride + v, q, n);
 }
 
 // d x = d y * slope, slope = 1, or 1 / repetition (x > 0) or repetition (x <= 0) of a taken action; 0 where
-// not legal.  gb: the same without the slope, per row, in float.
+// not legal.  gb: the same without the slope, per row, in float.  part: the columns' sums of that over the workgroup's
+// rows, for a bias that all rows share; a workgroup takes `per` rows one after the other.
 template <int DT>
 __global__ __launch_bounds__(NT) void k_adjust_grad(const typename Elem<DT>::T* gy, int64_t gy_stride,
                                                     const typename Elem<DT>::T* x, int64_t x_stride,
                                                     typename Elem<DT>::T* gx, int64_t gx_stride, float* gb,
-                                                    int64_t gb_stride, int cols, int tiles, Legal legal, Taken taken) {
+                                                    int64_t gb_stride, float* part, int64_t rows, int per, int cols,
+                                                    int tiles, Legal legal, Taken taken) {
   typedef Elem<DT> E;
-  __shared__ uint32_t cnt[TILE];
-  const int64_t row = blockIdx.x / tiles;
-  const int v0 = (int)(blockIdx.x % tiles) * TILE;
-  const int nv = min(TILE, cols - v0);
-  const bool counted = taken.actions != nullptr;
-  float rep = 1.f, inv = 1.f;
-  if (counted) {
-    count_taken(taken, row, v0, nv, cnt);
-    rep = penalty_of(taken, row).repetition;
-    inv = 1.f / rep;
-  }
-  for (int i = PER * threadIdx.x; i < nv; i += PER * NT) {
-    const int v = v0 + i, n = nv - i;
-    const uint32_t ok = legal.four(row, v);
-    Pack<typename E::T, PER> g = load4(gy + row * gy_stride + v, n);
-    Pack<float, PER> f;
-#pragma unroll
-    for (int j = 0; j < PER; ++j) f.v[j] = (ok >> j) & 1u ? E::get(g.v[j]) : 0.f;
-    if (gb) store4(gb + row * gb_stride + v, f, n);
-    if (!gx) continue;
-#pragma unroll
-    for (int j = 0; j < PER; ++j) {
-      if (counted && j < n && cnt[i + j] && ((ok >> j) & 1u)) f.v[j] *= E::get(x[row * x_stride + v + j]) > 0.f ? inv : rep;
-      g.v[j] = E::put(f.v[j]);
-    }
-    store4(gx + row * gx_stride + v, g, n);
-  }
-}
-
-// Shared bias: columns summed over rows in a fixed order, chunk by chunk of rows, then over the chunks.
-constexpr int BIAS_COLS = NT * PER;
-template <int DT>
-__global__ __launch_bounds__(NT) void k_bias_sum(const typename Elem<DT>::T* gy, int64_t gy_stride, int64_t rows,
-                                                 int64_t per_chunk, int cols, Legal legal, float* part) {
-  typedef Elem<DT> E;
-  const int v = blockIdx.x * BIAS_COLS + PER * threadIdx.x, n = cols - v;
-  if (n <= 0) return;
-  const int64_t r0 = blockIdx.y * per_chunk, r1 = min(rows, r0 + per_chunk);
-  Pack<float, PER> s = {};
+  constexpr int N = PER<DT>;
+  __shared__ uint32_t seen[2][TILE<DT> / 32];           // in turn, so that a row needs two barriers
+  const int64_t chunk = blockIdx.x / tiles, r0 = chunk * per, r1 = min(rows, r0 + per);
+  const int v0 = (int)(blockIdx.x % tiles) * TILE<DT>, i = N * threadIdx.x, v = v0 + i, n = cols - v;
+  const bool counted = taken.actions != nullptr && gx;
+  Pack<float, N> sum = {};
+  Pack<typename E::T, N> g, z;
+  uint32_t ok = 0;
+  auto fetch = [&](int64_t row) {
+    ok = legal.some<N>(row, v, n);
+    if (n > 0) g = load<typename E::T, N>(gy + row * gy_stride + v, n);
+    if (counted && n > 0) z = load<typename E::T, N>(x + row * x_stride + v, n);
+  };
+  fetch(r0);
   for (int64_t row = r0; row < r1; ++row) {
-    const uint32_t ok = legal.four(row, v);
-    const Pack<typename E::T, PER> g = load4(gy + row * gy_stride + v, n);
+    const Pack<typename E::T, N> dy = g, logit = z;
+    const uint32_t legal_here = ok;
+    uint32_t hit = 0;
+    float rep = 1.f, inv = 1.f;
+    if (row + 1 < r1) fetch(row + 1);                   // under way while this row's actions are looked at
+    if (counted) {
+      uint32_t* bits = seen[(row - r0) & 1];
+      if (threadIdx.x < TILE<DT> / 32) bits[threadIdx.x] = 0;
+      __syncthreads();
+      each_taken<NT>(taken, row, threadIdx.x, [&](int a) {
+        const uint32_t at = (uint32_t)a - (uint32_t)v0;
+        if (at < (uint32_t)TILE<DT>) atomicOr(&bits[at >> 5], 1u << (at & 31));
+      });
+      rep = penalty_of(taken, row).repetition;
+      inv = 1.f / rep;
+      __syncthreads();
+      hit = bits[i >> 5] >> (i & 31);
+    }
+    if (n <= 0) continue;
+    Pack<float, N> f;
 #pragma unroll
-    for (int j = 0; j < PER; ++j) s.v[j] += (ok >> j) & 1u ? E::get(g.v[j]) : 0.f;
+    for (int j = 0; j < N; ++j) {
+      f.v[j] = (legal_here >> j) & 1u ? E::get(dy.v[j]) : 0.f;
+      sum.v[j] += f.v[j];
+    }
+    if (gb) store(gb + row * gb_stride + v, f, n);
+    if (!gx) continue;
+    Pack<typename E::T, N> o;
+#pragma unroll
+    for (int j = 0; j < N; ++j)
+      o.v[j] = E::put((hit >> j) & 1u ? f.v[j] * (E::get(logit.v[j]) > 0.f ? inv : rep) : f.v[j]);
+    store(gx + row * gx_stride + v, o, n);
   }
-  store4(part + (int64_t)blockIdx.y * cols + v, s, n);
+  if (part && n > 0) store(part + chunk * cols + v, sum, n);
 }
-__global__ __launch_bounds__(NT) void k_bias_join(const float* part, int chunks, int cols, float* gb) {
-  const int v = blockIdx.x * NT + threadIdx.x;
+// the workgroups' sums, in order
+__global__ __launch_bounds__(256) void k_bias_join(const float* part, int chunks, int cols, float* gb) {
+  const int v = blockIdx.x * 256 + threadIdx.x;
   if (v >= cols) return;
   float s = 0.f;
+#pragma unroll 8
   for (int c = 0; c < chunks; ++c) s += part[(int64_t)c * cols + v];
   gb[v] = s;
 }
-int bias_chunks(int64_t rows) { return (int)(rows < 64 ? rows : 64); }
 
 // ---- policy/value loss -------------------------------------------------------------------------------------
-// Statistics of a row or a piece of it: the largest logit, sum exp(z - top), sum pi, sum pi (z - top).
+// With top the largest legal logit, total = sum exp(z - top), pi = sum of the targets, dot = sum pi (z - top):
+//   row = pi log(total) - dot,   d row / d z = exp(z - top) / total * pi - target.
+// exp by the instruction for 2^x: the product with log2(e) is off by 2^-24 of z - top, which a term e^(z - top) turns
+// into at most 0.37 * 2^-24 of the largest.
+__device__ __forceinline__ float soft_exp(float d) { return __builtin_amdgcn_exp2f(d * 1.44269504088896341f); }
+
+struct Row {
+  float loss;          // without the value term
+  float top, inv, pi;  // inv = 1 / total, 0 where nothing is legal
+};
+__device__ __forceinline__ Row row_of(float top, float total, float pi, float dot) {
+  const bool some = top != -INFINITY || total != 0.f;   // a NaN among the logits is no empty row
+  return {some ? pi * logf(total) - dot : 0.f, top, some ? 1.f / total : 0.f, pi};
+}
+// the value term, the row's statistics for k_loss_mean and k_loss_grad, the value's gradient
+__device__ __forceinline__ float finish_row(const Row& r, int64_t row, const float* value, const float* reward, float k,
+                                            float* stats, float* value_grad) {
+  float loss = r.loss;
+  if (value) {
+    const float d = value[row] - reward[row];
+    loss += d * d;
+    if (value_grad) value_grad[row] = 2.f * k * d;
+  }
+  *reinterpret_cast<float4*>(stats + 4 * row) = make_float4(r.top, r.inv, r.pi, loss);
+  return loss;
+}
+__device__ __forceinline__ float wave_sum(float x) {
+  for (int o = 32; o; o >>= 1) x += __shfl_xor(x, o);
+  return x;
+}
+__device__ __forceinline__ float wave_max(float x) {
+  for (int o = 32; o; o >>= 1) x = fmaxf(x, __shfl_xor(x, o));
+  return x;
+}
+
+// A row in registers, THREADS threads with REP times PER logits each; `both` reduces over them.
+template <int DT, int DP, int THREADS, int REP> struct Held {
+  static constexpr int N = PER<DT>;
+  Pack<typename Elem<DT>::T, N> z[REP];
+  Pack<typename Elem<DP>::T, N> w[REP];
+  uint32_t ok[REP];
+  __device__ __forceinline__ void fetch(const typename Elem<DT>::T* logits, const typename Elem<DP>::T* target, int64_t row,
+                                        int cols, const Legal& legal, int thread) {
+#pragma unroll
+    for (int k = 0; k < REP; ++k) {
+      const int v = N * (thread + THREADS * k), n = cols - v;
+      ok[k] = legal.some<N>(row, v, n);
+      if (n > 0) z[k] = load<typename Elem<DT>::T, N>(logits + v, n);
+      if (n > 0) w[k] = load<typename Elem<DP>::T, N>(target + v, n);
+    }
+  }
+  __device__ __forceinline__ float top() const {
+    float t = -INFINITY;
+#pragma unroll
+    for (int k = 0; k < REP; ++k)
+#pragma unroll
+      for (int j = 0; j < N; ++j)
+        if ((ok[k] >> j) & 1u) t = fmaxf(t, Elem<DT>::get(z[k].v[j]));
+    return t;
+  }
+  // A logit of -inf has no part in the sums, except that a target there makes the loss infinite; a target of 0 adds
+  // nothing.
+  __device__ __forceinline__ void sums(float top, float& total, float& pi, float& dot) const {
+    total = pi = dot = 0.f;
+#pragma unroll
+    for (int k = 0; k < REP; ++k)
+#pragma unroll
+      for (int j = 0; j < N; ++j)
+        if ((ok[k] >> j) & 1u) {
+          const float x = Elem<DT>::get(z[k].v[j]), t = Elem<DP>::get(w[k].v[j]);
+          const float d = x == -INFINITY ? -INFINITY : x - top;
+          total += d == -INFINITY ? 0.f : soft_exp(d);
+          pi += t;
+          if (t != 0.f) dot += t * d;
+        }
+  }
+  __device__ __forceinline__ void leave(typename Elem<DT>::T* g, int cols, const Row& r, float k, int thread) {
+#pragma unroll
+    for (int q = 0; q < REP; ++q) {
+      const int v = N * (thread + THREADS * q), n = cols - v;
+      if (n <= 0) continue;
+#pragma unroll
+      for (int j = 0; j < N; ++j)
+        z[q].v[j] = Elem<DT>::put((ok[q] >> j) & 1u ? slope(Elem<DT>::get(z[q].v[j]), Elem<DP>::get(w[q].v[j]), r, k) : 0.f);
+      store(g + v, z[q], n);
+    }
+  }
+  static __device__ __forceinline__ float slope(float x, float t, const Row& r, float k) {
+    const float e = x == -INFINITY ? 0.f : soft_exp(x - r.top) * r.inv;
+    return k * (r.inv == 0.f ? 0.f : e * r.pi - t);
+  }
+};
+
+// Rows of up to WAVE_COLS columns: a wave each.  ONE: a single workgroup takes all rows and their mean.
+template <int DT, int DP, bool ONE>
+__global__ __launch_bounds__(ONE ? 1024 : 256) void k_loss_wave(const typename Elem<DT>::T* z, int64_t z_stride,
+                                                                const typename Elem<DP>::T* pi, int64_t pi_stride,
+                                                                int64_t rows, int cols, Legal legal, const float* value,
+                                                                const float* reward, float* stats, float* loss,
+                                                                typename Elem<DT>::T* grad, int64_t grad_stride,
+                                                                float* value_grad, float k) {
+  constexpr int WAVES = ONE ? 16 : 4;
+  const int lane = threadIdx.x % 64, wave = threadIdx.x / 64;
+  double mean = 0.;
+  for (int64_t row = ONE ? wave : (int64_t)blockIdx.x * WAVES + wave; row < rows; row += ONE ? WAVES : rows) {
+    Held<DT, DP, 64, WAVE_COLS / (64 * PER<DT>)> h;
+    h.fetch(z + row * z_stride, pi + row * pi_stride, row, cols, legal, lane);
+    const float top = wave_max(h.top());
+    float total, sum, dot;
+    h.sums(top, total, sum, dot);
+    const Row r = row_of(top, wave_sum(total), wave_sum(sum), wave_sum(dot));
+    if (grad) h.leave(grad + row * grad_stride, cols, r, k, lane);
+    if (lane == 0) mean += (double)finish_row(r, row, value, reward, k, stats, value_grad);
+  }
+  if (!ONE) return;
+  __shared__ double ws[WAVES];
+  if (lane == 0) ws[wave] = mean;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    for (int w = 1; w < WAVES; ++w) mean += ws[w];
+    *loss = (float)(mean / (double)rows);
+  }
+}
+
+// Rows that fit into a workgroup's registers: one workgroup each
+template <int DT, int DP, int THREADS, int REP>
+__global__ __launch_bounds__(THREADS) void k_loss_block(const typename Elem<DT>::T* z, int64_t z_stride,
+                                                        const typename Elem<DP>::T* pi, int64_t pi_stride, int cols,
+                                                        Legal legal, const float* value, const float* reward,
+                                                        float* stats, typename Elem<DT>::T* grad, int64_t grad_stride,
+                                                        float* value_grad, float k) {
+  constexpr int WAVES = THREADS / 64;
+  __shared__ float ws[4][WAVES];
+  const int64_t row = blockIdx.x;
+  const int lane = threadIdx.x % 64, wave = threadIdx.x / 64;
+  Held<DT, DP, THREADS, REP> h;
+  h.fetch(z + row * z_stride, pi + row * pi_stride, row, cols, legal, threadIdx.x);
+  float top = wave_max(h.top());
+  if (lane == 0) ws[0][wave] = top;
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < WAVES; ++w) top = fmaxf(top, ws[0][w]);
+  float total, sum, dot;
+  h.sums(top, total, sum, dot);
+  total = wave_sum(total), sum = wave_sum(sum), dot = wave_sum(dot);
+  if (lane == 0) ws[1][wave] = total, ws[2][wave] = sum, ws[3][wave] = dot;
+  __syncthreads();
+  total = sum = dot = 0.f;
+#pragma unroll
+  for (int w = 0; w < WAVES; ++w) total += ws[1][w], sum += ws[2][w], dot += ws[3][w];
+  const Row r = row_of(top, total, sum, dot);
+  if (grad) h.leave(grad + row * grad_stride, cols, r, k, threadIdx.x);
+  if (threadIdx.x == 0) finish_row(r, row, value, reward, k, stats, value_grad);
+}
+
+// Longer rows in tiles: the statistics of a tile, then of the row from its tiles'.
 struct Soft {
   float top, total, pi, dot;
 };
-
 // The statistics of two pieces joined: each sum moves from its own top to the larger one.  A piece whose
 // top is -inf has no finite logit: its total is 0 (or NaN) and its dot 0 (no target there) or infinite already.
 __device__ __forceinline__ Soft join(const Soft& a, const Soft& b) {
   Soft r;
   r.top = fmaxf(a.top, b.top);
   const float da = a.top == -INFINITY ? 0.f : a.top - r.top, db = b.top == -INFINITY ? 0.f : b.top - r.top;
-  r.total = a.total * expf(da) + b.total * expf(db);
+  r.total = a.total * soft_exp(da) + b.total * soft_exp(db);
   r.pi = a.pi + b.pi;
   r.dot = (a.dot + da * a.pi) + (b.dot + db * b.pi);
   return r;
 }
-__device__ __forceinline__ Soft wave_join(Soft s) {
-  for (int o = 32; o; o >>= 1) {
-    const Soft t = {__shfl_xor(s.top, o), __shfl_xor(s.total, o), __shfl_xor(s.pi, o), __shfl_xor(s.dot, o)};
-    s = (threadIdx.x & o) ? join(t, s) : join(s, t);   // lower lane first on both sides: the same sums
-  }
-  return s;
-}
-
+constexpr int TILE_REP = 2;
+template <int DT> constexpr int LOSS_TILE = NT * PER<DT> * TILE_REP;
 template <int DT, int DP>
 __global__ __launch_bounds__(NT) void k_loss_part(const typename Elem<DT>::T* z, int64_t z_stride,
                                                   const typename Elem<DP>::T* pi, int64_t pi_stride, int cols,
                                                   int tiles, Legal legal, Soft* part) {
+  constexpr int WAVES = NT / 64;
+  __shared__ float ws[4][WAVES];
   const int64_t row = blockIdx.x / tiles;
-  const int v0 = (int)(blockIdx.x % tiles) * TILE;
-  const int nv = min(TILE, cols - v0);
-  constexpr int REP = TILE / (PER * NT);
-  Pack<typename Elem<DT>::T, PER> q[REP];
-  uint32_t ok[REP];
-  float top = -INFINITY;
+  const int v0 = (int)(blockIdx.x % tiles) * LOSS_TILE<DT>;
+  const int lane = threadIdx.x % 64, wave = threadIdx.x / 64;
+  Held<DT, DP, NT, TILE_REP> h;
+  const Legal here = {legal.bits ? legal.bits + v0 / 32 : nullptr, legal.stride};
+  h.fetch(z + row * z_stride + v0, pi + row * pi_stride + v0, row, cols - v0, here, threadIdx.x);
+  float top = wave_max(h.top());
+  if (lane == 0) ws[0][wave] = top;
+  __syncthreads();
 #pragma unroll
-  for (int k = 0; k < REP; ++k) {
-    const int i = PER * (threadIdx.x + NT * k), n = nv - i;
-    ok[k] = 0;
-    if (n <= 0) continue;
-    ok[k] = legal.four(row, v0 + i) & (n < PER ? (1u << n) - 1u : 15u);
-    q[k] = load4(z + row * z_stride + v0 + i, n);
-#pragma unroll
-    for (int j = 0; j < PER; ++j)
-      if ((ok[k] >> j) & 1u) top = fmaxf(top, Elem<DT>::get(q[k].v[j]));
-  }
-  Soft s = {top, 0.f, 0.f, 0.f};
-#pragma unroll
-  for (int k = 0; k < REP; ++k) {
-    const int i = PER * (threadIdx.x + NT * k), n = nv - i;
-    if (!ok[k]) continue;
-    const Pack<typename Elem<DP>::T, PER> t = load4(pi + row * pi_stride + v0 + i, n);
-#pragma unroll
-    for (int j = 0; j < PER; ++j)
-      if ((ok[k] >> j) & 1u) {
-        const float w = Elem<DP>::get(t.v[j]), x = Elem<DT>::get(q[k].v[j]);
-        const float d = x == -INFINITY ? -INFINITY : x - top;
-        s.total += d == -INFINITY ? 0.f : expf(d);
-        s.pi += w;
-        if (w != 0.f) s.dot += w * d;
-      }
-  }
-  __shared__ Soft ws[NT / 64];
-  s = wave_join(s);
-  if (threadIdx.x % 64 == 0) ws[threadIdx.x / 64] = s;
+  for (int w = 0; w < WAVES; ++w) top = fmaxf(top, ws[0][w]);
+  float total, sum, dot;
+  h.sums(top, total, sum, dot);
+  total = wave_sum(total), sum = wave_sum(sum), dot = wave_sum(dot);
+  if (lane == 0) ws[1][wave] = total, ws[2][wave] = sum, ws[3][wave] = dot;
   __syncthreads();
   if (threadIdx.x == 0) {
-    for (int w = 1; w < NT / 64; ++w) s = join(s, ws[w]);
-    part[blockIdx.x] = s;
+    total = sum = dot = 0.f;
+    for (int w = 0; w < WAVES; ++w) total += ws[1][w], sum += ws[2][w], dot += ws[3][w];
+    part[blockIdx.x] = {top, total, sum, dot};
   }
 }
 
-// The gradient of one element from the row's statistics {top, 1 / total, sum pi}
-__device__ __forceinline__ float loss_slope(float x, float w, const float* st, float k) {
-  const float e = x == -INFINITY ? 0.f : expf(x - st[0]) * st[1];
-  return k * (st[1] == 0.f ? 0.f : e * st[2] - w);
-}
-
+// One tile of the gradient from the row's statistics
 template <int DT, int DP>
-__device__ __forceinline__ void loss_grad_tile(const typename Elem<DT>::T* z, const typename Elem<DP>::T* pi,
-                                               typename Elem<DT>::T* g, int64_t row, int v0, int nv, const Legal& legal,
-                                               const float* st, float k) {
-  for (int i = PER * threadIdx.x; i < nv; i += PER * NT) {
-    const int n = nv - i;
-    const uint32_t ok = legal.four(row, v0 + i);
-    Pack<typename Elem<DT>::T, PER> q = load4(z + i, n);
-    const Pack<typename Elem<DP>::T, PER> t = load4(pi + i, n);
-#pragma unroll
-    for (int j = 0; j < PER; ++j)
-      q.v[j] = Elem<DT>::put((ok >> j) & 1u ? loss_slope(Elem<DT>::get(q.v[j]), Elem<DP>::get(t.v[j]), st, k) : 0.f);
-    store4(g + i, q, n);
-  }
+__device__ __forceinline__ void grad_tile(const typename Elem<DT>::T* z, const typename Elem<DP>::T* pi,
+                                          typename Elem<DT>::T* g, int64_t row, int v0, int cols, const Legal& legal,
+                                          const Row& r, float k) {
+  Held<DT, DP, NT, TILE_REP> h;
+  const Legal here = {legal.bits ? legal.bits + v0 / 32 : nullptr, legal.stride};
+  h.fetch(z + v0, pi + v0, row, cols - v0, here, threadIdx.x);
+  h.leave(g + v0, cols - v0, r, k, threadIdx.x);
 }
 
-// Joins the row's tiles (every workgroup of a row the same way), writes its own tile of the gradient; the
-// row's first workgroup writes its statistics and loss.
+// Joins the row's tiles, every workgroup of a row in the same order, and writes its own tile of the gradient; the row's
+// first workgroup writes its statistics.
 template <int DT, int DP>
 __global__ __launch_bounds__(NT) void k_loss_row(const typename Elem<DT>::T* z, int64_t z_stride,
                                                  const typename Elem<DP>::T* pi, int64_t pi_stride, int cols,
                                                  int tiles, Legal legal, const Soft* part, const float* value,
                                                  const float* reward, float* stats, typename Elem<DT>::T* grad,
                                                  int64_t grad_stride, float* value_grad, float k) {
-  const int64_t row = blockIdx.x / tiles;
-  const int tile = (int)(blockIdx.x % tiles), v0 = tile * TILE;
-  __shared__ float st[4];
+  const int per_row = grad ? tiles : 1;                 // workgroups
+  const int64_t row = blockIdx.x / per_row;
+  const int tile = (int)(blockIdx.x % per_row);
+  __shared__ Row joined;
   if (threadIdx.x < 64) {
     Soft s = {-INFINITY, 0.f, 0.f, 0.f};
     for (int t = threadIdx.x; t < tiles; t += 64) s = join(s, part[row * tiles + t]);
-    s = wave_join(s);
+    for (int o = 32; o; o >>= 1) {
+      const Soft t = {__shfl_xor(s.top, o), __shfl_xor(s.total, o), __shfl_xor(s.pi, o), __shfl_xor(s.dot, o)};
+      s = (threadIdx.x & o) ? join(t, s) : join(s, t);   // the lower lane first on both sides: the same sums
+    }
     if (threadIdx.x == 0) {
-      const bool some = s.top != -INFINITY || s.total != 0.f;   // a NaN among the logits is no empty row
-      float loss = some ? s.pi * logf(s.total) - s.dot : 0.f;
-      st[0] = s.top;
-      st[1] = some ? 1.f / s.total : 0.f;
-      st[2] = s.pi;
-      if (tile == 0) {
-        if (value) {
-          const float d = value[row] - reward[row];
-          loss += d * d;
-          if (value_grad) value_grad[row] = 2.f * k * d;
-        }
-        float* o = stats + 4 * row;
-        o[0] = st[0], o[1] = st[1], o[2] = st[2], o[3] = loss;
-      }
+      joined = row_of(s.top, s.total, s.pi, s.dot);
+      if (tile == 0) finish_row(joined, row, value, reward, k, stats, value_grad);
     }
   }
   if (!grad) return;
   __syncthreads();
-  loss_grad_tile<DT, DP>(z + row * z_stride + v0, pi + row * pi_stride + v0, grad + row * grad_stride + v0, row, v0,
-                         min(TILE, cols - v0), legal, st, k);
+  grad_tile<DT, DP>(z + row * z_stride, pi + row * pi_stride, grad + row * grad_stride, row, tile * LOSS_TILE<DT>, cols, legal,
+                    joined, k);
 }
 
+// The gradient from the statistics: rows of up to WAVE_COLS a wave each, longer ones in tiles
+template <int DT, int DP>
+__global__ __launch_bounds__(256) void k_loss_grad_wave(const typename Elem<DT>::T* z, int64_t z_stride,
+                                                        const typename Elem<DP>::T* pi, int64_t pi_stride, int64_t rows,
+                                                        int cols, Legal legal, const float* value, const float* reward,
+                                                        const float* stats, const float* grad_out,
+                                                        typename Elem<DT>::T* grad, int64_t grad_stride,
+                                                        float* value_grad) {
+  const int lane = threadIdx.x % 64;
+  const int64_t row = (int64_t)blockIdx.x * 4 + threadIdx.x / 64;
+  if (row >= rows) return;
+  const float k = *grad_out / (float)rows;
+  if (value_grad && lane == 0) value_grad[row] = 2.f * k * (value[row] - reward[row]);
+  if (!grad) return;
+  const float4 st = *reinterpret_cast<const float4*>(stats + 4 * row);
+  Held<DT, DP, 64, WAVE_COLS / (64 * PER<DT>)> h;
+  h.fetch(z + row * z_stride, pi + row * pi_stride, row, cols, legal, lane);
+  h.leave(grad + row * grad_stride, cols, Row{0.f, st.x, st.y, st.z}, k, lane);
+}
 template <int DT, int DP>
 __global__ __launch_bounds__(NT) void k_loss_grad(const typename Elem<DT>::T* z, int64_t z_stride,
                                                   const typename Elem<DP>::T* pi, int64_t pi_stride, int64_t rows,
@@ -314,18 +505,19 @@ __global__ __launch_bounds__(NT) void k_loss_grad(const typename Elem<DT>::T* z,
                                                   const float* reward, const float* stats, const float* grad_out,
                                                   typename Elem<DT>::T* grad, int64_t grad_stride, float* value_grad) {
   const int64_t row = blockIdx.x / tiles;
-  const int tile = (int)(blockIdx.x % tiles), v0 = tile * TILE;
+  const int tile = (int)(blockIdx.x % tiles);
   const float k = *grad_out / (float)rows;
   if (value_grad && tile == 0 && threadIdx.x == 0) value_grad[row] = 2.f * k * (value[row] - reward[row]);
   if (!grad) return;
-  const float st[3] = {stats[4 * row], stats[4 * row + 1], stats[4 * row + 2]};
-  loss_grad_tile<DT, DP>(z + row * z_stride + v0, pi + row * pi_stride + v0, grad + row * grad_stride + v0, row, v0,
-                         min(TILE, cols - v0), legal, st, k);
+  const float4 st = *reinterpret_cast<const float4*>(stats + 4 * row);
+  grad_tile<DT, DP>(z + row * z_stride, pi + row * pi_stride, grad + row * grad_stride, row, tile * LOSS_TILE<DT>, cols, legal,
+                    Row{0.f, st.x, st.y, st.z}, k);
 }
 
 // The mean of the rows' losses by one workgroup, in a fixed order and in 64 bits
 __global__ __launch_bounds__(1024) void k_loss_mean(const float* stats, int64_t rows, float* loss) {
   double s = 0.;
+#pragma unroll 4
   for (int64_t r = threadIdx.x; r < rows; r += 1024) s += (double)stats[4 * r + 3];
   __shared__ double ws[16];
   for (int o = 32; o; o >>= 1) s += __shfl_xor(s, o);
@@ -340,10 +532,11 @@ __global__ __launch_bounds__(1024) void k_loss_mean(const float* stats, int64_t 
 // ---- host ----------------------------------------------------------------------------------------------------
 constexpr int64_t MOST_COLS = 1 << 24;
 
+int64_t tiles_of(int64_t cols, int tile) { return (cols + tile - 1) / tile; }
 const char* bad_shape(int64_t rows, int64_t cols, int dtype) {
   if (rows < 0) return "rows must not be negative";
   if (cols < 1 || cols > MOST_COLS) return "cols must be in [1, 2^24]";
-  if (rows * ((cols + TILE - 1) / TILE) > INT32_MAX || rows > INT32_MAX) return "too many rows for one call";
+  if (rows > INT32_MAX || rows * tiles_of(cols, 512 * 4) > INT32_MAX) return "too many rows for one call";
   if (dtype < MTAZ_F32 || dtype > MTAZ_BF16) return "unknown element type";
   return nullptr;
 }
@@ -365,11 +558,26 @@ Taken taken_of(const int32_t* actions, int64_t stride, int history, const int32_
   if (!per_row) t.repetition = (float)penalties[0], t.frequency = (float)penalties[1], t.presence = (float)penalties[2];
   return t;
 }
+// Longest row that stays in the registers of one workgroup
+constexpr int BLOCK_COLS = 32768;
+int64_t loss_workspace(int64_t rows, int64_t cols) {
+  return cols <= BLOCK_COLS ? 256 : (int64_t)sizeof(Soft) * rows * tiles_of(cols, LOSS_TILE<MTAZ_F32>);
+}
 int launched(const char* what) {
   const hipError_t e = hipGetLastError();
   return e == hipSuccess ? 0 : ops_error(MTAZ_E_DEVICE, what, hipGetErrorString(e));
 }
-int tiles_of(int64_t cols) { return (int)((cols + TILE - 1) / TILE); }
+// Rows a workgroup of k_adjust_grad takes one after the other, and how many workgroups a column then has: one row,
+// unless a bias that the rows share is summed over them; then so few workgroups that they are all on the CUs at once.
+int64_t rows_each(int64_t rows, int64_t cols, bool shared) {
+  if (!shared) return 1;
+  const int64_t across = tiles_of(cols, 512 * 8), chunks = across >= 1024 ? 1 : 1024 / across;
+  return rows <= chunks ? 1 : (rows + chunks - 1) / chunks;
+}
+int64_t bias_chunks(int64_t rows, int64_t cols) {
+  const int64_t each = rows_each(rows, cols, true);
+  return (rows + each - 1) / each;
+}
 
 }  // namespace
 }  // namespace mtaz
@@ -400,17 +608,28 @@ extern "C" int mtaz_adjust_logits(int device, int64_t rows, int64_t cols, int dt
   if (rows == 0) return 0;
   DeviceScope on(device);
   if (on.status != hipSuccess) return ops_error(MTAZ_E_DEVICE, "adjust_logits", hipGetErrorString(on.status));
-  const int tiles = tiles_of(cols);
   const Taken t = taken_of(d_actions, actions_stride, history, d_lengths, penalties, d_penalties);
-  FOR_TYPE(dtype, (k_adjust<DT><<<(unsigned)(rows * tiles), NT, 0, (hipStream_t)stream>>>(
-                      (const Elem<DT>::T*)d_logits, logits_stride, (Elem<DT>::T*)d_out, out_stride, (int)cols, tiles,
-                      Legal{d_legal, legal_stride}, d_bias, bias_stride, t)));
+  const Legal legal{d_legal, legal_stride};
+  const hipStream_t s = (hipStream_t)stream;
+  const int nc = (int)cols;
+  FOR_TYPE(dtype, {
+    const auto* x = (const Elem<DT>::T*)d_logits;
+    auto* y = (Elem<DT>::T*)d_out;
+    if (cols <= WAVE_COLS) {
+      k_adjust_wave<DT><<<(unsigned)((rows + 3) / 4), 256, 0, s>>>(x, logits_stride, y, out_stride, rows, nc, legal, d_bias,
+                                                                 bias_stride, t);
+    } else {
+      const int tiles = (int)tiles_of(cols, TILE<DT>);
+      k_adjust<DT><<<(unsigned)(rows * tiles), NT, 0, s>>>(x, logits_stride, y, out_stride, nc, tiles, legal, d_bias,
+                                                          bias_stride, t);
+    }
+  });
   return launched("adjust_logits");
 }
 
 extern "C" int64_t mtaz_adjust_logits_grad_workspace(int64_t rows, int64_t cols) {
   if (const char* bad = bad_shape(rows, cols, MTAZ_F32)) return ops_error(MTAZ_E_FAIL, "adjust_logits_grad", bad);
-  return 4 * cols * bias_chunks(rows);
+  return 4 * cols * bias_chunks(rows, cols);
 }
 
 extern "C" int mtaz_adjust_logits_grad(int device, int64_t rows, int64_t cols, int dtype, const void* d_grad_out,
@@ -429,33 +648,29 @@ extern "C" int mtaz_adjust_logits_grad(int device, int64_t rows, int64_t cols, i
   if (!bad && rows && t.actions && d_grad && !d_logits) bad = "the penalties' gradient needs the logits";
   if (!bad && rows > 1 && ((d_grad && grad_stride < cols) || (d_bias_grad && !shared && bias_grad_stride < cols)))
     bad = "rows of an output overlap";
-  if (!bad && shared && rows && (!d_work || work_bytes < 4 * cols * bias_chunks(rows))) bad = "workspace too small";
+  if (!bad && shared && rows && (!d_work || work_bytes < 4 * cols * bias_chunks(rows, cols))) bad = "workspace too small";
   if (bad) return ops_error(MTAZ_E_FAIL, what, bad);
   DeviceScope on(device);
   if (on.status != hipSuccess) return ops_error(MTAZ_E_DEVICE, what, hipGetErrorString(on.status));
   const hipStream_t s = (hipStream_t)stream;
-  const int tiles = tiles_of(cols), nc = (int)cols;
-  const Legal legal{d_legal, legal_stride};
-  float* row_bias = shared ? nullptr : d_bias_grad;
-  const int chunks = bias_chunks(rows);
-  const int64_t per_chunk = chunks ? (rows + chunks - 1) / chunks : 0;
-  FOR_TYPE(dtype, {
-    if (rows && (d_grad || row_bias))
-      k_adjust_grad<DT><<<(unsigned)(rows * tiles), NT, 0, s>>>((const Elem<DT>::T*)d_grad_out, grad_out_stride,
-                                                              (const Elem<DT>::T*)d_logits, logits_stride,
-                                                              (Elem<DT>::T*)d_grad, grad_stride, row_bias,
-                                                              bias_grad_stride, nc, tiles, legal, t);
-    if (shared && rows)
-      k_bias_sum<DT><<<dim3((nc + BIAS_COLS - 1) / BIAS_COLS, chunks), NT, 0, s>>>(
-          (const Elem<DT>::T*)d_grad_out, grad_out_stride, rows, per_chunk, nc, legal, (float*)d_work);
-  });
-  if (shared) k_bias_join<<<(nc + NT - 1) / NT, NT, 0, s>>>((const float*)d_work, chunks, nc, d_bias_grad);
+  const int nc = (int)cols;
+  const int64_t each = rows_each(rows, cols, shared), chunks = rows ? (rows + each - 1) / each : 0;
+  if (rows && (d_grad || d_bias_grad)) {
+    FOR_TYPE(dtype, {
+      const int tiles = (int)tiles_of(cols, TILE<DT>);
+      k_adjust_grad<DT><<<(unsigned)(chunks * tiles), NT, 0, s>>>(
+          (const Elem<DT>::T*)d_grad_out, grad_out_stride, (const Elem<DT>::T*)d_logits, logits_stride,
+          (Elem<DT>::T*)d_grad, grad_stride, shared ? nullptr : d_bias_grad, bias_grad_stride,
+          shared ? (float*)d_work : nullptr, rows, (int)each, nc, tiles, Legal{d_legal, legal_stride}, t);
+    });
+  }
+  if (shared) k_bias_join<<<(nc + 255) / 256, 256, 0, s>>>((const float*)d_work, (int)chunks, nc, d_bias_grad);
   return launched(what);
 }
 
 extern "C" int64_t mtaz_policy_loss_workspace(int64_t rows, int64_t cols) {
   if (const char* bad = bad_shape(rows, cols, MTAZ_F32)) return ops_error(MTAZ_E_FAIL, "policy_loss", bad);
-  return (int64_t)sizeof(Soft) * rows * tiles_of(cols);
+  return loss_workspace(rows, cols);
 }
 
 static const char* bad_loss(int64_t rows, int64_t cols, int dtype, int target_dtype, const void* logits,
@@ -465,6 +680,7 @@ static const char* bad_loss(int64_t rows, int64_t cols, int dtype, int target_dt
   if (rows < 1) return "the mean of no rows";
   if (target_dtype != MTAZ_F32 && target_dtype != dtype) return "targets are float32 or of the logits' type";
   if (!logits || !target || !stats) return "no logits, targets or statistics";
+  if ((uintptr_t)stats & 15) return "statistics must be aligned to 16 bytes";
   if (!value != !reward) return "a value without a reward, or a reward without a value";
   if (value_grad && !value) return "the gradient of a value that is not there";
   if (grad && grad_stride < cols && rows > 1) return "rows of the gradient overlap";
@@ -481,25 +697,46 @@ extern "C" int mtaz_policy_loss(int device, int64_t rows, int64_t cols, int dtyp
   const char* bad = bad_loss(rows, cols, dtype, target_dtype, d_logits, d_target, d_value, d_reward, d_stats, d_grad,
                              grad_stride, d_value_grad);
   if (!bad && !d_loss) bad = "no place for the loss";
-  if (!bad && (!d_work || work_bytes < (int64_t)sizeof(Soft) * rows * tiles_of(cols))) bad = "workspace too small";
+  if (!bad && (!d_work || work_bytes < loss_workspace(rows, cols))) bad = "workspace too small";
   if (bad) return ops_error(MTAZ_E_FAIL, what, bad);
   DeviceScope on(device);
   if (on.status != hipSuccess) return ops_error(MTAZ_E_DEVICE, what, hipGetErrorString(on.status));
   const hipStream_t s = (hipStream_t)stream;
-  const int tiles = tiles_of(cols), nc = (int)cols;
-  const unsigned grid = (unsigned)(rows * tiles);
+  const int nc = (int)cols;
   const Legal legal{d_legal, legal_stride};
   const float k = (float)(scale / (double)rows);
+  // A handful of short rows: one launch, mean included.
+  const bool one = cols <= WAVE_COLS && rows <= 64;
   FOR_TYPES(dtype, target_dtype, {
     const auto* z = (const Elem<DT>::T*)d_logits;
     const auto* pi = (const Elem<DP>::T*)d_target;
-    k_loss_part<DT, DP><<<grid, NT, 0, s>>>(z, logits_stride, pi, target_stride, nc, tiles, legal, (Soft*)d_work);
-    // without a gradient one workgroup per row joins its tiles
-    k_loss_row<DT, DP><<<grid, NT, 0, s>>>(z, logits_stride, pi, target_stride, nc, tiles, legal, (const Soft*)d_work,
-                                          d_value, d_reward, d_stats, (Elem<DT>::T*)d_grad, grad_stride, d_value_grad,
-                                          k);
+    auto* g = (Elem<DT>::T*)d_grad;
+    const unsigned n = (unsigned)rows;
+    constexpr int N = PER<DT>;
+    if (one) {
+      k_loss_wave<DT, DP, true><<<1, 1024, 0, s>>>(z, logits_stride, pi, target_stride, rows, nc, legal, d_value, d_reward,
+                                                  d_stats, d_loss, g, grad_stride, d_value_grad, k);
+    } else if (cols <= WAVE_COLS) {
+      k_loss_wave<DT, DP, false><<<(n + 3) / 4, 256, 0, s>>>(z, logits_stride, pi, target_stride, rows, nc, legal, d_value,
+                                                           d_reward, d_stats, d_loss, g, grad_stride, d_value_grad, k);
+    } else if (cols <= 4096) {
+      k_loss_block<DT, DP, 256, 16 / N><<<n, 256, 0, s>>>(z, logits_stride, pi, target_stride, nc, legal, d_value, d_reward,
+                                                         d_stats, g, grad_stride, d_value_grad, k);
+    } else if (cols <= 16384) {
+      k_loss_block<DT, DP, 1024, 16 / N><<<n, 1024, 0, s>>>(z, logits_stride, pi, target_stride, nc, legal, d_value, d_reward,
+                                                           d_stats, g, grad_stride, d_value_grad, k);
+    } else if (cols <= BLOCK_COLS) {
+      k_loss_block<DT, DP, 1024, 32 / N><<<n, 1024, 0, s>>>(z, logits_stride, pi, target_stride, nc, legal, d_value, d_reward,
+                                                           d_stats, g, grad_stride, d_value_grad, k);
+    } else {
+      const int tiles = (int)tiles_of(cols, LOSS_TILE<DT>);
+      k_loss_part<DT, DP><<<n * tiles, NT, 0, s>>>(z, logits_stride, pi, target_stride, nc, tiles, legal, (Soft*)d_work);
+      k_loss_row<DT, DP><<<g ? n * tiles : n, NT, 0, s>>>(z, logits_stride, pi, target_stride, nc, tiles, legal,
+                                                        (const Soft*)d_work, d_value, d_reward, d_stats, g, grad_stride,
+                                                        d_value_grad, k);
+    }
   });
-  k_loss_mean<<<1, 1024, 0, s>>>(d_stats, rows, d_loss);
+  if (!one) k_loss_mean<<<1, 1024, 0, s>>>(d_stats, rows, d_loss);
   return launched(what);
 }
 
@@ -517,11 +754,23 @@ extern "C" int mtaz_policy_loss_grad(int device, int64_t rows, int64_t cols, int
   if (!d_grad && !d_value_grad) return 0;
   DeviceScope on(device);
   if (on.status != hipSuccess) return ops_error(MTAZ_E_DEVICE, what, hipGetErrorString(on.status));
-  const int tiles = tiles_of(cols), nc = (int)cols;
-  FOR_TYPES(dtype, target_dtype,
-            (k_loss_grad<DT, DP><<<(unsigned)(rows * tiles), NT, 0, (hipStream_t)stream>>>(
-                (const Elem<DT>::T*)d_logits, logits_stride, (const Elem<DP>::T*)d_target, target_stride, rows, nc,
-                tiles, Legal{d_legal, legal_stride}, d_value, d_reward, d_stats, d_grad_out, (Elem<DT>::T*)d_grad,
-                grad_stride, d_value_grad)));
+  const int nc = (int)cols;
+  const Legal legal{d_legal, legal_stride};
+  const hipStream_t s = (hipStream_t)stream;
+  FOR_TYPES(dtype, target_dtype, {
+    const auto* z = (const Elem<DT>::T*)d_logits;
+    const auto* pi = (const Elem<DP>::T*)d_target;
+    auto* g = (Elem<DT>::T*)d_grad;
+    if (cols <= WAVE_COLS) {
+      k_loss_grad_wave<DT, DP><<<(unsigned)((rows + 3) / 4), 256, 0, s>>>(z, logits_stride, pi, target_stride, rows, nc, legal,
+                                                                        d_value, d_reward, d_stats, d_grad_out, g,
+                                                                        grad_stride, d_value_grad);
+    } else {
+      const int tiles = (int)tiles_of(cols, LOSS_TILE<DT>);
+      k_loss_grad<DT, DP><<<(unsigned)(rows * tiles), NT, 0, s>>>(z, logits_stride, pi, target_stride, rows, nc, tiles, legal,
+                                                                d_value, d_reward, d_stats, d_grad_out, g, grad_stride,
+                                                                d_value_grad);
+    }
+  });
   return launched(what);
 }

@@ -10,14 +10,12 @@ A mask is packed 32 actions a word: action v is legal where bit v & 31 of word v
 float16 or bfloat16, sums are float32, and the operators enqueue on the current stream without a
 synchronization; they may be captured in a HIP graph.  There is no CPU form: tensors elsewhere are refused.
 """
-import ctypes
-
 import torch
 from torch.autograd.function import once_differentiable
 
 from . import _lib
 from .environment import MOVE_CAP, RULES_FLAGS
-from .optim import TYPES, _check_type, _stream
+from .optim import TYPES, _check_type, _doubles, _stream
 
 
 def _ptr(t):
@@ -39,8 +37,12 @@ def _check_rows(t, what, like, shapes, dtypes):
         raise ValueError(f'{what} must be on {like.device}, not on {t.device}')
     if t.dtype not in dtypes:
         raise ValueError(f'{what} must be {" or ".join(str(d) for d in dtypes)}, not {t.dtype}')
-    if tuple(t.shape) not in shapes:
+    if t.shape not in shapes:
         raise ValueError(f'{what} has shape {tuple(t.shape)}, expected {" or ".join(str(s) for s in shapes)}')
+
+
+def _fresh(like):
+    return torch.empty_like(like) if like.is_contiguous() else torch.empty(like.shape, dtype=like.dtype, device=like.device)
 
 
 def _check_logits(logits):
@@ -52,7 +54,7 @@ def _check_logits(logits):
 def _check_legal(legal, logits):
     if legal is not None:
         rows, words = logits.shape[0], (logits.shape[1] + 31) // 32
-        _check_rows(legal, 'legal', logits, {(rows, words), (1, words), (words,)}, (torch.int32, torch.uint32))
+        _check_rows(legal, 'legal', logits, ((rows, words), (1, words), (words,)), (torch.int32, torch.uint32))
 
 
 def legal_masks(positions, device, rules_flags=RULES_FLAGS, move_cap=MOVE_CAP):
@@ -79,83 +81,86 @@ def legal_masks(positions, device, rules_flags=RULES_FLAGS, move_cap=MOVE_CAP):
 
 # ---- penalties, bias and mask ----------------------------------------------------------------------------
 class _Taken:
-    """The actions taken and their penalties, as the C entries take them."""
+    """The actions taken and their penalties, as the C entries take them (args); keep: the tensors behind them."""
+    __slots__ = ('args', 'keep', 'bends')
 
     def __init__(self, logits, actions, lengths, repetition, frequency, presence):
         rows = logits.shape[0]
         given = (repetition, frequency, presence)
-        self.actions = self.lengths = self.per_row = None
-        self.history = 0
-        if lengths is not None and actions is None:
-            raise ValueError('lengths without actions')
-        tensors = [t for t in given if torch.is_tensor(t)]
+        per_row = None
+        tensors = [t for t in given if isinstance(t, torch.Tensor)]
         for t in tensors:
-            _check_rows(t, 'a penalty', logits, {(rows,)}, (torch.float32,))
+            _check_rows(t, 'a penalty', logits, ((rows,),), (torch.float32,))
             if t.requires_grad and torch.is_grad_enabled():
                 raise ValueError('penalties have no gradient')
-        if not torch.is_tensor(repetition) and not repetition > 0:
-            raise ValueError(f'repetition must be positive, got {repetition}')
-        self.host = (ctypes.c_double * 3)(*[1.0 if torch.is_tensor(t) else float(t) for t in given])
-        self.bends = torch.is_tensor(repetition) or repetition != 1.0   # the slope is not 1 everywhere
+        if tensors:
+            host = None
+            if not isinstance(repetition, torch.Tensor) and not repetition > 0:
+                raise ValueError(f'repetition must be positive, got {repetition}')
+        else:
+            host = _doubles(float(repetition), float(frequency), float(presence))
+            if not repetition > 0:
+                raise ValueError(f'repetition must be positive, got {repetition}')
+        self.bends = (isinstance(repetition, torch.Tensor) or repetition != 1.0)   # slope not 1
         if actions is None:
+            if lengths is not None:
+                raise ValueError('lengths without actions')
+            self.args, self.keep, self.bends = (None, 0, 0, None, host, None), (None, None, None), False
             return
         if actions.dim() != 2:
             raise ValueError(f'actions must be [rows, history], got {tuple(actions.shape)}')
-        _check_rows(actions, 'actions', logits, {(rows, actions.shape[1])}, (torch.int32,))
+        _check_rows(actions, 'actions', logits, ((rows, actions.shape[1]),), (torch.int32,))
         if lengths is not None:
-            _check_rows(lengths, 'lengths', logits, {(rows,)}, (torch.int32,))
-            self.lengths = lengths.contiguous()
-        self.actions, self.history = _unit(actions), actions.shape[1]
+            _check_rows(lengths, 'lengths', logits, ((rows,),), (torch.int32,))
+            lengths = lengths.contiguous()
+        actions = _unit(actions)
         if tensors:
-            self.per_row = torch.stack([t if torch.is_tensor(t) else torch.full((rows,), float(t), device=logits.device)
-                                        for t in given], 1).contiguous()
-
-    def args(self):
-        return (_ptr(self.actions), 0 if self.actions is None else self.actions.stride(0), self.history,
-                _ptr(self.lengths), self.host, _ptr(self.per_row))
+            per_row = torch.stack([t if isinstance(t, torch.Tensor) else torch.full((rows,), float(t), device=logits.device)
+                                   for t in given], 1)
+        self.keep = (actions, lengths, per_row)
+        self.args = (actions.data_ptr(), actions.stride(0), actions.shape[1], _ptr(lengths), host, _ptr(per_row))
 
 
-def _adjust(logits, legal, bias, taken, out):
-    x = _unit(logits)
+def _adjust(x, legal, bias, taken, out):
+    x, legal, bias = _unit(x), _unit(legal), _unit(bias)
     rows, cols = x.shape
-    legal, bias = _unit(legal), _unit(bias)
     _lib.check(_lib.lib().mtaz_adjust_logits(
         x.device.index, rows, cols, TYPES[x.dtype], x.data_ptr(), x.stride(0), out.data_ptr(), out.stride(0),
-        _ptr(legal), _row_stride(legal), _ptr(bias), _row_stride(bias), *taken.args(), _stream(x.device)))
+        _ptr(legal), _row_stride(legal), _ptr(bias), _row_stride(bias), *taken.args, _stream(x.device)))
     return out
 
 
 class _Adjust(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, bias, legal, taken):
-        ctx.taken, ctx.shape, ctx.dtype = taken, logits.shape, logits.dtype
+        ctx.taken, ctx.dtype = taken, logits.dtype
         ctx.bias_shape = None if bias is None else bias.shape
-        keep = logits if taken.bends and taken.actions is not None else None
-        ctx.save_for_backward(keep, legal, taken.actions, taken.lengths)
-        return _adjust(logits, legal, bias, taken, torch.empty(logits.shape, dtype=logits.dtype, device=logits.device))
+        actions, lengths, _ = taken.keep
+        ctx.save_for_backward(logits if taken.bends else None, legal, actions, lengths)
+        return _adjust(logits, legal, bias, taken, _fresh(logits))
 
     @staticmethod
     @once_differentiable
     def backward(ctx, grad):
-        x, legal, _, _ = ctx.saved_tensors   # raises where actions or lengths were changed in between
+        x, legal, _, _ = ctx.saved_tensors   # raises where one of them was changed in between
         g, x, legal = _unit(grad), _unit(x), _unit(legal)
-        rows, cols = ctx.shape
+        rows, cols = g.shape
         dx = db = work = None
+        size = 0
         shared = False
         if ctx.needs_input_grad[0]:
-            dx = torch.empty(ctx.shape, dtype=ctx.dtype, device=g.device)
+            dx = _fresh(g)
         if ctx.needs_input_grad[1]:
             db = torch.empty(ctx.bias_shape, dtype=torch.float32, device=g.device)
             shared = len(ctx.bias_shape) == 1 or ctx.bias_shape[0] == 1
             if shared:
                 size = _lib.check(_lib.lib().mtaz_adjust_logits_grad_workspace(rows, cols))
                 work = torch.empty(max(size, 1), dtype=torch.uint8, device=g.device)
-        t = ctx.taken
-        taken = t.args() if x is not None else (None, 0, 0, None, t.host, None)   # the slope is 1 everywhere
+        taken = ctx.taken.args if x is not None else (None, 0, 0, None, None, None)   # else the slope is 1 everywhere
         _lib.check(_lib.lib().mtaz_adjust_logits_grad(
             g.device.index, rows, cols, TYPES[ctx.dtype], g.data_ptr(), g.stride(0), _ptr(x),
             0 if x is None else x.stride(0), _ptr(dx), cols, _ptr(db), 0 if shared else cols, _ptr(legal),
-            _row_stride(legal), *taken, _ptr(work), 0 if work is None else work.numel(), _stream(g.device)))
+            _row_stride(legal), *taken, _ptr(work), size, _stream(g.device)))
         return dx, db, None, None
 
 
@@ -175,22 +180,21 @@ def adjust_logits(logits, legal=None, bias=None, actions=None, lengths=None, rep
     rows, cols = logits.shape
     _check_legal(legal, logits)
     if bias is not None:
-        _check_rows(bias, 'bias', logits, {(cols,), (1, cols), (rows, cols)}, (torch.float32,))
+        _check_rows(bias, 'bias', logits, ((cols,), (1, cols), (rows, cols)), (torch.float32,))
     taken = _Taken(logits, actions, lengths, repetition, frequency, presence)
     if torch.is_grad_enabled() and (logits.requires_grad or (bias is not None and bias.requires_grad)):
         if out is not None:
             raise ValueError('out is not supported where a gradient is required')
         return _Adjust.apply(logits, bias, legal, taken)
     if out is None:
-        out = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
-    else:
-        if out.shape != logits.shape or out.dtype != logits.dtype or out.device != logits.device:
-            raise ValueError('out must have the shape, type and device of logits')
-        if (cols > 1 and out.stride(1) != 1) or (rows > 1 and out.stride(0) < cols):
-            raise ValueError('out must have dense rows that do not overlap')
-        if torch.is_grad_enabled() and out.requires_grad:
-            raise ValueError('out must not require a gradient')
-    _adjust(logits.detach(), legal, bias, taken, out)
+        return _adjust(logits, legal, bias, taken, _fresh(logits))
+    if out.shape != logits.shape or out.dtype != logits.dtype or out.device != logits.device:
+        raise ValueError('out must have the shape, type and device of logits')
+    if (cols > 1 and out.stride(1) != 1) or (rows > 1 and out.stride(0) < cols):
+        raise ValueError('out must have dense rows that do not overlap')
+    if torch.is_grad_enabled() and out.requires_grad:
+        raise ValueError('out must not require a gradient')
+    _adjust(logits, legal, bias, taken, out)
     torch.autograd.graph.increment_version(out)
     return out
 
@@ -201,29 +205,34 @@ def _check_loss(logits, target, value, reward, legal):
     rows, cols = logits.shape
     if rows == 0:
         raise ValueError('the mean loss of no rows')
-    _check_rows(target, 'target', logits, {(rows, cols)}, (torch.float32, logits.dtype))
+    _check_rows(target, 'target', logits, ((rows, cols),), (torch.float32, logits.dtype))
     if (value is None) != (reward is None):
         raise ValueError('value and reward come together')
-    for t, what in ((value, 'value'), (reward, 'reward')):
-        if t is not None:
-            _check_rows(t, what, logits, {(rows,), (rows, 1)}, (torch.float32,))
+    if value is not None:
+        shapes = ((rows,), (rows, 1))
+        _check_rows(value, 'value', logits, shapes, (torch.float32,))
+        _check_rows(reward, 'reward', logits, shapes, (torch.float32,))
     _check_legal(legal, logits)
     if torch.is_grad_enabled() and (target.requires_grad or (reward is not None and reward.requires_grad)):
         raise ValueError('target and reward have no gradient')
 
 
 def _loss(logits, target, value, reward, legal, grad, value_grad, scale):
+    """(loss, the rows' statistics with the call's scratch memory behind them)"""
     z, t, legal = _unit(logits), _unit(target), _unit(legal)
     rows, cols = z.shape
     dev = z.device
-    value, reward = (None if x is None else x.reshape(-1).contiguous() for x in (value, reward))
+    if value is not None:
+        value, reward = value.contiguous(), reward.contiguous()
+    entries = _lib.lib()
+    work = _lib.check(entries.mtaz_policy_loss_workspace(rows, cols))
     loss = torch.empty((), dtype=torch.float32, device=dev)
-    stats = torch.empty((rows, 4), dtype=torch.float32, device=dev)
-    work = torch.empty(_lib.check(_lib.lib().mtaz_policy_loss_workspace(rows, cols)), dtype=torch.uint8, device=dev)
-    _lib.check(_lib.lib().mtaz_policy_loss(
+    stats = torch.empty(4 * rows + work // 4, dtype=torch.float32, device=dev)
+    at = stats.data_ptr()
+    _lib.check(entries.mtaz_policy_loss(
         dev.index, rows, cols, TYPES[z.dtype], TYPES[t.dtype], z.data_ptr(), z.stride(0), t.data_ptr(), t.stride(0),
-        _ptr(legal), _row_stride(legal), _ptr(value), _ptr(reward), loss.data_ptr(), stats.data_ptr(), _ptr(grad), cols,
-        _ptr(value_grad), float(scale), work.data_ptr(), work.numel(), _stream(dev)))
+        _ptr(legal), _row_stride(legal), _ptr(value), _ptr(reward), loss.data_ptr(), at, _ptr(grad), cols,
+        _ptr(value_grad), scale, at + 16 * rows, work, _stream(dev)))
     return loss, stats
 
 
@@ -240,12 +249,15 @@ class _PolicyValueLoss(torch.autograd.Function):
         logits, value, target, reward, legal, stats = ctx.saved_tensors
         z, t, legal = _unit(logits), _unit(target), _unit(legal)
         rows, cols = z.shape
-        flat, reward = (None if x is None else x.reshape(-1).contiguous() for x in (value, reward))
-        dz = torch.empty(z.shape, dtype=z.dtype, device=z.device) if ctx.needs_input_grad[0] else None
-        dv = torch.empty(value.shape, device=z.device) if value is not None and ctx.needs_input_grad[1] else None
+        dz = _fresh(z) if ctx.needs_input_grad[0] else None
+        dv = None
+        if value is not None:
+            value, reward = value.contiguous(), reward.contiguous()
+            if ctx.needs_input_grad[1]:
+                dv = torch.empty_like(value)
         _lib.check(_lib.lib().mtaz_policy_loss_grad(
             z.device.index, rows, cols, TYPES[z.dtype], TYPES[t.dtype], z.data_ptr(), z.stride(0), t.data_ptr(),
-            t.stride(0), _ptr(legal), _row_stride(legal), _ptr(flat), _ptr(reward), stats.data_ptr(), grad.data_ptr(),
+            t.stride(0), _ptr(legal), _row_stride(legal), _ptr(value), _ptr(reward), stats.data_ptr(), grad.data_ptr(),
             _ptr(dz), cols, _ptr(dv), _stream(z.device)))
         return dz, dv, None, None, None
 
@@ -264,13 +276,13 @@ def policy_value_loss(logits, target, value=None, reward=None, legal=None):
     return _loss(logits, target, value, reward, legal, None, None, 1.0)[0]
 
 
-@torch.no_grad()
 def policy_value_loss_grad(logits, target, value=None, reward=None, legal=None, scale=1.0):
     """policy_value_loss and the gradients of scale * loss, from one pass: (loss, d logits, d value or None),
-    for torch.autograd.backward((logits, value), (d logits, d value)).  With 16-bit logits a scale keeps
-    small gradients in range."""
+    for torch.autograd.backward((logits, value), (d logits, d value)); the three are cut off from autograd's graph.
+    With 16-bit logits a scale keeps small gradients in range."""
     _check_loss(logits, target, value, reward, legal)
-    dz = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
+    logits = logits.detach()
+    dz = _fresh(logits)
     dv = None if value is None else torch.empty(value.shape, dtype=torch.float32, device=logits.device)
-    loss, _ = _loss(logits, target, value, reward, legal, dz, dv, scale)
+    loss, _ = _loss(logits, target, None if value is None else value.detach(), reward, legal, dz, dv, float(scale))
     return loss, dz, dv

@@ -12,6 +12,7 @@ Every function enqueues on the current stream of its tensors' device, synchroniz
 captured in a HIP graph.  There is no CPU form: tensors elsewhere are refused.
 """
 import ctypes
+import functools
 import math
 
 import torch
@@ -23,11 +24,16 @@ COEFFICIENTS = (3.4445, -4.7750, 2.0315)
 TYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
 
 
+@functools.lru_cache(maxsize=64)
+def _doubles(*values):
+    return (ctypes.c_double * len(values))(*values)
+
+
 def _coefficients(values):
     values = tuple(float(v) for v in values)
     if len(values) != 3:
         raise ValueError(f'expected three coefficients, got {len(values)}')
-    return (ctypes.c_double * 3)(*values)
+    return _doubles(*values)
 
 
 def _pointers(tensors):
@@ -47,7 +53,8 @@ def _check_type(t, what):
 
 
 def _stream(device):
-    return ctypes.c_void_p(torch.cuda.current_stream(device).cuda_stream)
+    """The current stream of a device, as the C entries take it."""
+    return torch._C._cuda_getCurrentRawStream(device.index)
 
 
 def orthogonalize(grad, steps=5, coefficients=COEFFICIENTS, eps=1e-7, out=None):
