@@ -43,19 +43,23 @@ __device__ __forceinline__ Penalty penalty_of(const Taken& t, int64_t row) {
   if (t.per_row) return {t.per_row[3 * row], t.per_row[3 * row + 1], t.per_row[3 * row + 2]};
   return {t.repetition, t.frequency, t.presence};
 }
-// calls f for every action that the row has taken, THREADS threads in steps of four entries.  Entries outside
-// [0, cols) lie outside every tile.
+// calls f for every action that the row has taken, THREADS threads in steps of four entries; the first entries are
+// asked for before the length is there.  Entries outside [0, cols) lie outside every tile.
 template <int THREADS, typename F> __device__ __forceinline__ void each_taken(const Taken& t, int64_t row, int thread, F f) {
-  const int len = t.lengths ? min(max(t.lengths[row], 0), t.history) : t.history;
   const int32_t* a = t.actions + row * t.stride;
-  for (int i = 4 * thread; i < len; i += 4 * THREADS) {
-    if (i + 4 <= len) {
-      const Pack<int32_t, 4> q = *reinterpret_cast<const Pack<int32_t, 4>*>(a + i);
-#pragma unroll
-      for (int j = 0; j < 4; ++j) f(q.v[j]);
+  const int len = t.lengths ? min(max(t.lengths[row], 0), t.history) : t.history;
+  for (int i = 4 * thread; i < t.history; i += 4 * THREADS) {
+    Pack<int32_t, 4> q;
+    if (i + 4 <= t.history) {
+      q = *reinterpret_cast<const Pack<int32_t, 4>*>(a + i);
     } else {
-      for (int j = i; j < len; ++j) f(a[j]);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) q.v[j] = i + j < t.history ? a[i + j] : -1;
     }
+    if (i >= len) break;
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (i + j < len) f(q.v[j]);
   }
 }
 
@@ -129,102 +133,107 @@ __global__ __launch_bounds__(256) void k_adjust_wave(const typename Elem<DT>::T*
 }
 
 // Longer rows in tiles, so that one long row fills the chip as well as many: a workgroup per tile counts the actions
-// in its columns.  Integer adds, so their order does not matter.
+// in its columns.  Integer adds, so their order does not matter.  REP: accesses a thread; the more, the fewer
+// workgroups look through a row's actions.
 constexpr int NT = 512;
-template <int DT> constexpr int TILE = NT * PER<DT>;
-template <int DT>
+template <int DT, int REP>
 __global__ __launch_bounds__(NT) void k_adjust(const typename Elem<DT>::T* x, int64_t x_stride,
                                                typename Elem<DT>::T* y, int64_t y_stride, int cols, int tiles,
                                                Legal legal, const float* bias, int64_t bias_stride, Taken taken) {
   typedef Elem<DT> E;
-  constexpr int N = PER<DT>;
-  __shared__ __attribute__((aligned(16))) uint32_t cnt[TILE<DT>];
+  constexpr int N = PER<DT>, TILE = NT * N * REP;
+  __shared__ __attribute__((aligned(16))) uint32_t cnt[TILE];
   const int64_t row = blockIdx.x / tiles;
-  const int v0 = (int)(blockIdx.x % tiles) * TILE<DT>, i = N * threadIdx.x, v = v0 + i, n = cols - v;
+  const int v0 = (int)(blockIdx.x % tiles) * TILE;
   const bool counted = taken.actions != nullptr;
-  Pack<typename E::T, N> q;
-  Pack<float, N> b = {};
-  const uint32_t ok = legal.some<N>(row, v, n);
-  if (n > 0) q = load<typename E::T, N>(x + row * x_stride + v, n);
-  if (bias && ok) b = load<float, N>(bias + row * bias_stride + v, n);
+  Pack<typename E::T, N> q[REP];
+  Pack<float, N> b[REP] = {};
+  uint32_t ok[REP];
+#pragma unroll
+  for (int k = 0; k < REP; ++k) {
+    const int v = v0 + N * (threadIdx.x + NT * k), n = cols - v;
+    ok[k] = legal.some<N>(row, v, n);
+    if (n > 0) q[k] = load<typename E::T, N>(x + row * x_stride + v, n);
+    if (bias && ok[k]) b[k] = load<float, N>(bias + row * bias_stride + v, n);
+  }
   Penalty p = {1.f, 0.f, 0.f};
   if (counted) {
     p = penalty_of(taken, row);
 #pragma unroll
-    for (int j = 0; j < N; j += 4) *reinterpret_cast<uint4*>(cnt + i + j) = make_uint4(0, 0, 0, 0);
+    for (int k = 0; k < TILE / (4 * NT); ++k) *reinterpret_cast<uint4*>(cnt + 4 * (threadIdx.x + NT * k)) = make_uint4(0, 0, 0, 0);
     __syncthreads();
     each_taken<NT>(taken, row, threadIdx.x, [&](int a) {
       const uint32_t at = (uint32_t)a - (uint32_t)v0;
-      if (at < (uint32_t)TILE<DT>) atomicAdd(&cnt[at], 1u);
+      if (at < (uint32_t)TILE) atomicAdd(&cnt[at], 1u);
     });
     __syncthreads();
   }
-  if (n <= 0) return;
 #pragma unroll
-  for (int j = 0; j < N; ++j)
-    q.v[j] = E::put((ok >> j) & 1u ? adjusted(E::get(q.v[j]), counted ? cnt[i + j] : 0u, b.v[j], p) : -INFINITY);
-  store(y + row * y_stride + v, q, n);
+  for (int k = 0; k < REP; ++k) {
+    const int i = N * (threadIdx.x + NT * k), n = cols - v0 - i;
+    if (n <= 0) continue;
+#pragma unroll
+    for (int j = 0; j < N; ++j)
+      q[k].v[j] = E::put((ok[k] >> j) & 1u ? adjusted(E::get(q[k].v[j]), counted ? cnt[i + j] : 0u, b[k].v[j], p) : -INFINITY);
+    store(y + row * y_stride + v0 + i, q[k], n);
+  }
 }
 
-// d x = d y * slope, slope = 1, or 1 / repetition (x > 0) or repetition (x <= 0) of a taken action; 0 where
-// not legal.  gb: the same without the slope, per row, in float.  part: the columns' sums of that over the workgroup's
-// rows, for a bias that all rows share; a workgroup takes `per` rows one after the other.
+// d x = d y where legal, else 0; gb: the same in float, per row; part: its sums over the columns of the workgroup's rows,
+// for a bias that all rows share.  A workgroup takes `per` rows one after the other.
 template <int DT>
 __global__ __launch_bounds__(NT) void k_adjust_grad(const typename Elem<DT>::T* gy, int64_t gy_stride,
-                                                    const typename Elem<DT>::T* x, int64_t x_stride,
                                                     typename Elem<DT>::T* gx, int64_t gx_stride, float* gb,
                                                     int64_t gb_stride, float* part, int64_t rows, int per, int cols,
-                                                    int tiles, Legal legal, Taken taken) {
+                                                    int tiles, Legal legal) {
   typedef Elem<DT> E;
   constexpr int N = PER<DT>;
-  __shared__ uint32_t seen[2][TILE<DT> / 32];           // in turn, so that a row needs two barriers
   const int64_t chunk = blockIdx.x / tiles, r0 = chunk * per, r1 = min(rows, r0 + per);
-  const int v0 = (int)(blockIdx.x % tiles) * TILE<DT>, i = N * threadIdx.x, v = v0 + i, n = cols - v;
-  const bool counted = taken.actions != nullptr && gx;
+  const int v = ((int)(blockIdx.x % tiles) * NT + threadIdx.x) * N, n = cols - v;
+  if (n <= 0) return;
   Pack<float, N> sum = {};
-  Pack<typename E::T, N> g, z;
-  uint32_t ok = 0;
-  auto fetch = [&](int64_t row) {
-    ok = legal.some<N>(row, v, n);
-    if (n > 0) g = load<typename E::T, N>(gy + row * gy_stride + v, n);
-    if (counted && n > 0) z = load<typename E::T, N>(x + row * x_stride + v, n);
-  };
-  fetch(r0);
-  for (int64_t row = r0; row < r1; ++row) {
-    const Pack<typename E::T, N> dy = g, logit = z;
-    const uint32_t legal_here = ok;
-    uint32_t hit = 0;
-    float rep = 1.f, inv = 1.f;
-    if (row + 1 < r1) fetch(row + 1);                   // under way while this row's actions are looked at
-    if (counted) {
-      uint32_t* bits = seen[(row - r0) & 1];
-      if (threadIdx.x < TILE<DT> / 32) bits[threadIdx.x] = 0;
-      __syncthreads();
-      each_taken<NT>(taken, row, threadIdx.x, [&](int a) {
-        const uint32_t at = (uint32_t)a - (uint32_t)v0;
-        if (at < (uint32_t)TILE<DT>) atomicOr(&bits[at >> 5], 1u << (at & 31));
-      });
-      rep = penalty_of(taken, row).repetition;
-      inv = 1.f / rep;
-      __syncthreads();
-      hit = bits[i >> 5] >> (i & 31);
-    }
-    if (n <= 0) continue;
+  auto take = [&](int64_t row, const Pack<typename E::T, N>& g) {
+    const uint32_t ok = legal.some<N>(row, v, n);
+    Pack<typename E::T, N> o;
     Pack<float, N> f;
 #pragma unroll
     for (int j = 0; j < N; ++j) {
-      f.v[j] = (legal_here >> j) & 1u ? E::get(dy.v[j]) : 0.f;
+      f.v[j] = (ok >> j) & 1u ? E::get(g.v[j]) : 0.f;
       sum.v[j] += f.v[j];
+      o.v[j] = E::put(f.v[j]);
     }
     if (gb) store(gb + row * gb_stride + v, f, n);
-    if (!gx) continue;
-    Pack<typename E::T, N> o;
+    if (gx) store(gx + row * gx_stride + v, o, n);
+  };
+  int64_t row = r0;
+  if (n >= N)                                           // four rows' loads under way at once
+    for (; row + 4 <= r1; row += 4) {
+      Pack<typename E::T, N> g[4];
 #pragma unroll
-    for (int j = 0; j < N; ++j)
-      o.v[j] = E::put((hit >> j) & 1u ? f.v[j] * (E::get(logit.v[j]) > 0.f ? inv : rep) : f.v[j]);
-    store(gx + row * gx_stride + v, o, n);
-  }
-  if (part && n > 0) store(part + chunk * cols + v, sum, n);
+      for (int k = 0; k < 4; ++k) g[k] = *reinterpret_cast<const Pack<typename E::T, N>*>(gy + (row + k) * gy_stride + v);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) take(row + k, g[k]);
+    }
+  for (; row < r1; ++row) take(row, load<typename E::T, N>(gy + row * gy_stride + v, n));
+  if (part) store(part + chunk * cols + v, sum, n);
+}
+// Afterwards the few places of taken actions: d x = d y * slope, the slope 1 / repetition (x > 0) or repetition.  A
+// thread per entry of the list; an action that is in it twice is written twice alike.
+template <int DT>
+__global__ __launch_bounds__(256) void k_taken_grad(const typename Elem<DT>::T* gy, int64_t gy_stride,
+                                                    const typename Elem<DT>::T* x, int64_t x_stride,
+                                                    typename Elem<DT>::T* gx, int64_t gx_stride, int64_t rows, int cols,
+                                                    int groups, Legal legal, Taken taken) {
+  typedef Elem<DT> E;
+  const int64_t id = (int64_t)blockIdx.x * 4 + threadIdx.x / 64, row = id / groups;
+  const int i = (int)(id % groups) * 64 + threadIdx.x % 64;
+  if (row >= rows || i >= taken.history) return;
+  const int v = taken.actions[row * taken.stride + i];
+  if (taken.lengths && i >= taken.lengths[row]) return;
+  if ((uint32_t)v >= (uint32_t)cols || !legal.some<1>(row, v, 1)) return;
+  const float rep = penalty_of(taken, row).repetition;
+  const float g = E::get(gy[row * gy_stride + v]);
+  gx[row * gx_stride + v] = E::put(E::get(x[row * x_stride + v]) > 0.f ? g * (1.f / rep) : g * rep);
 }
 // the workgroups' sums, in order
 __global__ __launch_bounds__(256) void k_bias_join(const float* part, int chunks, int cols, float* gb) {
@@ -251,6 +260,8 @@ __device__ __forceinline__ Row row_of(float top, float total, float pi, float do
   const bool some = top != -INFINITY || total != 0.f;   // a NaN among the logits is no empty row
   return {some ? pi * logf(total) - dot : 0.f, top, some ? 1.f / total : 0.f, pi};
 }
+// what exp is taken relative to: nothing in a row without a finite logit
+__device__ __forceinline__ float base_of(float top) { return top == -INFINITY ? 0.f : top; }
 // the value term, the row's statistics for k_loss_mean and k_loss_grad, the value's gradient
 __device__ __forceinline__ float finish_row(const Row& r, int64_t row, const float* value, const float* reward, float k,
                                             float* stats, float* value_grad) {
@@ -272,61 +283,123 @@ __device__ __forceinline__ float wave_max(float x) {
   return x;
 }
 
-// A row in registers, THREADS threads with REP times PER logits each; `both` reduces over them.
-template <int DT, int DP, int THREADS, int REP> struct Held {
+// N elements packed in 32-bit words: 16-bit values of their own would take a register each.
+template <int DT, int N> struct Words {
+  typedef typename Elem<DT>::T T;
+  static constexpr int W = N * (int)sizeof(T) / 4;
+  uint32_t w[W];
+  __device__ __forceinline__ void fetch(const T* p, int n) {   // n of them there, the others 0
+    if (n >= N) {
+      const Pack<T, N> q = *reinterpret_cast<const Pack<T, N>*>(p);
+      __builtin_memcpy(w, &q, sizeof(q));
+    } else {
+#pragma unroll
+      for (int i = 0; i < W; ++i) w[i] = 0;
+#pragma unroll
+      for (int j = 0; j < N; ++j)
+        if (j < n) put(j, p[j]);
+    }
+  }
+  __device__ __forceinline__ float get(int j) const {
+    if constexpr (DT == MTAZ_F32) return __builtin_bit_cast(float, w[j]);
+    if constexpr (DT == MTAZ_BF16) return __builtin_bit_cast(float, j & 1 ? w[j / 2] & 0xffff0000u : w[j / 2] << 16);
+    if constexpr (DT == MTAZ_F16) return (float)__builtin_bit_cast(_Float16, (uint16_t)(w[j / 2] >> (16 * (j & 1))));
+  }
+  __device__ __forceinline__ void put(int j, T x) {
+    if constexpr (DT == MTAZ_F32) w[j] = __builtin_bit_cast(uint32_t, x);
+    else {
+      const uint32_t half = __builtin_bit_cast(uint16_t, x);
+      w[j / 2] = j & 1 ? (w[j / 2] & 0xffffu) | half << 16 : (w[j / 2] & 0xffff0000u) | half;
+    }
+  }
+  __device__ __forceinline__ void leave(T* p, int n) const {
+    Pack<T, N> q;
+    __builtin_memcpy(&q, w, sizeof(q));
+    store(p, q, n);
+  }
+  // The compiler forgets how the words came about: else it keeps every value as a float from one phase to the next.
+  __device__ __forceinline__ void forget() {
+#pragma unroll
+    for (int i = 0; i < W; ++i) asm volatile("" : "+v"(w[i]));
+  }
+};
+
+// A row in registers, THREADS threads with REP times PER logits each.  What is not legal, or not there, is held as a
+// logit of -inf with a target of 0, which adds nothing anywhere.  KEEP: the exponentials stay in registers from the sums
+// to the gradient; else they are taken twice.
+template <int DT, int DP, int THREADS, int REP, bool KEEP = true> struct Held {
   static constexpr int N = PER<DT>;
-  Pack<typename Elem<DT>::T, N> z[REP];
-  Pack<typename Elem<DP>::T, N> w[REP];
+  typedef typename Elem<DT>::T Z;
+  typedef typename Elem<DP>::T W;
+  Words<DT, N> z[REP];
+  Words<DP, N> w[REP];
+  float e[KEEP ? REP : 1][N];   // exp(z - top), after sums()
   uint32_t ok[REP];
-  __device__ __forceinline__ void fetch(const typename Elem<DT>::T* logits, const typename Elem<DP>::T* target, int64_t row,
-                                        int cols, const Legal& legal, int thread) {
+  __device__ __forceinline__ void fetch(const Z* logits, const W* target, int64_t row, int cols, const Legal& legal,
+                                        int thread) {
 #pragma unroll
     for (int k = 0; k < REP; ++k) {
-      const int v = N * (thread + THREADS * k), n = cols - v;
+      const uint32_t v = N * (thread + THREADS * k);
+      const int n = cols - (int)v;
       ok[k] = legal.some<N>(row, v, n);
-      if (n > 0) z[k] = load<typename Elem<DT>::T, N>(logits + v, n);
-      if (n > 0) w[k] = load<typename Elem<DP>::T, N>(target + v, n);
+      if (n > 0) z[k].fetch(logits + v, n), w[k].fetch(target + v, n);
     }
+  }
+  __device__ __forceinline__ void clear() {
+#pragma unroll
+    for (int k = 0; k < REP; ++k)
+      if (ok[k] != (1u << N) - 1)
+#pragma unroll
+        for (int j = 0; j < N; ++j)
+          if (!((ok[k] >> j) & 1u)) z[k].put(j, Elem<DT>::put(-INFINITY)), w[k].put(j, Elem<DP>::put(0.f));
   }
   __device__ __forceinline__ float top() const {
     float t = -INFINITY;
 #pragma unroll
-    for (int k = 0; k < REP; ++k)
+    for (int k = 0; k < REP; ++k) {
 #pragma unroll
-      for (int j = 0; j < N; ++j)
-        if ((ok[k] >> j) & 1u) t = fmaxf(t, Elem<DT>::get(z[k].v[j]));
+      for (int j = 0; j < N; ++j) t = fmaxf(t, z[k].get(j));
+    }
     return t;
   }
-  // A logit of -inf has no part in the sums, except that a target there makes the loss infinite; a target of 0 adds
-  // nothing.
-  __device__ __forceinline__ void sums(float top, float& total, float& pi, float& dot) const {
+  __device__ __forceinline__ void forget() {
+#pragma unroll
+    for (int k = 0; k < REP; ++k) z[k].forget(), w[k].forget();
+  }
+  // A logit of -inf makes the loss infinite if it has a target, and a target of 0 adds nothing.
+  __device__ __forceinline__ void sums(float base, float& total, float& pi, float& dot) {
+    if (!KEEP) forget();
     total = pi = dot = 0.f;
 #pragma unroll
-    for (int k = 0; k < REP; ++k)
+    for (int k = 0; k < REP; ++k) {
 #pragma unroll
-      for (int j = 0; j < N; ++j)
-        if ((ok[k] >> j) & 1u) {
-          const float x = Elem<DT>::get(z[k].v[j]), t = Elem<DP>::get(w[k].v[j]);
-          const float d = x == -INFINITY ? -INFINITY : x - top;
-          total += d == -INFINITY ? 0.f : soft_exp(d);
-          pi += t;
-          if (t != 0.f) dot += t * d;
-        }
+      for (int j = 0; j < N; ++j) {
+        const float d = z[k].get(j) - base, t = w[k].get(j);
+        const float x = soft_exp(d);
+        if (KEEP) e[k][j] = x;
+        total += x;
+        pi += t;
+        dot += t != 0.f ? t * d : 0.f;
+      }
+    }
   }
-  __device__ __forceinline__ void leave(typename Elem<DT>::T* g, int cols, const Row& r, float k, int thread) {
+  __device__ __forceinline__ void leave(Z* g, int cols, const Row& r, float k, int thread) {
+    if (!KEEP) forget();
+    const float soft = k * r.inv * r.pi, kt = r.inv == 0.f ? 0.f : k, base = base_of(r.top);
 #pragma unroll
     for (int q = 0; q < REP; ++q) {
       const int v = N * (thread + THREADS * q), n = cols - v;
       if (n <= 0) continue;
+      Words<DT, N> o;
 #pragma unroll
-      for (int j = 0; j < N; ++j)
-        z[q].v[j] = Elem<DT>::put((ok[q] >> j) & 1u ? slope(Elem<DT>::get(z[q].v[j]), Elem<DP>::get(w[q].v[j]), r, k) : 0.f);
-      store(g + v, z[q], n);
+      for (int j = 0; j < N; ++j) o.put(j, Elem<DT>::put(fmaf(KEEP ? e[q][j] : soft_exp(z[q].get(j) - base), soft,
+                                      -kt * w[q].get(j))));
+      if (ok[q] != (1u << N) - 1)                       // 0 there in a row of NaN too
+#pragma unroll
+        for (int j = 0; j < N; ++j)
+          if (!((ok[q] >> j) & 1u)) o.put(j, Elem<DT>::put(0.f));
+      o.leave(g + v, n);
     }
-  }
-  static __device__ __forceinline__ float slope(float x, float t, const Row& r, float k) {
-    const float e = x == -INFINITY ? 0.f : soft_exp(x - r.top) * r.inv;
-    return k * (r.inv == 0.f ? 0.f : e * r.pi - t);
   }
 };
 
@@ -344,9 +417,10 @@ __global__ __launch_bounds__(ONE ? 1024 : 256) void k_loss_wave(const typename E
   for (int64_t row = ONE ? wave : (int64_t)blockIdx.x * WAVES + wave; row < rows; row += ONE ? WAVES : rows) {
     Held<DT, DP, 64, WAVE_COLS / (64 * PER<DT>)> h;
     h.fetch(z + row * z_stride, pi + row * pi_stride, row, cols, legal, lane);
+    h.clear();
     const float top = wave_max(h.top());
     float total, sum, dot;
-    h.sums(top, total, sum, dot);
+    h.sums(base_of(top), total, sum, dot);
     const Row r = row_of(top, wave_sum(total), wave_sum(sum), wave_sum(dot));
     if (grad) h.leave(grad + row * grad_stride, cols, r, k, lane);
     if (lane == 0) mean += (double)finish_row(r, row, value, reward, k, stats, value_grad);
@@ -361,26 +435,29 @@ __global__ __launch_bounds__(ONE ? 1024 : 256) void k_loss_wave(const typename E
   }
 }
 
-// Rows that fit into a workgroup's registers: one workgroup each
+// Rows that fit into a workgroup's registers: one workgroup each.  With 32 logits a thread and more the exponentials are
+// taken twice; 64 of 16 bits and their targets still leave room for two workgroups of 512 on a CU, so that one loads
+// while the other computes.
 template <int DT, int DP, int THREADS, int REP>
-__global__ __launch_bounds__(THREADS) void k_loss_block(const typename Elem<DT>::T* z, int64_t z_stride,
-                                                        const typename Elem<DP>::T* pi, int64_t pi_stride, int cols,
-                                                        Legal legal, const float* value, const float* reward,
-                                                        float* stats, typename Elem<DT>::T* grad, int64_t grad_stride,
-                                                        float* value_grad, float k) {
+__global__ __launch_bounds__(THREADS, 4) void k_loss_block(const typename Elem<DT>::T* z, int64_t z_stride,
+                                                           const typename Elem<DP>::T* pi, int64_t pi_stride, int cols,
+                                                           Legal legal, const float* value, const float* reward,
+                                                           float* stats, typename Elem<DT>::T* grad, int64_t grad_stride,
+                                                           float* value_grad, float k) {
   constexpr int WAVES = THREADS / 64;
   __shared__ float ws[4][WAVES];
   const int64_t row = blockIdx.x;
   const int lane = threadIdx.x % 64, wave = threadIdx.x / 64;
-  Held<DT, DP, THREADS, REP> h;
+  Held<DT, DP, THREADS, REP, (REP * PER<DT> < 32)> h;
   h.fetch(z + row * z_stride, pi + row * pi_stride, row, cols, legal, threadIdx.x);
+  h.clear();
   float top = wave_max(h.top());
   if (lane == 0) ws[0][wave] = top;
   __syncthreads();
 #pragma unroll
   for (int w = 0; w < WAVES; ++w) top = fmaxf(top, ws[0][w]);
   float total, sum, dot;
-  h.sums(top, total, sum, dot);
+  h.sums(base_of(top), total, sum, dot);
   total = wave_sum(total), sum = wave_sum(sum), dot = wave_sum(dot);
   if (lane == 0) ws[1][wave] = total, ws[2][wave] = sum, ws[3][wave] = dot;
   __syncthreads();
@@ -421,13 +498,14 @@ __global__ __launch_bounds__(NT) void k_loss_part(const typename Elem<DT>::T* z,
   Held<DT, DP, NT, TILE_REP> h;
   const Legal here = {legal.bits ? legal.bits + v0 / 32 : nullptr, legal.stride};
   h.fetch(z + row * z_stride + v0, pi + row * pi_stride + v0, row, cols - v0, here, threadIdx.x);
+  h.clear();
   float top = wave_max(h.top());
   if (lane == 0) ws[0][wave] = top;
   __syncthreads();
 #pragma unroll
   for (int w = 0; w < WAVES; ++w) top = fmaxf(top, ws[0][w]);
   float total, sum, dot;
-  h.sums(top, total, sum, dot);
+  h.sums(base_of(top), total, sum, dot);
   total = wave_sum(total), sum = wave_sum(sum), dot = wave_sum(dot);
   if (lane == 0) ws[1][wave] = total, ws[2][wave] = sum, ws[3][wave] = dot;
   __syncthreads();
@@ -443,9 +521,10 @@ template <int DT, int DP>
 __device__ __forceinline__ void grad_tile(const typename Elem<DT>::T* z, const typename Elem<DP>::T* pi,
                                           typename Elem<DT>::T* g, int64_t row, int v0, int cols, const Legal& legal,
                                           const Row& r, float k) {
-  Held<DT, DP, NT, TILE_REP> h;
+  Held<DT, DP, NT, TILE_REP, false> h;
   const Legal here = {legal.bits ? legal.bits + v0 / 32 : nullptr, legal.stride};
   h.fetch(z + v0, pi + v0, row, cols - v0, here, threadIdx.x);
+  h.clear();
   h.leave(g + v0, cols - v0, r, k, threadIdx.x);
 }
 
@@ -494,8 +573,9 @@ __global__ __launch_bounds__(256) void k_loss_grad_wave(const typename Elem<DT>:
   if (value_grad && lane == 0) value_grad[row] = 2.f * k * (value[row] - reward[row]);
   if (!grad) return;
   const float4 st = *reinterpret_cast<const float4*>(stats + 4 * row);
-  Held<DT, DP, 64, WAVE_COLS / (64 * PER<DT>)> h;
+  Held<DT, DP, 64, WAVE_COLS / (64 * PER<DT>), false> h;
   h.fetch(z + row * z_stride, pi + row * pi_stride, row, cols, legal, lane);
+    h.clear();
   h.leave(grad + row * grad_stride, cols, Row{0.f, st.x, st.y, st.z}, k, lane);
 }
 template <int DT, int DP>
@@ -619,9 +699,15 @@ extern "C" int mtaz_adjust_logits(int device, int64_t rows, int64_t cols, int dt
       k_adjust_wave<DT><<<(unsigned)((rows + 3) / 4), 256, 0, s>>>(x, logits_stride, y, out_stride, rows, nc, legal, d_bias,
                                                                  bias_stride, t);
     } else {
-      const int tiles = (int)tiles_of(cols, TILE<DT>);
-      k_adjust<DT><<<(unsigned)(rows * tiles), NT, 0, s>>>(x, logits_stride, y, out_stride, nc, tiles, legal, d_bias,
-                                                          bias_stride, t);
+      // two accesses a thread where the chip is full twice over either way (1024 x 50021 f16: 75 us with one, see there)
+      constexpr int TILE = NT * PER<DT>;
+      const int two = (int)tiles_of(cols, 2 * TILE), one = (int)tiles_of(cols, TILE);
+      if (rows * two >= 2048)
+        k_adjust<DT, 2><<<(unsigned)(rows * two), NT, 0, s>>>(x, logits_stride, y, out_stride, nc, two, legal, d_bias,
+                                                             bias_stride, t);
+      else
+        k_adjust<DT, 1><<<(unsigned)(rows * one), NT, 0, s>>>(x, logits_stride, y, out_stride, nc, one, legal, d_bias,
+                                                             bias_stride, t);
     }
   });
   return launched("adjust_logits");
@@ -646,22 +732,32 @@ extern "C" int mtaz_adjust_logits_grad(int device, int64_t rows, int64_t cols, i
   const bool shared = d_bias_grad && bias_grad_stride == 0;
   if (!bad && rows && !d_grad_out) bad = "no incoming gradient";
   if (!bad && rows && t.actions && d_grad && !d_logits) bad = "the penalties' gradient needs the logits";
+  if (!bad && rows * ((history + 63) / 64) > INT32_MAX) bad = "too many rows for one call";
   if (!bad && rows > 1 && ((d_grad && grad_stride < cols) || (d_bias_grad && !shared && bias_grad_stride < cols)))
     bad = "rows of an output overlap";
   if (!bad && shared && rows && (!d_work || work_bytes < 4 * cols * bias_chunks(rows, cols))) bad = "workspace too small";
+  if (!bad && rows && t.actions && d_grad == d_grad_out) bad = "the penalties' gradient is not taken in place";
   if (bad) return ops_error(MTAZ_E_FAIL, what, bad);
   DeviceScope on(device);
   if (on.status != hipSuccess) return ops_error(MTAZ_E_DEVICE, what, hipGetErrorString(on.status));
   const hipStream_t s = (hipStream_t)stream;
   const int nc = (int)cols;
+  const Legal legal{d_legal, legal_stride};
+  const int64_t groups = (t.history + 63) / 64;         // of 64 entries
   const int64_t each = rows_each(rows, cols, shared), chunks = rows ? (rows + each - 1) / each : 0;
   if (rows && (d_grad || d_bias_grad)) {
     FOR_TYPE(dtype, {
-      const int tiles = (int)tiles_of(cols, TILE<DT>);
-      k_adjust_grad<DT><<<(unsigned)(chunks * tiles), NT, 0, s>>>(
-          (const Elem<DT>::T*)d_grad_out, grad_out_stride, (const Elem<DT>::T*)d_logits, logits_stride,
-          (Elem<DT>::T*)d_grad, grad_stride, shared ? nullptr : d_bias_grad, bias_grad_stride,
-          shared ? (float*)d_work : nullptr, rows, (int)each, nc, tiles, Legal{d_legal, legal_stride}, t);
+      const auto* gy = (const Elem<DT>::T*)d_grad_out;
+      auto* gx = (Elem<DT>::T*)d_grad;
+      const int tiles = (int)tiles_of(cols, NT * PER<DT>);
+      k_adjust_grad<DT><<<(unsigned)(chunks * tiles), NT, 0, s>>>(gy, grad_out_stride, gx, grad_stride,
+                                                                shared ? nullptr : d_bias_grad, bias_grad_stride,
+                                                                shared ? (float*)d_work : nullptr, rows, (int)each, nc,
+                                                                tiles, legal);
+      if (gx && t.actions)
+        k_taken_grad<DT><<<(unsigned)((rows * groups + 3) / 4), 256, 0, s>>>(gy, grad_out_stride,
+                                                                           (const Elem<DT>::T*)d_logits, logits_stride, gx,
+                                                                           grad_stride, rows, nc, (int)groups, legal, t);
     });
   }
   if (shared) k_bias_join<<<(nc + 255) / 256, 256, 0, s>>>((const float*)d_work, (int)chunks, nc, d_bias_grad);
@@ -719,15 +815,15 @@ extern "C" int mtaz_policy_loss(int device, int64_t rows, int64_t cols, int dtyp
     } else if (cols <= WAVE_COLS) {
       k_loss_wave<DT, DP, false><<<(n + 3) / 4, 256, 0, s>>>(z, logits_stride, pi, target_stride, rows, nc, legal, d_value,
                                                            d_reward, d_stats, d_loss, g, grad_stride, d_value_grad, k);
-    } else if (cols <= 4096) {
-      k_loss_block<DT, DP, 256, 16 / N><<<n, 256, 0, s>>>(z, logits_stride, pi, target_stride, nc, legal, d_value, d_reward,
-                                                         d_stats, g, grad_stride, d_value_grad, k);
-    } else if (cols <= 16384) {
-      k_loss_block<DT, DP, 1024, 16 / N><<<n, 1024, 0, s>>>(z, logits_stride, pi, target_stride, nc, legal, d_value, d_reward,
-                                                           d_stats, g, grad_stride, d_value_grad, k);
     } else if (cols <= BLOCK_COLS) {
-      k_loss_block<DT, DP, 1024, 32 / N><<<n, 1024, 0, s>>>(z, logits_stride, pi, target_stride, nc, legal, d_value, d_reward,
-                                                           d_stats, g, grad_stride, d_value_grad, k);
+      auto launch = [&](auto kernel, int threads) {
+        kernel<<<n, threads, 0, s>>>(z, logits_stride, pi, target_stride, nc, legal, d_value, d_reward, d_stats, g,
+                                     grad_stride, d_value_grad, k);
+      };
+      constexpr int LONG = DP == MTAZ_F32 ? 1024 : 512;
+      if (cols <= 4096) launch(k_loss_block<DT, DP, 256, 16 / N>, 256);
+      else if (cols <= 16384) launch(k_loss_block<DT, DP, 1024, 16 / N>, 1024);
+      else launch(k_loss_block<DT, DP, LONG, BLOCK_COLS / (LONG * N)>, LONG);
     } else {
       const int tiles = (int)tiles_of(cols, LOSS_TILE<DT>);
       k_loss_part<DT, DP><<<n * tiles, NT, 0, s>>>(z, logits_stride, pi, target_stride, nc, tiles, legal, (Soft*)d_work);

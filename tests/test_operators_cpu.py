@@ -70,7 +70,7 @@ def test_adjust_nothing():
 
 @pytest.mark.parametrize('args,why', [
     (dict(gy=None), 'incoming'), (dict(x=None), 'needs the logits'), (dict(gs=39), 'overlap'), (dict(bs=39), 'overlap'),
-    (dict(bs=0, size=100), 'workspace'), (dict(bs=0, work=None), 'workspace')])
+    (dict(bs=0, size=100), 'workspace'), (dict(bs=0, work=None), 'workspace'), (dict(), 'in place')])
 def test_adjust_grad_refuses(args, why):
     a = dict(gy=P, x=P, gs=40, bs=40, work=P, size=1 << 20)
     a.update(args)
