@@ -39,8 +39,10 @@ struct Matrices {
 struct Shape {
   int rows, cols;             // of the matrix as it lies in memory
   int r, L;                   // short and long side
-  int rp, Lp;                 // padded to whole tiles
-  int tile_r, tile_L;         // tile of the products over r x r and over r x L: 64 or 128
+  int rp, Lp;                 // padded to whole tiles over r x L
+  int tile_r, tile_L;         // tile of the products over r x r (64, 96 or 128) and over r x L (64 or 128)
+  int height;                 // rows of X, S, B and C in memory: rp, padded to whole tiles over r x r; what lies behind
+                              // rp is read, but by nothing that is kept
   int parts;                  // workgroups for the sum of squares
 };
 struct Update {
@@ -282,7 +284,7 @@ void k_product(Product pr, Out out) {
   constexpr int PITCH = W + 4, PART = W * PITCH;        // floats of a wave's sums in LDS
   constexpr int LOOP = RING * 2 * HALF * 2, END = WAVES * PART * 4;
   static_assert(T * DEPTH % (256 * WAVES) == 0 && DEPTH % (16 * GROUPS) == 0 && 64 % DEPTH == 0, "round");
-  static_assert(F % 2 == 0, "read_cols");
+  static_assert(!COLS || F % 2 == 0, "read_cols");
   __shared__ __attribute__((aligned(1024))) char shared[LOOP > END ? LOOP : END];
   _Float16* lds = reinterpret_cast<_Float16*>(shared);
   const int lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
@@ -407,9 +409,11 @@ void k_product(Product pr, Out out) {
       }
   ready<0>();
   constexpr int PER_ROW = W / 8, SHARE = W / GROUPS;    // lanes a row, 8 elements each; rows a wave
+  constexpr int ROWS = 64 / PER_ROW;                    // rows at a time; lanes behind the last whole row have none
+  const int row0 = lane < ROWS * PER_ROW ? group * SHARE + lane / PER_ROW : W;
   const bool turn = KIND < APPLY ? bm != bn : KIND > APPLY && tall(out);   // leaves transposed (too), below
 #pragma unroll 4
-  for (int row = group * SHARE + lane / PER_ROW; row < (group + 1) * SHARE; row += 64 / PER_ROW) {
+  for (int row = row0; row < (group + 1) * SHARE; row += ROWS) {
     const int col = lane % PER_ROW * 8, n = bn * T + n0 + row, m = bm * T + m0 + col;
     float* at = sums + row * PITCH + col;
     float v[8];
@@ -445,7 +449,7 @@ void k_product(Product pr, Out out) {
   if (!turn) return;
   ready<0>();
 #pragma unroll 4
-  for (int row = group * SHARE + lane / PER_ROW; row < (group + 1) * SHARE; row += 64 / PER_ROW) {
+  for (int row = row0; row < (group + 1) * SHARE; row += ROWS) {
     const int col = lane % PER_ROW * 8, m = bm * T + m0 + row, n = bn * T + n0 + col;
     float v[8];
 #pragma unroll
@@ -746,25 +750,32 @@ Work layout(int n, const Shape& sh, char* base) {
     return p;
   };
   w.part = (double*)take(8 * PARTS * n);
-  w.X[0] = pairs(sh.rp, sh.Lp);
-  w.X[1] = pairs(sh.rp, sh.Lp);
-  w.S = pairs(sh.rp, sh.rp);
-  w.B = pairs(sh.rp, sh.rp);
-  w.C = pairs(sh.rp, sh.rp);
+  w.X[0] = pairs(sh.height, sh.Lp);
+  w.X[1] = pairs(sh.height, sh.Lp);
+  w.S = pairs(sh.height, sh.height);
+  w.B = pairs(sh.height, sh.height);
+  w.C = pairs(sh.height, sh.height);
   w.bytes = at;
   return w;
 }
 
-// Tiles of 128 where the matrices have enough of them to occupy half of the 256 CUs, else of 64
+// Tiles over r x L: 128 where the matrices have enough of them to occupy half of the 256 CUs, else 64.  Over r x r, on
+// and below the diagonal: the size that takes the fewest rounds of 256, each in proportion to its area; a tile of 64
+// reads twice as much a product as one of 128 and counts for a third more.  (2048 x 2048: 136 tiles of 128 leave half
+// of the chip without work and take 47 us a square; 253 of 96 fill it.)
 Shape shape_of(int n, int64_t rows, int64_t cols) {
   Shape s;
   s.rows = (int)rows, s.cols = (int)cols;
   s.r = (int)(rows < cols ? rows : cols), s.L = (int)(rows < cols ? cols : rows);
-  const int64_t tr = up(s.r, 128) / 128, tL = up(s.L, 128) / 128;
-  s.tile_r = n * tr * (tr + 1) / 2 >= 128 ? 128 : 64;
-  s.tile_L = n * tr * tL >= 128 ? 128 : 64;
-  s.rp = (int)up(s.r, s.tile_r > s.tile_L ? s.tile_r : s.tile_L);
-  s.Lp = (int)up(s.L, s.tile_L);
+  s.tile_L = n * (up(s.r, 128) / 128) * (up(s.L, 128) / 128) >= 128 ? 128 : 64;
+  s.rp = (int)up(s.r, s.tile_L), s.Lp = (int)up(s.L, s.tile_L);
+  double best = 0.;
+  for (int T : {128, 96, 64}) {
+    const int64_t t = up(s.rp, T) / T, tiles = n * t * (t + 1) / 2;
+    const double cost = (double)T * T * (double)((tiles + 255) / 256) * (T == 64 ? 4. / 3. : T == 96 ? 1.05 : 1.);
+    if (T == 128 || cost < best) best = cost, s.tile_r = T;
+  }
+  s.height = (int)up(s.rp, s.tile_r);
   const int64_t parts = up(rows * cols, 8 * NT * 2) / (8 * NT * 2);   // two rounds each at least
   s.parts = (int)(parts < PARTS ? parts : PARTS);
   return s;
@@ -837,6 +848,8 @@ void product(Product pr, int T, const Out& out, hipStream_t s) {
   if (T == 128) {
     if (grid <= 256) k_product<128, 2, 2, 32, 4, KIND, DT, Out><<<grid, 512, 0, s>>>(pr, out);
     else k_product<128, 2, 1, 32, 2, KIND, DT, Out><<<grid, 256, 0, s>>>(pr, out);
+  } else if (T == 96) {
+    if constexpr (KIND < APPLY) k_product<96, 1, 4, 64, 3, KIND, DT, Out><<<grid, 256, 0, s>>>(pr, out);
   } else {
     if (grid <= 256) k_product<64, 1, 4, 64, 4, KIND, DT, Out><<<grid, 256, 0, s>>>(pr, out);
     else k_product<64, 1, 4, 64, 2, KIND, DT, Out><<<grid, 256, 0, s>>>(pr, out);
@@ -865,7 +878,7 @@ void iterate(const Matrices& ms, int n, const Shape& sh, const Update& u, int st
   const int64_t count = (int64_t)sh.rows * sh.cols;
   k_squares<DT, MUON><<<dim3(sh.parts, n), NT, 0, s>>>(ms, count, u, w.part);
   k_pairs<DT, MUON><<<dim3(sh.Lp / 64, sh.rp / 64, n), NT, 0, s>>>(ms, sh, u, w.part, eps, ldexp(1., e.x[0]), w.X[0]);
-  const int tr = sh.rp / sh.tile_r, tri = tr * (tr + 1) / 2;
+  const int tr = sh.height / sh.tile_r, tri = tr * (tr + 1) / 2;
   const int tL = sh.Lp / sh.tile_L, tall = sh.rp / sh.tile_L * tL;
   auto two = [](int k) { return (float)ldexp(1., k); };
   auto gram = [&](const Pairs& P, const Pairs& Q, const Pairs& D, int depth, int shift) {   // D = 2^shift P Q^T, symmetric
@@ -905,12 +918,15 @@ void iterate(const Matrices& ms, int n, const Shape& sh, const Update& u, int st
   }
 }
 
-// of the largest group; a smaller last one may choose smaller tiles, never larger ones
+// of the whole groups or of the last one, which may choose other tiles
 int64_t workspace(int n, int64_t rows, int64_t cols) {
-  const int m = n < MOST ? n : MOST;
-  const Shape sh = shape_of(m, rows, cols);
-  Small sm;
-  return small(sh, sm) ? 256 : layout(m, sh, nullptr).bytes;
+  auto of = [&](int m) {
+    const Shape sh = shape_of(m, rows, cols);
+    Small sm;
+    return m == 0 || small(sh, sm) ? 256 : layout(m, sh, nullptr).bytes;
+  };
+  const int64_t whole = of(n < MOST ? n : MOST), rest = of(n % MOST);
+  return whole > rest ? whole : rest;
 }
 
 // All checks, then the matrices in groups of at most MOST over the same workspace

@@ -46,6 +46,13 @@ def test_gaussian(shape, dtype):
     assert off(optim.orthogonalize(g), reference(g)) <= TIGHT + HALF[dtype]
 
 
+@pytest.mark.parametrize('shape,dtype', [((8, 530, 1100), torch.float32), ((1, 1450, 2900), torch.bfloat16),
+                                         ((67, 140, 300), torch.float32)], ids=str)
+def test_other_tiles_and_groups(shape, dtype):
+    g = randn(*shape, seed=sum(shape), dtype=dtype)
+    assert off(optim.orthogonalize(g), reference(g)) <= TIGHT + HALF[dtype]
+
+
 @pytest.mark.parametrize('shape', [(1, 1), (1, 7), (7, 1), (2, 2), (31, 33), (64, 64), (128, 128), (255, 255), (300, 301)],
                          ids=str)
 def test_square_small_and_odd(shape):
