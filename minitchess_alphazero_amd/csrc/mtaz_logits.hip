@@ -33,15 +33,18 @@ struct Taken {
   int64_t stride;
   const int32_t* lengths;
   int history;
-  float repetition, frequency, presence;
+  float repetition, inverse, frequency, presence;       // inverse: 1 / repetition
   const float* per_row;
 };
 struct Penalty {
-  float repetition, frequency, presence;
+  float repetition, inverse, frequency, presence;
 };
 __device__ __forceinline__ Penalty penalty_of(const Taken& t, int64_t row) {
-  if (t.per_row) return {t.per_row[3 * row], t.per_row[3 * row + 1], t.per_row[3 * row + 2]};
-  return {t.repetition, t.frequency, t.presence};
+  if (t.per_row) {
+    const float* p = t.per_row + 3 * row;
+    return {p[0], 1.f / p[0], p[1], p[2]};
+  }
+  return {t.repetition, t.inverse, t.frequency, t.presence};
 }
 // calls f for every action that the row has taken, THREADS threads in steps of four entries; the first entries are
 // asked for before the length is there.  Entries outside [0, cols) lie outside every tile.
@@ -63,28 +66,101 @@ template <int THREADS, typename F> __device__ __forceinline__ void each_taken(co
   }
 }
 
-// N elements, n of them there
-template <typename T, int N> __device__ __forceinline__ Pack<T, N> load(const T* p, int n) {
-  Pack<T, N> r;
-  if (n >= N) return *reinterpret_cast<const Pack<T, N>*>(p);
-#pragma unroll
-  for (int j = 0; j < N; ++j) r.v[j] = j < n ? p[j] : (T)0.f;
-  return r;
+// An address that the compiler does not know to be p: it joins the first of a row's last few elements with the wide
+// access of the other path, which then falls into two or three.
+template <typename T> __device__ __forceinline__ T* apart(T* p) {
+  asm("" : "+v"(p));
+  return p;
 }
-template <typename T, int N> __device__ __forceinline__ void store(T* p, const Pack<T, N>& r, int n) {
-  if (n >= N) {
-    *reinterpret_cast<Pack<T, N>*>(p) = r;
-    return;
+// N elements packed in 32-bit words: 16-bit values of their own would take a register each, and where two paths join,
+// the wide load's words would be taken apart as soon as they are there.
+template <int DT, int N> struct Words {
+  typedef typename Elem<DT>::T T;
+  static constexpr int W = N * (int)sizeof(T) / 4;
+  uint32_t w[W];
+  __device__ __forceinline__ void fetch(const T* p, int n) {   // n of them there, the others 0
+    if (n >= N) {
+      __builtin_memcpy(w, p, sizeof(w));
+    } else {
+      p = apart(p);
+#pragma unroll
+      for (int i = 0; i < W; ++i) w[i] = 0;
+#pragma unroll
+      for (int j = 0; j < N; ++j)
+        if (j < n) put(j, p[j]);
+      forget();
+    }
   }
+  __device__ __forceinline__ float get(int j) const {
+    if constexpr (DT == MTAZ_F32) return __builtin_bit_cast(float, w[j]);
+    if constexpr (DT == MTAZ_BF16) return __builtin_bit_cast(float, j & 1 ? w[j / 2] & 0xffff0000u : w[j / 2] << 16);
+    if constexpr (DT == MTAZ_F16) return (float)__builtin_bit_cast(_Float16, (uint16_t)(w[j / 2] >> (16 * (j & 1))));
+  }
+  __device__ __forceinline__ void put(int j, T x) {
+    if constexpr (DT == MTAZ_F32) w[j] = __builtin_bit_cast(uint32_t, x);
+    else {
+      const uint32_t half = __builtin_bit_cast(uint16_t, x);
+      w[j / 2] = j & 1 ? (w[j / 2] & 0xffffu) | half << 16 : (w[j / 2] & 0xffff0000u) | half;
+    }
+  }
+  __device__ __forceinline__ void leave(T* p, int n) const {
+    if (n >= N) {
+      __builtin_memcpy(p, w, sizeof(w));
+      return;
+    }
+    p = apart(p);
 #pragma unroll
-  for (int j = 0; j < N; ++j)
-    if (j < n) p[j] = r.v[j];
-}
+    for (int j = 0; j < N; ++j) {
+      if (j >= n) continue;
+      if constexpr (sizeof(T) == 4) p[j] = __builtin_bit_cast(T, w[j]);
+      else p[j] = __builtin_bit_cast(T, (uint16_t)(w[j / 2] >> (16 * (j & 1))));
+    }
+  }
+  // what lies under the bits of ok, and `other` elsewhere (a value's bits, twice where they are 16)
+  __device__ __forceinline__ void keep(uint32_t ok, uint32_t other) {
+#pragma unroll
+    for (int i = 0; i < W; ++i) {
+      uint32_t m;
+      if constexpr (DT == MTAZ_F32) m = bits_of(ok, i);
+      else m = (bits_of(ok, 2 * i) & 0xffffu) | (bits_of(ok, 2 * i + 1) << 16);
+      w[i] = (w[i] & m) | (other & ~m);
+    }
+  }
+  static __device__ __forceinline__ uint32_t bits_of(uint32_t ok, int j) { return 0u - ((ok >> j) & 1u); }
+  // The compiler forgets how the words came about: else it keeps every value as a float from one phase to the next.
+  __device__ __forceinline__ void forget() {
+#pragma unroll
+    for (int i = 0; i < W; ++i) asm volatile("" : "+v"(w[i]));
+  }
+};
 
 // ---- penalties, bias, mask -----------------------------------------------------------------------------------
-__device__ __forceinline__ float adjusted(float x, uint32_t count, float bias, const Penalty& p) {
-  if (count) x = (x > 0.f ? x / p.repetition : x * p.repetition) - p.frequency * (float)count - p.presence;
-  return x + bias;
+template <int DT> constexpr uint32_t NEVER = DT == MTAZ_F32 ? 0xff800000u : DT == MTAZ_F16 ? 0xfc00fc00u : 0xff80ff80u;
+// One access: N logits, the counts of their actions (none: nullptr), their bias and legality.  Without a branch and
+// with the reciprocal of the repetition penalty, because a few taken actions among many others are enough to send
+// every wave through all branches.
+template <int DT, int N>
+__device__ __forceinline__ void adjust(Words<DT, N>& q, const uint32_t* cnt, const Words<MTAZ_F32, N>& bias, uint32_t ok,
+                                       const Penalty& p) {
+  typedef Elem<DT> E;
+  float f[N];
+#pragma unroll
+  for (int j = 0; j < N; ++j) f[j] = q.get(j);
+  if (cnt) {
+#pragma unroll
+    for (int i = 0; i < N; i += 4) {
+      const uint4 four = *reinterpret_cast<const uint4*>(cnt + i);
+      const uint32_t c[4] = {four.x, four.y, four.z, four.w};
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const float x = f[i + j], y = fmaf(-p.frequency, (float)c[j], x * (x > 0.f ? p.inverse : p.repetition)) - p.presence;
+        f[i + j] = c[j] ? y : x;
+      }
+    }
+  }
+#pragma unroll
+  for (int j = 0; j < N; ++j) q.put(j, E::put(f[j] + bias.get(j)));
+  q.keep(ok, NEVER<DT>);
 }
 
 // Rows of up to WAVE_COLS columns: a wave each, with the counts of its actions in its own piece of LDS.
@@ -93,19 +169,18 @@ template <int DT>
 __global__ __launch_bounds__(256) void k_adjust_wave(const typename Elem<DT>::T* x, int64_t x_stride,
                                                      typename Elem<DT>::T* y, int64_t y_stride, int64_t rows, int cols,
                                                      Legal legal, const float* bias, int64_t bias_stride, Taken taken) {
-  typedef Elem<DT> E;
   constexpr int N = PER<DT>, REP = WAVE_COLS / (64 * N);
   __shared__ __attribute__((aligned(16))) uint32_t counts[4][WAVE_COLS];
   const int lane = threadIdx.x % 64, wave = threadIdx.x / 64;
   const int64_t row = (int64_t)blockIdx.x * 4 + wave;
   if (row >= rows) return;
-  Pack<typename E::T, N> q[REP];
+  Words<DT, N> q[REP];
 #pragma unroll
   for (int k = 0; k < REP; ++k) {
     const int v = N * (lane + 64 * k);
-    if (v < cols) q[k] = load<typename E::T, N>(x + row * x_stride + v, cols - v);
+    if (v < cols) q[k].fetch(x + row * x_stride + v, cols - v);
   }
-  Penalty p = {1.f, 0.f, 0.f};
+  Penalty p = {};
   uint32_t* cnt = counts[wave];
   const bool counted = taken.actions != nullptr;
   if (counted) {                                        // LDS serves one wave's accesses in order
@@ -123,59 +198,52 @@ __global__ __launch_bounds__(256) void k_adjust_wave(const typename Elem<DT>::T*
     const int v = N * (lane + 64 * k), n = cols - v;
     if (n <= 0) continue;
     const uint32_t ok = legal.some<N>(row, v, n);
-    Pack<float, N> b = {};
-    if (bias && ok) b = load<float, N>(bias + row * bias_stride + v, n);
-#pragma unroll
-    for (int j = 0; j < N; ++j)
-      q[k].v[j] = E::put((ok >> j) & 1u ? adjusted(E::get(q[k].v[j]), counted ? cnt[v + j] : 0u, b.v[j], p) : -INFINITY);
-    store(y + row * y_stride + v, q[k], n);
+    Words<MTAZ_F32, N> b = {};
+    if (bias && ok) b.fetch(bias + row * bias_stride + v, n);
+    adjust<DT, N>(q[k], counted ? cnt + v : nullptr, b, ok, p);
+    q[k].leave(y + row * y_stride + v, n);
   }
 }
 
-// Longer rows in tiles, so that one long row fills the chip as well as many: a workgroup per tile counts the actions
-// in its columns.  Integer adds, so their order does not matter.  REP: accesses a thread; the more, the fewer
-// workgroups look through a row's actions.
+// Longer rows in tiles, so that one long row fills the chip as well as many: a workgroup counts the actions in its
+// columns.  Integer adds, so their order does not matter.  One access a thread and four workgroups on a CU hide each
+// other's phases; two accesses take 84 registers and only two workgroups fit (1024 x 50021 f16 with everything 52 and
+// 62 us, 205 MB; f32 92 and 97).  A workgroup takes `per` rows one after the other, more than one only where they share
+// mask and bias, which it then reads once.
 constexpr int NT = 512;
-template <int DT, int REP>
+template <int DT, bool COUNTED>
 __global__ __launch_bounds__(NT) void k_adjust(const typename Elem<DT>::T* x, int64_t x_stride,
-                                               typename Elem<DT>::T* y, int64_t y_stride, int cols, int tiles,
-                                               Legal legal, const float* bias, int64_t bias_stride, Taken taken) {
-  typedef Elem<DT> E;
-  constexpr int N = PER<DT>, TILE = NT * N * REP;
-  __shared__ __attribute__((aligned(16))) uint32_t cnt[TILE];
-  const int64_t row = blockIdx.x / tiles;
-  const int v0 = (int)(blockIdx.x % tiles) * TILE;
-  const bool counted = taken.actions != nullptr;
-  Pack<typename E::T, N> q[REP];
-  Pack<float, N> b[REP] = {};
-  uint32_t ok[REP];
+                                               typename Elem<DT>::T* y, int64_t y_stride, int64_t rows, int per, int cols,
+                                               int tiles, Legal legal, const float* bias, int64_t bias_stride,
+                                               Taken taken) {
+  constexpr int N = PER<DT>, TILE = NT * N;
+  __shared__ __attribute__((aligned(16))) uint32_t cnt[COUNTED ? TILE : 4];
+  const int64_t r0 = (int64_t)(blockIdx.x / tiles) * per, r1 = min(rows, r0 + per);
+  const int v0 = (int)(blockIdx.x % tiles) * TILE, i = N * threadIdx.x, v = v0 + i, n = cols - v;
+  Words<DT, N> q;
+  Words<MTAZ_F32, N> b = {};
+  if (n > 0) q.fetch(x + r0 * x_stride + v, n);
+  const uint32_t ok = legal.some<N>(r0, v, n);
+  if (bias && ok) b.fetch(bias + r0 * bias_stride + v, n);
+  for (int64_t row = r0; row < r1; ++row) {
+    if (row > r0 && n > 0) q.fetch(x + row * x_stride + v, n);
+    Penalty p = {};
+    if (COUNTED) {
+      p = penalty_of(taken, row);
 #pragma unroll
-  for (int k = 0; k < REP; ++k) {
-    const int v = v0 + N * (threadIdx.x + NT * k), n = cols - v;
-    ok[k] = legal.some<N>(row, v, n);
-    if (n > 0) q[k] = load<typename E::T, N>(x + row * x_stride + v, n);
-    if (bias && ok[k]) b[k] = load<float, N>(bias + row * bias_stride + v, n);
-  }
-  Penalty p = {1.f, 0.f, 0.f};
-  if (counted) {
-    p = penalty_of(taken, row);
-#pragma unroll
-    for (int k = 0; k < TILE / (4 * NT); ++k) *reinterpret_cast<uint4*>(cnt + 4 * (threadIdx.x + NT * k)) = make_uint4(0, 0, 0, 0);
-    __syncthreads();
-    each_taken<NT>(taken, row, threadIdx.x, [&](int a) {
-      const uint32_t at = (uint32_t)a - (uint32_t)v0;
-      if (at < (uint32_t)TILE) atomicAdd(&cnt[at], 1u);
-    });
-    __syncthreads();
-  }
-#pragma unroll
-  for (int k = 0; k < REP; ++k) {
-    const int i = N * (threadIdx.x + NT * k), n = cols - v0 - i;
-    if (n <= 0) continue;
-#pragma unroll
-    for (int j = 0; j < N; ++j)
-      q[k].v[j] = E::put((ok[k] >> j) & 1u ? adjusted(E::get(q[k].v[j]), counted ? cnt[i + j] : 0u, b[k].v[j], p) : -INFINITY);
-    store(y + row * y_stride + v0 + i, q[k], n);
+      for (int k = 0; k < N / 4; ++k) *reinterpret_cast<uint4*>(cnt + 4 * (threadIdx.x + NT * k)) = make_uint4(0, 0, 0, 0);
+      __syncthreads();
+      each_taken<NT>(taken, row, threadIdx.x, [&](int a) {
+        const uint32_t at = (uint32_t)a - (uint32_t)v0;
+        if (at < (uint32_t)TILE) atomicAdd(&cnt[at], 1u);
+      });
+      __syncthreads();
+    }
+    if (n > 0) {
+      adjust<DT, N>(q, COUNTED ? cnt + i : nullptr, b, ok, p);
+      q.leave(y + row * y_stride + v, n);
+    }
+    if (COUNTED && row + 1 < r1) __syncthreads();       // all have read their counts
   }
 }
 
@@ -186,36 +254,41 @@ __global__ __launch_bounds__(NT) void k_adjust_grad(const typename Elem<DT>::T* 
                                                     typename Elem<DT>::T* gx, int64_t gx_stride, float* gb,
                                                     int64_t gb_stride, float* part, int64_t rows, int per, int cols,
                                                     int tiles, Legal legal) {
-  typedef Elem<DT> E;
   constexpr int N = PER<DT>;
   const int64_t chunk = blockIdx.x / tiles, r0 = chunk * per, r1 = min(rows, r0 + per);
   const int v = ((int)(blockIdx.x % tiles) * NT + threadIdx.x) * N, n = cols - v;
   if (n <= 0) return;
-  Pack<float, N> sum = {};
-  auto take = [&](int64_t row, const Pack<typename E::T, N>& g) {
-    const uint32_t ok = legal.some<N>(row, v, n);
-    Pack<typename E::T, N> o;
-    Pack<float, N> f;
+  float sum[N] = {};
+  const uint32_t first = legal.some<N>(r0, v, n);
+  auto take = [&](int64_t row, Words<DT, N>& g) {
+    g.keep(legal.stride == 0 ? first : legal.some<N>(row, v, n), 0);
+    if (gx) g.leave(gx + row * gx_stride + v, n);
+    Words<MTAZ_F32, N> f;
 #pragma unroll
     for (int j = 0; j < N; ++j) {
-      f.v[j] = (ok >> j) & 1u ? E::get(g.v[j]) : 0.f;
-      sum.v[j] += f.v[j];
-      o.v[j] = E::put(f.v[j]);
+      f.put(j, g.get(j));
+      sum[j] += g.get(j);
     }
-    if (gb) store(gb + row * gb_stride + v, f, n);
-    if (gx) store(gx + row * gx_stride + v, o, n);
+    if (gb) f.leave(gb + row * gb_stride + v, n);
   };
-  int64_t row = r0;
-  if (n >= N)                                           // four rows' loads under way at once
-    for (; row + 4 <= r1; row += 4) {
-      Pack<typename E::T, N> g[4];
+  constexpr int AHEAD = 4;                              // rows under way at once
+  Words<DT, N> g[AHEAD];
 #pragma unroll
-      for (int k = 0; k < 4; ++k) g[k] = *reinterpret_cast<const Pack<typename E::T, N>*>(gy + (row + k) * gy_stride + v);
+  for (int k = 0; k < AHEAD; ++k)
+    if (r0 + k < r1) g[k].fetch(gy + (r0 + k) * gy_stride + v, n);
+  for (int64_t row = r0; row < r1; row += AHEAD)
 #pragma unroll
-      for (int k = 0; k < 4; ++k) take(row + k, g[k]);
+    for (int k = 0; k < AHEAD; ++k) {
+      if (row + k >= r1) break;
+      take(row + k, g[k]);
+      if (row + k + AHEAD < r1) g[k].fetch(gy + (row + k + AHEAD) * gy_stride + v, n);
     }
-  for (; row < r1; ++row) take(row, load<typename E::T, N>(gy + row * gy_stride + v, n));
-  if (part) store(part + chunk * cols + v, sum, n);
+  if (part) {
+    Words<MTAZ_F32, N> f;
+#pragma unroll
+    for (int j = 0; j < N; ++j) f.put(j, sum[j]);
+    f.leave(part + chunk * cols + v, n);
+  }
 }
 // Afterwards the few places of taken actions: d x = d y * slope, the slope 1 / repetition (x > 0) or repetition.  A
 // thread per entry of the list; an action that is in it twice is written twice alike.
@@ -231,9 +304,9 @@ __global__ __launch_bounds__(256) void k_taken_grad(const typename Elem<DT>::T* 
   const int v = taken.actions[row * taken.stride + i];
   if (taken.lengths && i >= taken.lengths[row]) return;
   if ((uint32_t)v >= (uint32_t)cols || !legal.some<1>(row, v, 1)) return;
-  const float rep = penalty_of(taken, row).repetition;
+  const Penalty p = penalty_of(taken, row);
   const float g = E::get(gy[row * gy_stride + v]);
-  gx[row * gx_stride + v] = E::put(E::get(x[row * x_stride + v]) > 0.f ? g * (1.f / rep) : g * rep);
+  gx[row * gx_stride + v] = E::put(E::get(x[row * x_stride + v]) > 0.f ? g * p.inverse : g * p.repetition);
 }
 // the workgroups' sums, in order
 __global__ __launch_bounds__(256) void k_bias_join(const float* part, int chunks, int cols, float* gb) {
@@ -282,47 +355,6 @@ __device__ __forceinline__ float wave_max(float x) {
   for (int o = 32; o; o >>= 1) x = fmaxf(x, __shfl_xor(x, o));
   return x;
 }
-
-// N elements packed in 32-bit words: 16-bit values of their own would take a register each.
-template <int DT, int N> struct Words {
-  typedef typename Elem<DT>::T T;
-  static constexpr int W = N * (int)sizeof(T) / 4;
-  uint32_t w[W];
-  __device__ __forceinline__ void fetch(const T* p, int n) {   // n of them there, the others 0
-    if (n >= N) {
-      const Pack<T, N> q = *reinterpret_cast<const Pack<T, N>*>(p);
-      __builtin_memcpy(w, &q, sizeof(q));
-    } else {
-#pragma unroll
-      for (int i = 0; i < W; ++i) w[i] = 0;
-#pragma unroll
-      for (int j = 0; j < N; ++j)
-        if (j < n) put(j, p[j]);
-    }
-  }
-  __device__ __forceinline__ float get(int j) const {
-    if constexpr (DT == MTAZ_F32) return __builtin_bit_cast(float, w[j]);
-    if constexpr (DT == MTAZ_BF16) return __builtin_bit_cast(float, j & 1 ? w[j / 2] & 0xffff0000u : w[j / 2] << 16);
-    if constexpr (DT == MTAZ_F16) return (float)__builtin_bit_cast(_Float16, (uint16_t)(w[j / 2] >> (16 * (j & 1))));
-  }
-  __device__ __forceinline__ void put(int j, T x) {
-    if constexpr (DT == MTAZ_F32) w[j] = __builtin_bit_cast(uint32_t, x);
-    else {
-      const uint32_t half = __builtin_bit_cast(uint16_t, x);
-      w[j / 2] = j & 1 ? (w[j / 2] & 0xffffu) | half << 16 : (w[j / 2] & 0xffff0000u) | half;
-    }
-  }
-  __device__ __forceinline__ void leave(T* p, int n) const {
-    Pack<T, N> q;
-    __builtin_memcpy(&q, w, sizeof(q));
-    store(p, q, n);
-  }
-  // The compiler forgets how the words came about: else it keeps every value as a float from one phase to the next.
-  __device__ __forceinline__ void forget() {
-#pragma unroll
-    for (int i = 0; i < W; ++i) asm volatile("" : "+v"(w[i]));
-  }
-};
 
 // A row in registers, THREADS threads with REP times PER logits each.  What is not legal, or not there, is held as a
 // logit of -inf with a target of 0, which adds nothing anywhere.  KEEP: the exponentials stay in registers from the sums
@@ -635,7 +667,7 @@ Taken taken_of(const int32_t* actions, int64_t stride, int history, const int32_
   if (!actions || history == 0) return t;
   if (!per_row && penalties[0] == 1. && penalties[1] == 0. && penalties[2] == 0.) return t;   // nothing to do
   t.actions = actions, t.stride = stride, t.lengths = lengths, t.history = history, t.per_row = per_row;
-  if (!per_row) t.repetition = (float)penalties[0], t.frequency = (float)penalties[1], t.presence = (float)penalties[2];
+  if (!per_row) t.repetition = (float)penalties[0], t.inverse = (float)(1. / penalties[0]), t.frequency = (float)penalties[1], t.presence = (float)penalties[2];
   return t;
 }
 // Longest row that stays in the registers of one workgroup
@@ -647,15 +679,14 @@ int launched(const char* what) {
   const hipError_t e = hipGetLastError();
   return e == hipSuccess ? 0 : ops_error(MTAZ_E_DEVICE, what, hipGetErrorString(e));
 }
-// Rows a workgroup of k_adjust_grad takes one after the other, and how many workgroups a column then has: one row,
-// unless a bias that the rows share is summed over them; then so few workgroups that they are all on the CUs at once.
-int64_t rows_each(int64_t rows, int64_t cols, bool shared) {
-  if (!shared) return 1;
+// Rows a workgroup of k_adjust_grad takes one after the other where their gradients are summed for a bias that they
+// share: so many that all workgroups are on the CUs at once.
+int64_t rows_each(int64_t rows, int64_t cols) {
   const int64_t across = tiles_of(cols, 512 * 8), chunks = across >= 1024 ? 1 : 1024 / across;
   return rows <= chunks ? 1 : (rows + chunks - 1) / chunks;
 }
 int64_t bias_chunks(int64_t rows, int64_t cols) {
-  const int64_t each = rows_each(rows, cols, true);
+  const int64_t each = rows_each(rows, cols);
   return (rows + each - 1) / each;
 }
 
@@ -699,15 +730,15 @@ extern "C" int mtaz_adjust_logits(int device, int64_t rows, int64_t cols, int dt
       k_adjust_wave<DT><<<(unsigned)((rows + 3) / 4), 256, 0, s>>>(x, logits_stride, y, out_stride, rows, nc, legal, d_bias,
                                                                  bias_stride, t);
     } else {
-      // two accesses a thread where the chip is full twice over either way (1024 x 50021 f16: 75 us with one, see there)
-      constexpr int TILE = NT * PER<DT>;
-      const int two = (int)tiles_of(cols, 2 * TILE), one = (int)tiles_of(cols, TILE);
-      if (rows * two >= 2048)
-        k_adjust<DT, 2><<<(unsigned)(rows * two), NT, 0, s>>>(x, logits_stride, y, out_stride, nc, two, legal, d_bias,
-                                                             bias_stride, t);
-      else
-        k_adjust<DT, 1><<<(unsigned)(rows * one), NT, 0, s>>>(x, logits_stride, y, out_stride, nc, one, legal, d_bias,
-                                                             bias_stride, t);
+      const int64_t tiles = tiles_of(cols, NT * PER<DT>);
+      // Two rows a workgroup where they share what it would read again, a float's bias for each logit, and the chip is
+      // full twice over all the same (1024 x 50021 f16: 52 us, with one row 59, with four 52; f32 92, 97 and 95).
+      const bool two = d_bias && bias_stride == 0 && (!d_legal || legal_stride == 0) && rows * tiles >= 4096;
+      const unsigned grid = (unsigned)((two ? (rows + 1) / 2 : rows) * tiles);
+      if (t.actions) k_adjust<DT, true><<<grid, NT, 0, s>>>(x, logits_stride, y, out_stride, rows, two ? 2 : 1, nc, (int)tiles,
+                                                            legal, d_bias, bias_stride, t);
+      else k_adjust<DT, false><<<grid, NT, 0, s>>>(x, logits_stride, y, out_stride, rows, two ? 2 : 1, nc, (int)tiles, legal,
+                                                   d_bias, bias_stride, t);
     }
   });
   return launched("adjust_logits");
@@ -744,7 +775,7 @@ extern "C" int mtaz_adjust_logits_grad(int device, int64_t rows, int64_t cols, i
   const int nc = (int)cols;
   const Legal legal{d_legal, legal_stride};
   const int64_t groups = (t.history + 63) / 64;         // of 64 entries
-  const int64_t each = rows_each(rows, cols, shared), chunks = rows ? (rows + each - 1) / each : 0;
+  const int64_t each = shared ? rows_each(rows, cols) : 1, chunks = rows ? (rows + each - 1) / each : 0;
   if (rows && (d_grad || d_bias_grad)) {
     FOR_TYPE(dtype, {
       const auto* gy = (const Elem<DT>::T*)d_grad_out;
