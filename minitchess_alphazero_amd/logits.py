@@ -226,8 +226,8 @@ def _loss(logits, target, value, reward, legal, grad, value_grad, scale):
         value, reward = value.contiguous(), reward.contiguous()
     entries = _lib.lib()
     work = _lib.check(entries.mtaz_policy_loss_workspace(rows, cols))
-    loss = torch.empty((), dtype=torch.float32, device=dev)
     stats = torch.empty(4 * rows + work // 4, dtype=torch.float32, device=dev)
+    loss = stats.new_empty(())
     at = stats.data_ptr()
     _lib.check(entries.mtaz_policy_loss(
         dev.index, rows, cols, TYPES[z.dtype], TYPES[t.dtype], z.data_ptr(), z.stride(0), t.data_ptr(), t.stride(0),
@@ -281,8 +281,6 @@ def policy_value_loss_grad(logits, target, value=None, reward=None, legal=None, 
     for torch.autograd.backward((logits, value), (d logits, d value)); the three are cut off from autograd's graph.
     With 16-bit logits a scale keeps small gradients in range."""
     _check_loss(logits, target, value, reward, legal)
-    logits = logits.detach()
     dz = _fresh(logits)
-    dv = None if value is None else torch.empty(value.shape, dtype=torch.float32, device=logits.device)
-    loss, _ = _loss(logits, target, None if value is None else value.detach(), reward, legal, dz, dv, float(scale))
-    return loss, dz, dv
+    dv = None if value is None else _fresh(value)
+    return _loss(logits, target, value, reward, legal, dz, dv, float(scale))[0], dz, dv
