@@ -108,7 +108,8 @@ int mtaz_replay_put(int device, int n, const uint32_t* d_pos, const int32_t* d_k
 /* Orthogonalisation of n matrices G [rows][cols] (contiguous, one pointer each in the host array
  * d_grad), rows, cols <= 65536 and rows * cols <= 2^30: X = G / (|G|_F + eps), then `steps` times
  * X <- a X + (b S + c S S) X with S = X X^T over the shorter side, coefficients = {a, b, c}.
- * Computed to 32 bits whatever the type; d_out[i] may be d_grad[i]. */
+ * Computed to 32 bits whatever the type, relative to the largest singular value; d_out[i] may be
+ * d_grad[i], and no other two matrices of a call may overlap. */
 int64_t mtaz_orthogonalize_workspace(int n, int64_t rows, int64_t cols, int dtype);
 int mtaz_orthogonalize(int device, int n, int64_t rows, int64_t cols, int dtype, const void* const* d_grad,
                        void* const* d_out, int steps, const double* coefficients, double eps, void* d_work,
@@ -116,7 +117,8 @@ int mtaz_orthogonalize(int device, int n, int64_t rows, int64_t cols, int dtype,
 /* One Muon step on n parameters of one shape and type, momenta float32:
  *   m <- momentum m + (1 - momentum) g;  u = nesterov ? (1 - momentum) g + momentum m : m;
  *   w <- (1 - lr weight_decay) w - lr scale orthogonalize(u).
- * Same workspace and limits as mtaz_orthogonalize. */
+ * Same workspace and limits as mtaz_orthogonalize; no parameter or momentum may overlap another
+ * tensor of the call. */
 int mtaz_muon_step(int device, int n, int64_t rows, int64_t cols, int dtype, void* const* d_params,
                    const void* const* d_grads, float* const* d_momenta, double lr, double momentum, int nesterov,
                    double weight_decay, double scale, int steps, const double* coefficients, double eps, void* d_work,
@@ -129,7 +131,8 @@ int mtaz_muon_step(int device, int n, int64_t rows, int64_t cols, int dtype, voi
  * [0, cols) do not.  Penalties {repetition, frequency, presence}: the host triple, or one triple per
  * row in d_penalties.  Strides are in elements (words for d_legal); cols <= 2^24.
  *
- * Adjusted logits y (same type; d_out may be d_logits with the same stride): with c = how often v
+ * Adjusted logits y (same type; d_out may be d_logits with the same stride, and may not overlap it
+ * otherwise): with c = how often v
  * was taken in the row, x <- c ? (x > 0 ? x / repetition : x repetition) - c frequency - presence : x;
  * y = x + bias where legal, -inf elsewhere whatever x holds there. */
 int mtaz_adjust_logits(int device, int64_t rows, int64_t cols, int dtype, const void* d_logits, int64_t logits_stride,
@@ -139,7 +142,8 @@ int mtaz_adjust_logits(int device, int64_t rows, int64_t cols, int dtype, const 
                        void* stream);
 /* Its backward pass: d_grad (NULL: not wanted) = d y / d x of the logits times d_grad_out, 0 where
  * not legal; d_bias_grad (NULL: not wanted) float32, per row, or summed over the rows in a fixed order
- * when bias_grad_stride is 0.  d_logits is read only where a repetition penalty applies. */
+ * when bias_grad_stride is 0.  d_logits is read only where a repetition penalty applies.
+ * d_grad may be d_grad_out (same stride) where no penalty applies. */
 int64_t mtaz_adjust_logits_grad_workspace(int64_t rows, int64_t cols);
 int mtaz_adjust_logits_grad(int device, int64_t rows, int64_t cols, int dtype, const void* d_grad_out,
                             int64_t grad_out_stride, const void* d_logits, int64_t logits_stride, void* d_grad,
@@ -153,9 +157,9 @@ int mtaz_adjust_logits_grad(int device, int64_t rows, int64_t cols, int dtype, c
  * and its mean over the rows into *d_loss (float32).  target_dtype: MTAZ_F32 or dtype.  d_value and
  * d_reward: [rows] float32, or both NULL (no value term).  Masked places are never read into a sum
  * (infinities and NaN there do not matter), a target of 0 adds nothing, and a row with nothing
- * legal, or with every legal logit -inf, adds its value term alone.  d_stats [rows][4] float32
- * receives what mtaz_policy_loss_grad needs.  d_grad / d_value_grad (either may be NULL) receive
- * the gradients of scale * loss in the same call. */
+ * legal, or with every legal logit -inf, adds its value term alone.  d_stats [rows][4] float32,
+ * 16-byte aligned, receives what mtaz_policy_loss_grad needs.  d_grad / d_value_grad (either may be
+ * NULL) receive the gradients of scale * loss in the same call; d_grad may be d_logits (same stride). */
 int64_t mtaz_policy_loss_workspace(int64_t rows, int64_t cols);
 int mtaz_policy_loss(int device, int64_t rows, int64_t cols, int dtype, int target_dtype, const void* d_logits,
                      int64_t logits_stride, const void* d_target, int64_t target_stride, const uint32_t* d_legal,

@@ -62,6 +62,8 @@ def policy_match(new_net, old_net, games, device=0, seed=0, tau_change=6, repeti
     from .engine import Engine
     from .environment import STARTING_FEN
     from .logits import adjust_logits, legal_masks
+    if games < 1:
+        raise ValueError(f'games must be at least 1, got {games}')
     dev = torch.device('cuda', device)
     rng = torch.Generator(device=dev).manual_seed(seed)
     engines = [Engine(n_games=games, sims=1, device=device) for _ in range(2)]   # the new and the old network

@@ -648,9 +648,27 @@ int64_t tiles_of(int64_t cols, int tile) { return (cols + tile - 1) / tile; }
 const char* bad_shape(int64_t rows, int64_t cols, int dtype) {
   if (rows < 0) return "rows must not be negative";
   if (cols < 1 || cols > MOST_COLS) return "cols must be in [1, 2^24]";
-  if (rows > INT32_MAX || rows * tiles_of(cols, 512 * 4) > INT32_MAX) return "too many rows for one call";
+  // a launch has fewer than 2^32 threads: 64 a row in the kernels for short rows, 512 a tile in the others
+  if (rows >= 1 << 26 || (cols > WAVE_COLS && rows * tiles_of(cols, 512 * 4) >= 1 << 23)) return "too many rows for one call";
   if (dtype < MTAZ_F32 || dtype > MTAZ_BF16) return "unknown element type";
   return nullptr;
+}
+// `rows` rows of cols elements of type dtype in memory
+struct Place {
+  const char* at;
+  int64_t step, width;                                  // bytes from row to row, and of a row
+  Place(const void* p, int64_t stride, int64_t cols, int dtype)
+      : at((const char*)p), step(stride * elem_size(dtype)), width(cols * elem_size(dtype)) {}
+};
+// Whether two places overlap.  The very same rows are allowed where `same` says so, and so are rows that interleave
+// (columns of one matrix).
+bool tangled(const Place& a, const Place& b, int64_t rows, bool same) {
+  if (!a.at || !b.at || rows == 0) return false;
+  if (a.at == b.at && a.width == b.width && (a.step == b.step || rows == 1)) return !same;
+  if (a.at + (rows - 1) * a.step + a.width <= b.at || b.at + (rows - 1) * b.step + b.width <= a.at) return false;
+  if (a.step != b.step || a.step <= 0) return true;
+  const int64_t off = ((b.at - a.at) % a.step + a.step) % a.step;   // from a row of a to the next of b
+  return off < a.width || a.step - off < b.width;
 }
 const char* bad_taken(const int32_t* actions, int64_t stride, int history, const double* penalties,
                       const float* per_row) {
@@ -679,8 +697,7 @@ int launched(const char* what) {
   const hipError_t e = hipGetLastError();
   return e == hipSuccess ? 0 : ops_error(MTAZ_E_DEVICE, what, hipGetErrorString(e));
 }
-// Rows a workgroup of k_adjust_grad takes one after the other where their gradients are summed for a bias that they
-// share: so many that all workgroups are on the CUs at once.
+// Rows a workgroup of k_adjust_grad takes one after the other: so many that all workgroups are on the CUs at once.
 int64_t rows_each(int64_t rows, int64_t cols) {
   const int64_t across = tiles_of(cols, 512 * 8), chunks = across >= 1024 ? 1 : 1024 / across;
   return rows <= chunks ? 1 : (rows + chunks - 1) / chunks;
@@ -714,7 +731,8 @@ extern "C" int mtaz_adjust_logits(int device, int64_t rows, int64_t cols, int dt
   if (!bad) bad = bad_taken(d_actions, actions_stride, history, penalties, d_penalties);
   if (!bad && (!d_logits || !d_out) && rows) bad = "no logits or no output";
   if (!bad && out_stride < cols && rows > 1) bad = "rows of the output overlap";
-  if (!bad && d_out == d_logits && out_stride != logits_stride && rows > 1) bad = "in place needs equal strides";
+  if (!bad && tangled({d_logits, logits_stride, cols, dtype}, {d_out, out_stride, cols, dtype}, rows, true))
+    bad = "the output overlaps the logits and is not in place";
   if (bad) return ops_error(MTAZ_E_FAIL, "adjust_logits", bad);
   if (rows == 0) return 0;
   DeviceScope on(device);
@@ -763,11 +781,14 @@ extern "C" int mtaz_adjust_logits_grad(int device, int64_t rows, int64_t cols, i
   const bool shared = d_bias_grad && bias_grad_stride == 0;
   if (!bad && rows && !d_grad_out) bad = "no incoming gradient";
   if (!bad && rows && t.actions && d_grad && !d_logits) bad = "the penalties' gradient needs the logits";
-  if (!bad && rows * ((history + 63) / 64) > INT32_MAX) bad = "too many rows for one call";
+  if (!bad && rows * ((history + 63) / 64) >= 1 << 26) bad = "too many rows for one call";
   if (!bad && rows > 1 && ((d_grad && grad_stride < cols) || (d_bias_grad && !shared && bias_grad_stride < cols)))
     bad = "rows of an output overlap";
   if (!bad && shared && rows && (!d_work || work_bytes < 4 * cols * bias_chunks(rows, cols))) bad = "workspace too small";
-  if (!bad && rows && t.actions && d_grad == d_grad_out) bad = "the penalties' gradient is not taken in place";
+  if (!bad && tangled({d_grad_out, grad_out_stride, cols, dtype}, {d_grad, grad_stride, cols, dtype}, rows, !t.actions))
+    bad = "the gradient overlaps the incoming one (in place is allowed without penalties)";
+  if (!bad && t.actions && tangled({d_logits, logits_stride, cols, dtype}, {d_grad, grad_stride, cols, dtype}, rows, false))
+    bad = "the gradient overlaps the logits";
   if (bad) return ops_error(MTAZ_E_FAIL, what, bad);
   DeviceScope on(device);
   if (on.status != hipSuccess) return ops_error(MTAZ_E_DEVICE, what, hipGetErrorString(on.status));
@@ -775,7 +796,7 @@ extern "C" int mtaz_adjust_logits_grad(int device, int64_t rows, int64_t cols, i
   const int nc = (int)cols;
   const Legal legal{d_legal, legal_stride};
   const int64_t groups = (t.history + 63) / 64;         // of 64 entries
-  const int64_t each = shared ? rows_each(rows, cols) : 1, chunks = rows ? (rows + each - 1) / each : 0;
+  const int64_t each = rows_each(rows, cols), chunks = rows ? (rows + each - 1) / each : 0;
   if (rows && (d_grad || d_bias_grad)) {
     FOR_TYPE(dtype, {
       const auto* gy = (const Elem<DT>::T*)d_grad_out;
@@ -813,6 +834,16 @@ static const char* bad_loss(int64_t rows, int64_t cols, int dtype, int target_dt
   if (grad && grad_stride < cols && rows > 1) return "rows of the gradient overlap";
   return nullptr;
 }
+// A gradient over its own logits is written where a thread has read them; over the targets likewise.
+static const char* bad_place(int64_t rows, int64_t cols, int dtype, int target_dtype, const void* logits,
+                             int64_t logits_stride, const void* target, int64_t target_stride, const void* grad,
+                             int64_t grad_stride) {
+  const Place g(grad, grad_stride, cols, dtype);
+  if (tangled({logits, logits_stride, cols, dtype}, g, rows, true) ||
+      tangled({target, target_stride, cols, target_dtype}, g, rows, true))
+    return "the gradient overlaps the logits or the targets and is not in place";
+  return nullptr;
+}
 
 extern "C" int mtaz_policy_loss(int device, int64_t rows, int64_t cols, int dtype, int target_dtype,
                                 const void* d_logits, int64_t logits_stride, const void* d_target,
@@ -825,6 +856,7 @@ extern "C" int mtaz_policy_loss(int device, int64_t rows, int64_t cols, int dtyp
                              grad_stride, d_value_grad);
   if (!bad && !d_loss) bad = "no place for the loss";
   if (!bad && (!d_work || work_bytes < loss_workspace(rows, cols))) bad = "workspace too small";
+  if (!bad) bad = bad_place(rows, cols, dtype, target_dtype, d_logits, logits_stride, d_target, target_stride, d_grad, grad_stride);
   if (bad) return ops_error(MTAZ_E_FAIL, what, bad);
   DeviceScope on(device);
   if (on.status != hipSuccess) return ops_error(MTAZ_E_DEVICE, what, hipGetErrorString(on.status));
@@ -877,6 +909,7 @@ extern "C" int mtaz_policy_loss_grad(int device, int64_t rows, int64_t cols, int
   const char* bad = bad_loss(rows, cols, dtype, target_dtype, d_logits, d_target, d_value, d_reward, d_stats, d_grad,
                              grad_stride, d_value_grad);
   if (!bad && !d_grad_out) bad = "no incoming gradient";
+  if (!bad) bad = bad_place(rows, cols, dtype, target_dtype, d_logits, logits_stride, d_target, target_stride, d_grad, grad_stride);
   if (bad) return ops_error(MTAZ_E_FAIL, what, bad);
   if (!d_grad && !d_value_grad) return 0;
   DeviceScope on(device);

@@ -918,6 +918,12 @@ void iterate(const Matrices& ms, int n, const Shape& sh, const Update& u, int st
   }
 }
 
+// Matrices that go through the kernels together: up to MOST, and fewer where they are so large that one fills the chip,
+// so that the workspace stays near 2 GiB
+int group_of(int64_t rows, int64_t cols) {
+  const int64_t m = (2ll << 30) / layout(1, shape_of(1, rows, cols), nullptr).bytes;
+  return m < 1 ? 1 : m < MOST ? (int)m : MOST;
+}
 // of the whole groups or of the last one, which may choose other tiles
 int64_t workspace(int n, int64_t rows, int64_t cols) {
   auto of = [&](int m) {
@@ -925,11 +931,12 @@ int64_t workspace(int n, int64_t rows, int64_t cols) {
     Small sm;
     return m == 0 || small(sh, sm) ? 256 : layout(m, sh, nullptr).bytes;
   };
-  const int64_t whole = of(n < MOST ? n : MOST), rest = of(n % MOST);
+  const int most = group_of(rows, cols);
+  const int64_t whole = of(n < most ? n : most), rest = of(n % most);
   return whole > rest ? whole : rest;
 }
 
-// All checks, then the matrices in groups of at most MOST over the same workspace
+// All checks, then the matrices in groups over the same workspace
 template <bool MUON>
 int run(const char* what, int device, int n, int64_t rows, int64_t cols, int dtype, const void* const* grad,
         void* const* out, float* const* momenta, const Update& u, int steps, const double* co, double eps, void* work,
@@ -949,8 +956,9 @@ int run(const char* what, int device, int n, int64_t rows, int64_t cols, int dty
     return ops_error(MTAZ_E_FAIL, what, "workspace too small or not aligned to 256 bytes");
   DeviceScope on(device);
   if (on.status != hipSuccess) return ops_error(MTAZ_E_DEVICE, what, hipGetErrorString(on.status));
-  for (int first = 0; first < n; first += MOST) {
-    const int m = n - first < MOST ? n - first : MOST;
+  const int most = group_of(rows, cols);
+  for (int first = 0; first < n; first += most) {
+    const int m = n - first < most ? n - first : most;
     Matrices ms = {};
     for (int i = 0; i < m; ++i) {
       ms.grad[i] = grad[first + i], ms.out[i] = out[first + i];

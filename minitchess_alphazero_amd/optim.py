@@ -11,6 +11,7 @@ the matrix [out, in * kh * kw].
 Every function enqueues on the current stream of its tensors' device, synchronizes nothing, and may be
 captured in a HIP graph.  There is no CPU form: tensors elsewhere are refused.
 """
+import bisect
 import ctypes
 import functools
 import math
@@ -52,6 +53,12 @@ def _check_type(t, what):
         raise ValueError(f'{what} must be float32, float16 or bfloat16, not {t.dtype}')
 
 
+def _span(t):
+    """The addresses of a contiguous tensor: (first, behind the last)."""
+    at = t.data_ptr()
+    return at, at + t.numel() * t.element_size()
+
+
 def _stream(device):
     """The current stream of a device, as the C entries take it."""
     return torch._C._cuda_getCurrentRawStream(device.index)
@@ -78,6 +85,9 @@ def orthogonalize(grad, steps=5, coefficients=COEFFICIENTS, eps=1e-7, out=None):
     rows, cols = grad.shape[-2:]
     n = math.prod(grad.shape[:-2])
     src = grad.detach().contiguous()
+    (a, b), (c, d) = _span(src), _span(out)
+    if a != c and a < d and c < b:
+        raise ValueError('out overlaps grad and is not grad')
     step = rows * cols * src.element_size()
     ptrs, outs = (ctypes.c_void_p * n)(), (ctypes.c_void_p * n)()
     for i in range(n):
@@ -105,7 +115,7 @@ def muon_step(params, grads, momenta, *, lr, momentum=0.95, nesterov=True, weigh
     params, grads, momenta = list(params), list(grads), list(momenta)
     if not len(params) == len(grads) == len(momenta):
         raise ValueError(f'{len(params)} parameters, {len(grads)} gradients and {len(momenta)} momenta')
-    groups, seen = {}, set()
+    groups, written, read = {}, [], []
     for w, g, m in zip(params, grads, momenta):
         _check_type(w, 'a parameter')
         if w.dim() < 2 or w.numel() == 0:
@@ -116,11 +126,19 @@ def muon_step(params, grads, momenta, *, lr, momentum=0.95, nesterov=True, weigh
             raise ValueError('a momentum must be float32 and have its parameter\'s shape and device')
         if not (w.is_contiguous() and m.is_contiguous()):
             raise ValueError('parameters and momenta must be contiguous')
-        for t in (w, m):
-            if t.data_ptr() in seen:
-                raise ValueError('the same parameter or momentum twice in one step')
-            seen.add(t.data_ptr())
-        groups.setdefault((w.device, w.dtype, w.shape[0], w.numel() // w.shape[0]), []).append((w, g.contiguous(), m))
+        g = g.contiguous()
+        written += _span(w), _span(m)
+        if _span(g) != _span(w):   # a gradient in its own parameter's place has been read when that is written
+            read.append(_span(g))
+        groups.setdefault((w.device, w.dtype, w.shape[0], w.numel() // w.shape[0]), []).append((w, g, m))
+    written.sort()
+    for (_, end), (start, _) in zip(written, written[1:]):
+        if start < end:
+            raise ValueError('the same parameter or momentum twice in one step, or two that overlap')
+    for start, end in read:   # the written spans do not overlap: the last one that starts before `end` decides
+        at = bisect.bisect_left(written, (end,))
+        if at and written[at - 1][1] > start:
+            raise ValueError('a gradient overlaps a parameter or a momentum')
     co = _coefficients(coefficients)
     for (device, dtype, rows, cols), group in groups.items():
         ws, gs, ms = zip(*group)

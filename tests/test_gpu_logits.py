@@ -148,6 +148,49 @@ def test_adjust_backward(rows, cols, history, dtype):
             assert b.grad.shape == b.shape and bool(((b.grad.double().cpu() - wb).abs() <= (rows + 64) * U * size).all())
 
 
+@pytest.mark.parametrize('rows,cols', [(3000, 61), (1500, 1300), (17, 5000)])
+def test_adjust_backward_many_rows(rows, cols):
+    """Several rows a workgroup, without and with a bias they share, and gradients that are broadcast views."""
+    x, legal, _, _ = make(rows, cols, 1, rows, density=0.5)
+    mask = pack(legal).cuda()
+    for dy in (torch.randn(rows, cols, generator=gen(3)), torch.randn(1, cols, generator=gen(4)).expand(rows, cols),
+               torch.ones(1, 1).expand(rows, cols)):
+        for shape in ((cols,), (rows, cols)):
+            z, b = x.cuda().requires_grad_(), torch.zeros(shape, device='cuda', requires_grad=True)
+            ops.adjust_logits(z, mask, b).backward(dy.cuda() if dy.stride(0) else dy[:1].cuda().expand(rows, cols))
+            want = torch.where(legal, dy, 0.0)
+            assert torch.equal(z.grad.cpu(), want)
+            if b.dim() == 2:
+                assert torch.equal(b.grad.cpu(), want)
+            else:
+                size = want.double().abs().sum(0)
+                assert bool(((b.grad.double().cpu() - want.double().sum(0)).abs() <= (rows + 64) * U * size).all())
+
+
+@pytest.mark.parametrize('dtype', DTYPES, ids=str)
+def test_adjust_many_rows_share_bias_and_mask(dtype):
+    rows, cols = 4097, 1100                 # an odd number of rows, two a workgroup
+    x, legal, actions, lengths = make(rows, cols, 20, 6, dtype)
+    bias = torch.randn(cols, generator=gen(2))
+    got = ops.adjust_logits(x.cuda(), pack(legal[:1]).cuda(), bias.cuda(), actions.cuda(), lengths.cuda(), 1.3, 0.25, 0.5).cpu()
+    y, _, size = adjusted(x, legal[:1], bias, counts(actions, lengths, cols), 1.3, 0.25, 0.5)
+    keep = legal[:1].expand(rows, cols)
+    assert bool((got[~keep] == -math.inf).all())
+    err = (got.double() - y).abs()[keep]
+    assert bool((err <= (5 * U * size + HALF[dtype] * y.abs() + 1e-12 + (2.0 ** -25 if dtype == torch.float16 else 0))[keep]).all())
+
+
+def test_columns_of_one_matrix_and_overlaps():
+    both = torch.randn(6, 80, generator=gen(1)).cuda()
+    want = ops.adjust_logits(both[:, :40], bias=both.new_ones(40))
+    ops.adjust_logits(both[:, :40], bias=both.new_ones(40), out=both[:, 40:])
+    assert torch.equal(both[:, 40:], want)
+    with pytest.raises(_lib.MtazError, match='overlaps'):
+        ops.adjust_logits(both[:, :40], out=both[:, 39:79])
+    with pytest.raises(_lib.MtazError, match='overlaps'):
+        ops.adjust_logits(both[:5], out=both[1:])
+
+
 def test_adjust_gradient_against_differences():
     x, legal, actions, lengths = make(3, 40, 10, 2, density=0.6)
     x = x + 0.5 * x.sign()                  # no logit within a step of 0, where the slope jumps

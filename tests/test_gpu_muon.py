@@ -241,3 +241,29 @@ def test_refusals():
         optim.muon_step([g.t()], [g.t()], [m.t()], lr=0.1)
     with pytest.raises(_lib.MtazError, match='momentum'):
         optim.muon_step([g], [g], [m], lr=0.1, momentum=1.0)
+    both = randn(2, 8, 16)
+    flat = both.view(-1)
+    with pytest.raises(ValueError, match='overlaps grad'):
+        optim.orthogonalize(flat[:128].view(8, 16), out=flat[64:192].view(8, 16))
+    with pytest.raises(ValueError, match='overlap'):
+        optim.muon_step([flat[:128].view(8, 16), flat[64:192].view(8, 16)], [g, g], [m, m.clone()], lr=0.1)
+    with pytest.raises(ValueError, match='a gradient overlaps'):
+        optim.muon_step([g], [m], [m], lr=0.1)
+    with pytest.raises(ValueError, match='a gradient overlaps'):
+        optim.muon_step([both[0], both[1]], [both[1], g], [m, m.clone()], lr=0.1)
+
+
+def test_shared_and_own_gradients():
+    """One gradient for two parameters, and a gradient in its own parameter's place."""
+    w, g = randn(2, 20, 60, seed=5), randn(20, 60, seed=6)
+    m = torch.zeros(3, 20, 60, device='cuda')
+    both = [w[0].clone(), w[1].clone()]
+    optim.muon_step(both, [g, g], [m[0], m[1]], lr=0.1)
+    for k in range(2):
+        alone = w[k].clone()
+        optim.muon_step([alone], [g], [torch.zeros_like(g)], lr=0.1)
+        assert torch.equal(alone, both[k])
+    own, want = w[0].clone(), w[0].clone()
+    optim.muon_step([own], [own], [m[2]], lr=0.1)
+    optim.muon_step([want], [w[0]], [torch.zeros_like(g)], lr=0.1)
+    assert torch.equal(own, want)

@@ -95,6 +95,34 @@ def test_loss_grad_refuses():
     assert f(0, 2, 40, 0, 0, P, 40, P, 40, None, 0, None, None, P, P, None, 40, None, None) == 0
 
 
+@pytest.mark.parametrize('x,xs,out,os,rows,why', [
+    (P + 4, 40, P, 40, 2, 'overlaps'), (P, 40, P + 4 * 79, 40, 2, 'overlaps'), (P, 80, P + 4 * 39, 80, 2, 'overlaps'),
+    (P, 80, P + 4 * 41, 80, 2, 'overlaps'), (P, 0, P, 40, 2, 'in place'), (P, 40, P, 41, 2, 'in place'),
+    (P, 41, P, 40, 1 << 25, 'too many rows')])
+def test_overlaps_and_sizes_refused(x, xs, out, os, rows, why):
+    cols = 40 if rows < 1 << 25 else 2049
+    refused(adjust(x=x, xs=xs, out=out, os=max(os, cols), cols=cols, rows=rows, actions=None), why)
+
+
+def test_loss_gradient_over_the_logits_refused():
+    L = _lib.lib()
+
+    def loss(z, zs, grad, gs, dtype=1, target=P + 1600, ttype=1):
+        return L.mtaz_policy_loss(0, 2, 40, dtype, ttype, z, zs, target, 40, None, 0, None, None, P, P + 1024, grad, gs, None, 1.0,
+                                  P, 0, None)
+    refused(loss(P, 40, P + 2, 40), 'workspace')          # the other checks come first
+    for z, zs, grad, gs, ttype in ((P, 40, P + 2, 40, 1), (P, 41, P, 40, 1), (P, 40, P + 1600, 40, 0), (P, 40, P + 1598, 40, 1)):
+        refused(L.mtaz_policy_loss(0, 2, 40, 1, ttype, z, zs, P + 1600, 40, None, 0, None, None, P, P + 1024, grad, gs, None, 1.0,
+                                   P, 256, None), 'not in place')
+
+
+def test_workspace_of_large_matrices_does_not_grow():
+    """Matrices that fill the chip one by one go through the kernels one after the other."""
+    one, many = (_lib.lib().mtaz_orthogonalize_workspace(n, 16384, 16384, 2) for n in (1, 50))
+    assert one == many
+    assert _lib.lib().mtaz_orthogonalize_workspace(64, 4096, 4096, 0) < 3 << 30
+
+
 def test_python_refuses_cpu_tensors():
     g = torch.randn(4, 8)
     for call in (lambda: optim.orthogonalize(g), lambda: optim.muon_step([g], [g], [g.clone()], lr=0.1),
