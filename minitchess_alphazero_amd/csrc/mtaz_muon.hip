@@ -335,61 +335,101 @@ void k_product(Product pr, Out out) {
   };
   const int m0 = part % SIDE * W, n0 = part / SIDE * W;
   const int rounds = pr.k / DEPTH;
-  constexpr int AHEAD = RING - 1;                       // rounds under way while one is multiplied
+  // Where each wave has a tile to itself, a round's operands are read during the products of the round before (2048 x 8192
+  // bf16, five steps: 1311 us, without 1350); with four waves a tile 1024 deep that takes 35 us and without 32.
+  constexpr bool EARLY = !COLS && STEPS == 1 && SIDE == 1;
   f32x16 acc[F][F] = {};
+  struct Operands { f16x8 ah[F], al[F], bh[F], bl[F]; };
+  auto read = [&](int buf, int step, Operands& x) {
+    const _Float16 *p = lds + buf * 2 * HALF, *q = p + HALF;
+    const int kk = (group * STEPS + step) * 16;
+    const int line = kk / 32 * T * 64, piece = kk % 32 / 8 + (lane >> 5);   // rows: block of lines, piece
+#pragma unroll
+    for (int f = 0; f < F; ++f) {
+      const int m = m0 + 32 * f + (lane & 31), n = n0 + 32 * f + (lane & 31);
+      if (!COLS) {
+        x.ah[f] = read_rows(p + line, m, piece);
+        x.al[f] = read_rows(p + line, m, piece + 4);
+      }
+      x.bh[f] = read_rows(q + line, n, piece);
+      x.bl[f] = read_rows(q + line, n, piece + 4);
+    }
+    if constexpr (COLS) read_cols<T, F>(p, m0, kk, lane, x.ah, x.al);
+  };
+  // One step's products.  A round's loads are issued between its products: a wave issues in order, and the address path
+  // takes 1 KiB pieces too slowly to have them ahead of everything.
+  auto multiply = [&](const Operands& x, int step, auto loads, int r, int over) {
+#pragma unroll
+    for (int f = 0; f < F; ++f)
+#pragma unroll
+      for (int g = 0; g < F; ++g) {
+        acc[f][g] = __builtin_amdgcn_mfma_f32_32x32x16_f16(x.al[f], x.bh[g], acc[f][g], 0, 0, 0);
+        acc[f][g] = __builtin_amdgcn_mfma_f32_32x32x16_f16(x.ah[f], x.bl[g], acc[f][g], 0, 0, 0);
+        acc[f][g] = __builtin_amdgcn_mfma_f32_32x32x16_f16(x.ah[f], x.bh[g], acc[f][g], 0, 0, 0);
+        if constexpr (decltype(loads)::value) {
+          constexpr int ALL = STEPS * F * F;
+          const int at = (step * F + f) * F + g;
+#pragma unroll
+          for (int c = at * CH / ALL; c < (at + 1) * CH / ALL; ++c) load(r, over, c);
+          __builtin_amdgcn_sched_barrier(EARLY ? 0 : 0x7);   // these loads stay here; 0x7: arithmetic may pass
+        }
+      }
+  };
+  constexpr int AHEAD = EARLY ? RING : RING - 1;        // rounds under way beside the one that is multiplied
 #pragma unroll
   for (int r = 0; r < AHEAD; ++r)
     if (r < rounds)
 #pragma unroll
       for (int c = 0; c < CH; ++c) load(r, r, c);
-  int buf = 0;
-  // One round's products.  Its loads (of the round AHEAD, over the one read last) are issued between the products:
-  // a wave issues in order, and the address path takes 1 KiB pieces too slowly to have them ahead of everything.
-  auto multiply = [&](int r, auto loads) {
-    const int over = buf == 0 ? RING - 1 : buf - 1;
-    const _Float16 *p = lds + buf * 2 * HALF, *q = p + HALF;
-    buf = buf + 1 == RING ? 0 : buf + 1;
-#pragma unroll
-    for (int step = 0; step < STEPS; ++step) {
-      const int kk = (group * STEPS + step) * 16;
-      const int line = kk / 32 * T * 64, piece = kk % 32 / 8 + (lane >> 5);   // rows: block of lines, piece
-      f16x8 ah[F], al[F], bh[F], bl[F];
-#pragma unroll
-      for (int f = 0; f < F; ++f) {
-        const int m = m0 + 32 * f + (lane & 31), n = n0 + 32 * f + (lane & 31);
-        if (!COLS) {
-          ah[f] = read_rows(p + line, m, piece);
-          al[f] = read_rows(p + line, m, piece + 4);
-        }
-        bh[f] = read_rows(q + line, n, piece);
-        bl[f] = read_rows(q + line, n, piece + 4);
-      }
-      if (COLS) read_cols<T, F>(p, m0, kk, lane, ah, al);
-#pragma unroll
-      for (int f = 0; f < F; ++f)
-#pragma unroll
-        for (int g = 0; g < F; ++g) {
-          acc[f][g] = __builtin_amdgcn_mfma_f32_32x32x16_f16(al[f], bh[g], acc[f][g], 0, 0, 0);
-          acc[f][g] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ah[f], bl[g], acc[f][g], 0, 0, 0);
-          acc[f][g] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ah[f], bh[g], acc[f][g], 0, 0, 0);
-          if constexpr (decltype(loads)::value) {
-            constexpr int ALL = STEPS * F * F;
-            const int at = (step * F + f) * F + g;
-#pragma unroll
-            for (int c = at * CH / ALL; c < (at + 1) * CH / ALL; ++c) load(r + AHEAD, over, c);
-            __builtin_amdgcn_sched_barrier(0x7);        // arithmetic may move, products, loads and LDS reads not
-          }
-        }
+  if constexpr (EARLY) {
+    Operands even, odd;
+    int buf = 0;                                        // of round r, free once everybody has its operands
+    if (rounds >= RING) ready<2 * CH * (RING - 1)>();
+    else ready<0>();
+    read(0, 0, even);
+    auto round = [&](int r, auto loads, const Operands& now, Operands& next) {
+      constexpr bool more = decltype(loads)::value;
+      const int over = buf;
+      buf = buf + 1 == RING ? 0 : buf + 1;
+      ready<more ? 2 * CH * (RING - 2) : 0>();          // round r + 1 is there
+      read(buf, 0, next);                               // (of the last round nothing that is used)
+      __builtin_amdgcn_sched_barrier(0);
+      multiply(now, 0, loads, r + RING, over);
+    };
+    int r = 0;
+    for (; r + RING + 1 < rounds; r += 2) {
+      round(r, Yes{}, even, odd);
+      round(r + 1, Yes{}, odd, even);
     }
-  };
-  int r = 0;
-  for (; r + AHEAD < rounds; ++r) {
-    ready<2 * CH * (AHEAD - 1)>();                      // all rounds loaded so far but the newest AHEAD - 1
-    multiply(r, Yes{});
-  }
-  for (; r < rounds; ++r) {
-    ready<0>();
-    multiply(r, No{});
+    if (r + RING < rounds) {
+      round(r, Yes{}, even, odd);
+      even = odd, ++r;
+    }
+    for (; r < rounds; ++r) {
+      round(r, No{}, even, odd);
+      even = odd;
+    }
+  } else {
+    int buf = 0;
+    auto round = [&](int r, auto loads) {
+      const int over = buf == 0 ? RING - 1 : buf - 1;   // the round read last
+#pragma unroll
+      for (int step = 0; step < STEPS; ++step) {
+        Operands x;
+        read(buf, step, x);
+        multiply(x, step, loads, r + AHEAD, over);
+      }
+      buf = buf + 1 == RING ? 0 : buf + 1;
+    };
+    int r = 0;
+    for (; r + AHEAD < rounds; ++r) {
+      ready<2 * CH * (AHEAD - 1)>();                    // all rounds loaded so far but the newest AHEAD - 1
+      round(r, Yes{});
+    }
+    for (; r < rounds; ++r) {
+      ready<0>();
+      round(r, No{});
+    }
   }
 
   // The sums through LDS as [n][m], so that memory is read and written along rows: a lane holds column n and, four
