@@ -7,7 +7,7 @@
 //   k_loss_mean               the mean of the rows
 //
 // All are bound by memory or, for small calls, by latency: every element is read and written once, 16 bytes at a time
-// and before anything that does not need it, and arithmetic is in float.
+// and before anything that does not need it, and arithmetic is in float.  (A copy of 1 GiB reaches 5.2 TB/s here.)
 #include "ops.h"
 
 #include <math.h>
@@ -163,7 +163,8 @@ __device__ __forceinline__ void adjust(Words<DT, N>& q, const uint32_t* cnt, con
   q.keep(ok, NEVER<DT>);
 }
 
-// Rows of up to WAVE_COLS columns: a wave each, with the counts of its actions in its own piece of LDS.
+// Rows of up to WAVE_COLS columns: a wave each, with the counts of its actions in its own piece of LDS.  4096 x 554 f32
+// with 60 actions a row, mask and bias: 6.7 us (19 MB, 2.9 TB/s, most of it from the caches).
 constexpr int WAVE_COLS = 1024;
 template <int DT>
 __global__ __launch_bounds__(256) void k_adjust_wave(const typename Elem<DT>::T* x, int64_t x_stride,
@@ -248,7 +249,8 @@ __global__ __launch_bounds__(NT) void k_adjust(const typename Elem<DT>::T* x, in
 }
 
 // d x = d y where legal, else 0; gb: the same in float, per row; part: its sums over the columns of the workgroup's rows,
-// for a bias that all rows share.  A workgroup takes `per` rows one after the other.
+// for a bias that all rows share.  A workgroup takes `per` rows one after the other, four of them under way.  1024 x 50021
+// f16 with a shared bias: 51 us (205 MB, 4.0 TB/s).
 template <int DT>
 __global__ __launch_bounds__(NT) void k_adjust_grad(const typename Elem<DT>::T* gy, int64_t gy_stride,
                                                     typename Elem<DT>::T* gx, int64_t gx_stride, float* gb,
@@ -435,7 +437,8 @@ template <int DT, int DP, int THREADS, int REP, bool KEEP = true> struct Held {
   }
 };
 
-// Rows of up to WAVE_COLS columns: a wave each.  ONE: a single workgroup takes all rows and their mean.
+// Rows of up to WAVE_COLS columns: a wave each, and everything stays in its registers.  4096 x 554 f32 with targets:
+// 9 us (18 MB).  ONE: a single workgroup takes all rows and their mean (32 x 554 with the gradient 8.6 us).
 template <int DT, int DP, bool ONE>
 __global__ __launch_bounds__(ONE ? 1024 : 256) void k_loss_wave(const typename Elem<DT>::T* z, int64_t z_stride,
                                                                 const typename Elem<DP>::T* pi, int64_t pi_stride,
@@ -469,7 +472,8 @@ __global__ __launch_bounds__(ONE ? 1024 : 256) void k_loss_wave(const typename E
 
 // Rows that fit into a workgroup's registers: one workgroup each.  With 32 logits a thread and more the exponentials are
 // taken twice; 64 of 16 bits and their targets still leave room for two workgroups of 512 on a CU, so that one loads
-// while the other computes.
+// while the other computes.  2048 x 32003 bf16 with the gradient: 106 us (393 MB, 3.7 TB/s); its 26 operations a logit
+// take 44 us, and two workgroups hide half of them.
 template <int DT, int DP, int THREADS, int REP>
 __global__ __launch_bounds__(THREADS, 4) void k_loss_block(const typename Elem<DT>::T* z, int64_t z_stride,
                                                            const typename Elem<DP>::T* pi, int64_t pi_stride, int cols,
@@ -864,8 +868,9 @@ extern "C" int mtaz_policy_loss(int device, int64_t rows, int64_t cols, int dtyp
   const int nc = (int)cols;
   const Legal legal{d_legal, legal_stride};
   const float k = (float)(scale / (double)rows);
-  // A handful of short rows: one launch, mean included.
-  const bool one = cols <= WAVE_COLS && rows <= 64;
+  // A handful of short rows: one launch, mean included, which saves the host 4 us.  On the GPU it takes with 16, 32 and 64
+  // rows of 554 4.9, 7.4 and 12.9 us, the two launches 6.0 each time.
+  const bool one = cols <= WAVE_COLS && rows <= 32;
   FOR_TYPES(dtype, target_dtype, {
     const auto* z = (const Elem<DT>::T*)d_logits;
     const auto* pi = (const Elem<DP>::T*)d_target;

@@ -14,6 +14,15 @@
 // halves of 32 consecutive elements, so that one line is what a product reads of a row at a time.  They are padded
 // with zeros to whole tiles, so that the product kernel checks no bounds; a padded row or column stays zero through
 // every step.
+//
+// The products bound the large matrices: 1140 / 3 = 380 TFLOP/s at the rate that a large f16 product of the library
+// reaches here, counting a symmetric product once.  2048 x 8192 bf16 with five steps takes 1311 us (404 GFLOP: 308),
+// 18 x 256 x 2304 f32 270 us (35 GFLOP: 130; its products are 256 deep or 2304 long and wait for memory and for each
+// other), and a matrix that fits into one CU's LDS is bound by the latency of its 15 products (554 x 61: 50 us).
+//
+// One factor of f16 alone would take a third of the products, and be off by 2^-12 in every X, S and B: a gradient with
+// few strong directions has its weak ones, noise included, made up to 3.4 times larger a step, and five steps turn that
+// into several per cent of the result.  So 16-bit matrices are computed like 32-bit ones, and rounded once.
 #include "ops.h"
 
 #include <math.h>
@@ -67,7 +76,8 @@ __device__ __forceinline__ float update_of(float g, float m, const Update& u) {
 }
 
 // Partial sums of squares in 64 bits: neither large nor tiny gradients leave the range.  With momentum, the
-// pass also brings it up to date.
+// pass also brings it up to date.  Bound by memory: 18 x 256 x 2304 f32 8.4 us (42 MB, 5.0 TB/s), with momentum 22 us
+// (127 MB, 5.8 TB/s).
 template <int DT, bool MUON>
 __global__ __launch_bounds__(NT) void k_squares(Matrices ms, int64_t count, Update u, double* part) {
   const int parts = gridDim.x;
@@ -126,7 +136,8 @@ __device__ __forceinline__ void store_pairs(_Float16* to, const float* x) {
   *reinterpret_cast<f16x8*>(to + 32) = l;
 }
 
-// X = matrix * 2^e / (norm + eps) in pairs, transposed where the matrix is tall; 64 x 64 elements per workgroup
+// X = matrix * 2^e / (norm + eps) in pairs, transposed where the matrix is tall; 64 x 64 elements per workgroup, through
+// LDS, since either side may run along memory.  18 x 256 x 2304 f32: 21 us (85 MB, 4.0 TB/s).
 template <int DT, bool MUON>
 __global__ __launch_bounds__(NT) void k_pairs(Matrices ms, Shape sh, Update u, const double* part, double eps,
                                                double unit, Pairs X) {
@@ -172,6 +183,11 @@ __global__ __launch_bounds__(NT) void k_pairs(Matrices ms, Shape sh, Update u, c
 // A round is DEPTH elements deep.  It goes straight from memory into LDS, in a ring of RING rounds: all but one are
 // under way while one is multiplied, and a round costs one barrier.  SIDE x SIDE waves share the tile, GROUPS such
 // sets share the depth of a round, and their sums are added at the end in a fixed order.
+//
+// APPLY of 2048 x 8192 (128-tiles, two workgroups a CU): 200 us, 1030 TFLOP/s of f16 products against the library's 1140
+// for one large product; the matrix cores are busy two thirds of the time, at the clock that the power limit leaves.
+// GRAM 2048 x 2048 x 8192 (96-tiles, half the square): 118 us, 970 TFLOP/s.  Small ones are bound by what a launch costs
+// besides, about 6 us for the first loads, the sums through LDS and the stores: 18 x 256 x 256 x 256 takes 7.5 us.
 enum Kind { GRAM, POLY, APPLY, LAST_OUT, LAST_MUON };
 
 struct Product {
@@ -509,7 +525,8 @@ void k_product(Product pr, Out out) {
 // [r16][pitch], S and then B as [r16][pitch_s]; the 16-byte piece p of row m is at p ^ (m >> 1 & 7), and the pitches are
 // odd multiples of 128 bytes where there is room, so that the 16 rows of an operand lie in different banks.  Products
 // are 16 x 16 x 32: a wave takes whole tiles of S and B (on and below the diagonal, written twice) and whole strips of
-// 16 columns of X, which it reads before it overwrites them.
+// 16 columns of X, which it reads before it overwrites them.  554 x 61 f32 takes 50 us, 8 a step, where the general
+// kernels' 17 launches take 86; above SMALL_ROWS and where X does not fit those are taken.
 constexpr int SMALL_WAVES = 16;
 constexpr int SMALL_LDS = 160 * 1024;
 constexpr int SMALL_ROWS = 128;                         // r at most: three tiles of S a wave
@@ -799,10 +816,11 @@ Work layout(int n, const Shape& sh, char* base) {
   return w;
 }
 
-// Tiles over r x L: 128 where the matrices have enough of them to occupy half of the 256 CUs, else 64.  Over r x r, on
+// Tiles over r x L: 128 where the matrices have enough of them to occupy half of the 256 CUs, else 64 (B X of 18 x 256 x
+// 2304, 648 tiles of 128: 27.7 us, of 64 36.0; of 3 x 512 x 1021, 96 tiles of 128: 14.8, of 64 11.3).  Over r x r, on
 // and below the diagonal: the size that takes the fewest rounds of 256, each in proportion to its area; a tile of 64
 // reads twice as much a product as one of 128 and counts for a third more.  (2048 x 2048: 136 tiles of 128 leave half
-// of the chip without work and take 47 us a square; 253 of 96 fill it.)
+// of the chip without work and take 47 us a square; 253 of 96 fill it and take 36.)
 Shape shape_of(int n, int64_t rows, int64_t cols) {
   Shape s;
   s.rows = (int)rows, s.cols = (int)cols;
@@ -881,7 +899,8 @@ bool small(const Shape& sh, Small& sm) {
 }
 
 // Up to one tile a CU: the whole LDS for the ring, and waves that share the depth, so that each SIMD has work while
-// another wave waits.  More tiles: two workgroups a CU.
+// another wave waits (216 tiles of 128, 1024 deep: 34 us, in the other form 40; 180 of 64, 2304 deep: 20 and 27).  More tiles: two workgroups a CU, of which
+// one multiplies while the other begins or ends.
 template <int KIND, int DT, typename Out>
 void product(Product pr, int T, const Out& out, hipStream_t s) {
   const unsigned grid = (unsigned)(pr.tiles * pr.n);
