@@ -948,14 +948,15 @@ void iterate(const Matrices& ms, int n, const Shape& sh, const Update& u, int st
                              (float)ldexp(co[1], e.b[t] - e.s[t]), (float)ldexp(co[0], e.b[t])}, sh.tile_r, Stay{}, s);
   };
   // Two steps in one where the long side is long against the short one: with M = a I + b S + c S S the second step's S
-  // is M S M, and X <- M' M X; three products r x r more, and one product over the long side and one with X less.
-  // S loses accuracy by that in its small eigenvalues, a^2 = 12 times the rounding of its large ones: not visible
-  // where the result is rounded to 16 bits, and in 32 bits not when it is done for the first two steps alone
-  // (256 x 2304 Gaussian against 64 bits: 2.2e-6 either way, 3.8e-6 when the next two are joined as well).
+  // is M S M, and X <- M' M X; three products r x r more, and one product over the long side and one with X less
+  // (2048 x 8192 bf16 1902 us without, 1577 with it).  S loses accuracy by that in its small eigenvalues, a^2 = 12 times
+  // the rounding of its large ones: not visible where the result is rounded to 16 bits, and in 32 bits not when it is
+  // done for the first two steps alone and r is not small (against 64 bits, 256 x 2304 Gaussian: 2.2e-6 either way, 3.8e-6
+  // when the next two are joined as well; 64 x 5000 of falling spectrum 8e-7 either way, 15 x 5000 4e-7 and 9e-7).
   const bool joinable = sh.L >= 3 * sh.r || (sh.r >= 768 && 2 * sh.L >= 3 * sh.r);
   int now = 0;
   for (int t = 0; t < steps;) {
-    const bool join = joinable && t + 1 < steps && (DT != MTAZ_F32 || t == 0);
+    const bool join = joinable && t + 1 < steps && (DT != MTAZ_F32 || (t == 0 && sh.r >= 64));
     const Pairs &X = w.X[now], &Y = w.X[now ^ 1];
     gram(X, X, w.S, sh.Lp, e.s[t] - 2 * e.x[t]);
     poly(w.S, w.B, t);

@@ -60,6 +60,24 @@ def test_square_small_and_odd(shape):
     assert off(optim.orthogonalize(g), reference(g)) <= LOOSE
 
 
+@pytest.mark.parametrize('shape', [(4133, 15), (5, 9000), (64, 3000), (150, 1100)], ids=str)
+def test_long_sides_keep_32_bits(shape):
+    """A few strong directions and noise: within twice of what the same steps in float give (sums of r and L terms,
+    errors of both sides alike in kind)."""
+    g = randn(*shape, seed=sum(shape)).cpu()
+    u = randn(shape[0], 1, seed=1).cpu() @ randn(1, shape[1], seed=2).cpu()
+    g = (u + 0.3 * g).cuda()
+    want = reference(g)
+    x = g.cpu() / g.cpu().norm()
+    x = x.mT if shape[0] > shape[1] else x
+    a, b, c = optim.COEFFICIENTS
+    for _ in range(5):
+        s = x @ x.mT
+        x = a * x + (b * s + c * (s @ s)) @ x
+    plain = off(x.mT if shape[0] > shape[1] else x, want)
+    assert off(optim.orthogonalize(g), want) <= 2 * plain
+
+
 @pytest.mark.parametrize('shape', [(96, 400), (700, 90)], ids=str)
 def test_low_rank(shape):
     g = randn(shape[0], 5, seed=1) @ randn(5, shape[1], seed=2) + 1e-2 * randn(*shape, seed=4)
