@@ -7,6 +7,8 @@ Layout:
   engine.py        batched self-play engine (one per GPU)
   environment.py   drop-in exp/environment.py (rules in libmtaz)
   network.py       drop-in exp/policy.py Network (weights container)
+  optim.py         orthogonalisation and the Muon optimizer (HIP kernels)
+  logits.py        penalties, bias and legal masks on logits; the policy/value loss (HIP kernels)
   agent.py, policy.py, callbacks.py, erlyx_compat.py, puppet.py
                    the reference's plugin surface and the app/puppet entry point
 """

@@ -8,7 +8,8 @@
 A mask is packed 32 actions a word: action v is legal where bit v & 31 of word v >> 5 is set, int32
 [rows, ceil(cols / 32)], or [1, words] / [words] for one mask that all rows share.  Logits are float32,
 float16 or bfloat16, sums are float32, and the operators enqueue on the current stream without a
-synchronization; they may be captured in a HIP graph.  There is no CPU form: tensors elsewhere are refused.
+synchronization; they may be captured in a HIP graph (a backward pass like any of torch's: with no eager graph of the
+same leaves alive).  There is no CPU form: tensors elsewhere are refused.
 """
 import torch
 from torch.autograd.function import once_differentiable
