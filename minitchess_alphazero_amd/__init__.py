@@ -2,7 +2,8 @@
 reference's exp/agent.py + exp/environment.py + exp/policy.py hot path).
 
 Layout:
-  csrc/            HIP kernels (gfx950) + C ABI (include/mtaz.h) -> libmtaz.so
+  csrc/            HIP kernels (gfx950) + C ABI (include/mtaz.h) -> libmtaz.so;
+                   autograd nodes over it -> libmtaz_autograd.so
   _lib.py          ctypes binding (fails loudly when the HIP library is missing)
   engine.py        batched self-play engine (one per GPU)
   environment.py   drop-in exp/environment.py (rules in libmtaz)

@@ -150,6 +150,28 @@ def lib():
     return L
 
 
+_NODES = None
+
+
+def nodes():
+    """The operators that are nodes of torch's autograd graph (libmtaz_autograd.so, over libmtaz.so), loaded once."""
+    global _NODES
+    if _NODES is not None:
+        return _NODES
+    lib()
+    import torch
+    from . import build as _build
+    try:
+        torch.ops.load_library(_build.OUT_AUTOGRAD)
+    except OSError as e:
+        raise MtazLibraryError(f'cannot load {_build.OUT_AUTOGRAD}: {e}: run `python -m minitchess_alphazero_amd.build`') from e
+    if os.path.isdir(_build.CSRC) and not torch.ops.mtaz.built_from().endswith('=' + _build.autograd_hash()):
+        raise MtazLibraryError(f'{_build.OUT_AUTOGRAD} was not built from this tree and this torch: run '
+                               '`python -m minitchess_alphazero_amd.build`')
+    _NODES = torch.ops.mtaz
+    return _NODES
+
+
 def check_fingerprint(version):
     """The library must be built from the sources next to it (build.py source_hash, compiled into
     mtaz_version()); raises MtazLibraryError otherwise.  Skipped only where no sources exist."""

@@ -3,8 +3,9 @@
 Translation units: csrc/mtaz_device.hip (tree kernels + launchers), csrc/mtaz_net16.hip and
 csrc/mtaz_net8.hip (network kernels k_net_y, k_net_z), csrc/mtaz_host.cpp (C ABI, numpy-legacy
 RNG compiled with -ffp-contract=off, engine driver), csrc/mtaz_wire.cpp (episode wire
-format), csrc/mtaz_muon.hip and csrc/mtaz_logits.hip (the learner's operators).  The shared object lands next to this file so it travels to the GPU box with the repo
-snapshot.  build(diag=True) makes libmtaz_diag.so with -DMTAZ_NET_DIAG: the network kernels'
+format), csrc/mtaz_muon.hip and csrc/mtaz_logits.hip (the learner's operators).  The shared object
+lands next to this file.  libmtaz_autograd.so (csrc/mtaz_autograd.cpp, host code against torch's headers)
+makes the logits operators nodes of torch's autograd graph.  build(diag=True) makes libmtaz_diag.so with -DMTAZ_NET_DIAG: the network kernels'
 A/B and timing-only variants and round 3's k_net_y (csrc/mtaz_net16_r3.hip, variant 3; the
 round-3 comparison tests load it in a child process), never loaded by the product path.
 
@@ -14,6 +15,7 @@ build() rebuilds whenever the library does not carry the tree's hash (content, n
 _lib.lib() refuses a library whose hash differs from the sources next to it.
 """
 import hashlib
+import importlib.util
 import os
 import subprocess
 import sys
@@ -21,6 +23,7 @@ import sys
 HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, 'csrc')
 OUT = os.path.join(HERE, 'libmtaz.so')
+OUT_AUTOGRAD = os.path.join(HERE, 'libmtaz_autograd.so')
 BUILD = os.path.join(HERE, '_build')
 OUT_DIAG = os.path.join(HERE, 'libmtaz_diag.so')
 BUILD_DIAG = os.path.join(HERE, '_build_diag')
@@ -94,15 +97,46 @@ def _tu_key(src, cmd):
     return h.hexdigest()
 
 
-def embedded_hash(path):
+def _torch_dir():
+    return list(importlib.util.find_spec('torch').submodule_search_locations)[0]
+
+
+def autograd_hash():
+    """sha256 over what libmtaz_autograd.so is built from: its source, include/mtaz.h and torch's version."""
+    h = hashlib.sha256()
+    for path in (os.path.join(CSRC, 'mtaz_autograd.cpp'), os.path.join(INCLUDE, 'mtaz.h'),
+                 os.path.join(_torch_dir(), 'version.py')):
+        with open(path, 'rb') as f:
+            h.update(f.read() + b'\0')
+    return h.hexdigest()
+
+
+def build_autograd(force=False, verbose=True):
+    if not force and embedded_hash(OUT_AUTOGRAD, b'mtaz-autograd-sha256=') == autograd_hash():
+        return OUT_AUTOGRAD
+    torch_dir, tmp = _torch_dir(), OUT_AUTOGRAD + '.tmp'
+    cmd = ['g++', '-shared', '-fPIC', '-std=c++17', '-O2', '-Wall',
+           f'-DMTAZ_AUTOGRAD_SHA256="mtaz-autograd-sha256={autograd_hash()}"', f'-I{INCLUDE}',
+           '-isystem', os.path.join(torch_dir, 'include'),
+           '-isystem', os.path.join(torch_dir, 'include', 'torch', 'csrc', 'api', 'include'),
+           os.path.join(CSRC, 'mtaz_autograd.cpp'), '-o', tmp, '-L' + os.path.join(torch_dir, 'lib'), '-ltorch',
+           '-ltorch_cpu', '-lc10', '-L' + HERE, '-lmtaz', '-Wl,-rpath,$ORIGIN']
+    if verbose:
+        print(' '.join(cmd), flush=True)
+    subprocess.check_call(cmd)
+    os.replace(tmp, OUT_AUTOGRAD)
+    return OUT_AUTOGRAD
+
+
+def embedded_hash(path, mark=b'mtaz-src-sha256='):
     """The src=<hash> a built library carries (None if absent)."""
     try:
         with open(path, 'rb') as f:
             data = f.read()
     except OSError:
         return None
-    i = data.find(b'mtaz-src-sha256=')
-    return data[i + 16:i + 80].decode('ascii', 'replace') if i >= 0 else None
+    i = data.find(mark)
+    return data[i + len(mark):i + len(mark) + 64].decode('ascii', 'replace') if i >= 0 else None
 
 
 def _stale(out):
@@ -112,6 +146,8 @@ def _stale(out):
 def build(force=False, verbose=True, diag=False):
     out, bdir = (OUT_DIAG, BUILD_DIAG) if diag else (OUT, BUILD)
     if not force and not _stale(out):
+        if not diag:
+            build_autograd(verbose=verbose)
         return out
     os.makedirs(bdir, exist_ok=True)
     hipcc = _hipcc()
@@ -150,6 +186,8 @@ def build(force=False, verbose=True, diag=False):
         print(' '.join(cmd), flush=True)
     subprocess.check_call(cmd)
     os.replace(tmp, out)
+    if not diag:
+        build_autograd(force, verbose)
     return out
 
 

@@ -12,7 +12,6 @@ synchronization; they may be captured in a HIP graph (a backward pass like any o
 same leaves alive).  There is no CPU form: tensors elsewhere are refused.
 """
 import torch
-from torch.autograd.function import once_differentiable
 
 from . import _lib
 from .environment import MOVE_CAP, RULES_FLAGS
@@ -83,7 +82,7 @@ def legal_masks(positions, device, rules_flags=RULES_FLAGS, move_cap=MOVE_CAP):
 # ---- penalties, bias and mask ----------------------------------------------------------------------------
 class _Taken:
     """The actions taken and their penalties, as the C entries take them (args); keep: the tensors behind them."""
-    __slots__ = ('args', 'keep', 'bends')
+    __slots__ = ('args', 'keep', 'host', 'bends')
 
     def __init__(self, logits, actions, lengths, repetition, frequency, presence):
         rows = logits.shape[0]
@@ -95,11 +94,12 @@ class _Taken:
             if t.requires_grad and torch.is_grad_enabled():
                 raise ValueError('penalties have no gradient')
         if tensors:
-            host = None
+            host, self.host = None, (1.0, 0.0, 0.0)
             if not isinstance(repetition, torch.Tensor) and not repetition > 0:
                 raise ValueError(f'repetition must be positive, got {repetition}')
         else:
-            host = _doubles(float(repetition), float(frequency), float(presence))
+            self.host = (float(repetition), float(frequency), float(presence))
+            host = _doubles(*self.host)
             if not repetition > 0:
                 raise ValueError(f'repetition must be positive, got {repetition}')
         self.bends = (isinstance(repetition, torch.Tensor) or repetition != 1.0)   # slope not 1
@@ -131,40 +131,6 @@ def _adjust(x, legal, bias, taken, out):
     return out
 
 
-class _Adjust(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, logits, bias, legal, taken):
-        ctx.taken, ctx.dtype = taken, logits.dtype
-        ctx.bias_shape = None if bias is None else bias.shape
-        actions, lengths, _ = taken.keep
-        ctx.save_for_backward(logits if taken.bends else None, legal, actions, lengths)
-        return _adjust(logits, legal, bias, taken, _fresh(logits))
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, grad):
-        x, legal, _, _ = ctx.saved_tensors   # raises where one of them was changed in between
-        g, x, legal = _unit(grad), _unit(x), _unit(legal)
-        rows, cols = g.shape
-        dx = db = work = None
-        size = 0
-        shared = False
-        if ctx.needs_input_grad[0]:
-            dx = _fresh(g)
-        if ctx.needs_input_grad[1]:
-            db = torch.empty(ctx.bias_shape, dtype=torch.float32, device=g.device)
-            shared = len(ctx.bias_shape) == 1 or ctx.bias_shape[0] == 1
-            if shared:
-                size = _lib.check(_lib.lib().mtaz_adjust_logits_grad_workspace(rows, cols))
-                work = torch.empty(max(size, 1), dtype=torch.uint8, device=g.device)
-        taken = ctx.taken.args if x is not None else (None, 0, 0, None, None, None)   # else the slope is 1 everywhere
-        _lib.check(_lib.lib().mtaz_adjust_logits_grad(
-            g.device.index, rows, cols, TYPES[ctx.dtype], g.data_ptr(), g.stride(0), _ptr(x),
-            0 if x is None else x.stride(0), _ptr(dx), cols, _ptr(db), 0 if shared else cols, _ptr(legal),
-            _row_stride(legal), *taken, _ptr(work), size, _stream(g.device)))
-        return dx, db, None, None
-
-
 def adjust_logits(logits, legal=None, bias=None, actions=None, lengths=None, repetition=1.0, frequency=0.0,
                   presence=0.0, out=None):
     """Logits a policy is to answer with.  With c = how often the row has taken action v:
@@ -186,7 +152,8 @@ def adjust_logits(logits, legal=None, bias=None, actions=None, lengths=None, rep
     if torch.is_grad_enabled() and (logits.requires_grad or (bias is not None and bias.requires_grad)):
         if out is not None:
             raise ValueError('out is not supported where a gradient is required')
-        return _Adjust.apply(logits, bias, legal, taken)
+        return _lib.nodes().adjust_logits.default(logits, bias, legal, *taken.keep, *taken.host, taken.bends,
+                                                  _stream(logits.device))
     if out is None:
         return _adjust(logits, legal, bias, taken, _fresh(logits))
     if out.shape != logits.shape or out.dtype != logits.dtype or out.device != logits.device:
@@ -237,32 +204,6 @@ def _loss(logits, target, value, reward, legal, grad, value_grad, scale):
     return loss, stats
 
 
-class _PolicyValueLoss(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, logits, value, target, reward, legal):
-        loss, stats = _loss(logits, target, value, reward, legal, None, None, 1.0)
-        ctx.save_for_backward(logits, value, target, reward, legal, stats)
-        return loss
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, grad):
-        logits, value, target, reward, legal, stats = ctx.saved_tensors
-        z, t, legal = _unit(logits), _unit(target), _unit(legal)
-        rows, cols = z.shape
-        dz = _fresh(z) if ctx.needs_input_grad[0] else None
-        dv = None
-        if value is not None:
-            value, reward = value.contiguous(), reward.contiguous()
-            if ctx.needs_input_grad[1]:
-                dv = torch.empty_like(value)
-        _lib.check(_lib.lib().mtaz_policy_loss_grad(
-            z.device.index, rows, cols, TYPES[z.dtype], TYPES[t.dtype], z.data_ptr(), z.stride(0), t.data_ptr(),
-            t.stride(0), _ptr(legal), _row_stride(legal), _ptr(value), _ptr(reward), stats.data_ptr(), grad.data_ptr(),
-            _ptr(dz), cols, _ptr(dv), _stream(z.device)))
-        return dz, dv, None, None, None
-
-
 def policy_value_loss(logits, target, value=None, reward=None, legal=None):
     """The mean over the rows of (value - reward)^2 - sum over the legal v of target_v log softmax(logits)_v
     (exp/learner.py:86-87, where every action counts as legal), a float32 scalar.
@@ -273,7 +214,7 @@ def policy_value_loss(logits, target, value=None, reward=None, legal=None):
     alone.  Differentiable in logits and value."""
     _check_loss(logits, target, value, reward, legal)
     if torch.is_grad_enabled() and (logits.requires_grad or (value is not None and value.requires_grad)):
-        return _PolicyValueLoss.apply(logits, value, target, reward, legal)
+        return _lib.nodes().policy_loss.default(logits, value, target, reward, legal, _stream(logits.device))
     return _loss(logits, target, value, reward, legal, None, None, 1.0)[0]
 
 

@@ -410,3 +410,21 @@ def test_refusals():
     with pytest.raises(RuntimeError, match='modified by an inplace operation'):
         loss.backward()
     assert _lib.lib().mtaz_policy_loss_workspace(-1, 5) < 0
+
+
+def test_gradients_are_not_differentiated_again():
+    x = torch.randn(3, 40, generator=gen(1)).cuda().requires_grad_()
+    b = torch.zeros(40, device='cuda', requires_grad=True)
+    t = torch.softmax(x.detach(), 1)
+    for y in (ops.adjust_logits(x, bias=b).square().sum(), ops.policy_value_loss(x + b, t)):
+        dx, db = torch.autograd.grad(y, (x, b), create_graph=True)
+        with pytest.raises(RuntimeError, match='twice'):
+            (dx.sum() + db.sum()).backward()
+    only = torch.autograd.grad(ops.adjust_logits(x.detach(), bias=b).sum(), b)[0]     # one of the two wanted
+    assert torch.equal(only, torch.full_like(b, 3.0))
+    v = torch.ones(3, 1, device='cuda', requires_grad=True)
+    dv, = torch.autograd.grad(ops.policy_value_loss(x.detach(), t, v, torch.zeros_like(v)), v)
+    assert bool(((dv - 2 / 3).abs() <= 4 * U).all())
+    assert not ops.policy_value_loss(x.detach(), t).requires_grad
+    with torch.no_grad():
+        assert not ops.policy_value_loss(x, t).requires_grad and not ops.adjust_logits(x).requires_grad
