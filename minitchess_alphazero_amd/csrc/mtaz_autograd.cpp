@@ -1,7 +1,8 @@
-// The logits operators as nodes of torch's autograd graph, over the C entries of libmtaz.so.
+// The logits operators for torch, over the C entries of libmtaz.so: nodes of its autograd graph where a gradient is
+// required, plain calls elsewhere.
 //
 // A node written in Python has the engine's own thread wait for the interpreter: forward and backward of a loss of 64 x
-// 554 took the host 105 us that way and takes 72 here.
+// 554 took the host 105 us that way and takes 72 here.  A call without gradients costs it 3 us less than through ctypes.
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/library.h>
@@ -48,18 +49,37 @@ variable_list once(variable_list grads) {
   return grads;
 }
 
+// The loss and the rows' statistics; with gradients of scale * loss where dz or dv is defined.
+std::pair<Tensor, Tensor> loss_of(const Tensor& logits, const Tensor& value, const Tensor& target, const Tensor& reward,
+                                  const Tensor& legal, const Tensor& dz, const Tensor& dv, double scale, int64_t stream) {
+  const Tensor z = unit(logits), t = unit(target), mask = unit(legal), v = dense(value), r = dense(reward);
+  const int64_t rows = z.size(0), cols = z.size(1), work = checked(mtaz_policy_loss_workspace(rows, cols));
+  const auto floats = z.options().dtype(at::kFloat);
+  Tensor loss = at::empty({}, floats), stats = at::empty({4 * rows + work / 4}, floats);   // scratch memory behind them
+  float* const s = (float*)stats.data_ptr();
+  checked(mtaz_policy_loss(z.get_device(), rows, cols, type_of(z), type_of(t), at(z), z.stride(0), at(t), t.stride(0),
+                           (const uint32_t*)at(mask), row_stride(mask), (const float*)at(v), (const float*)at(r),
+                           (float*)at(loss), s, at(dz), cols, (float*)at(dv), scale, s + 4 * rows, work, (void*)stream));
+  return {loss, stats};
+}
+Tensor adjusted(const Tensor& logits, const Tensor& bias, const Tensor& legal, const Tensor& a, const Tensor& n,
+                const Tensor& p, const double* penalties, int64_t stream) {
+  const Tensor x = unit(logits), b = unit(bias), mask = unit(legal), y = fresh(x);
+  checked(mtaz_adjust_logits(x.get_device(), x.size(0), x.size(1), type_of(x), at(x), x.stride(0), at(y), x.size(1),
+                             (const uint32_t*)at(mask), row_stride(mask), (const float*)at(b), row_stride(b),
+                             (const int32_t*)at(a), a.defined() ? a.stride(0) : 0, a.defined() ? (int)a.size(1) : 0,
+                             (const int32_t*)at(n), penalties, (const float*)at(p), (void*)stream));
+  return y;
+}
+bool wanted(const Tensor& a, const MaybeTensor& b) {
+  return at::GradMode::is_enabled() && (a.requires_grad() || (b && b->defined() && b->requires_grad()));
+}
+
 struct PolicyLoss : torch::autograd::Function<PolicyLoss> {
   static Tensor forward(AutogradContext* ctx, const Tensor& logits, const MaybeTensor& value, const Tensor& target,
                         const MaybeTensor& reward, const MaybeTensor& legal, int64_t stream) {
-    const Tensor z = unit(logits), t = unit(target), mask = unit(or_none(legal)), v = dense(or_none(value)),
-                 r = dense(or_none(reward));
-    const int64_t rows = z.size(0), cols = z.size(1), work = checked(mtaz_policy_loss_workspace(rows, cols));
-    const auto floats = z.options().dtype(at::kFloat);
-    Tensor loss = at::empty({}, floats), stats = at::empty({4 * rows + work / 4}, floats);   // scratch memory behind them
-    float* const s = (float*)stats.data_ptr();
-    checked(mtaz_policy_loss(z.get_device(), rows, cols, type_of(z), type_of(t), at(z), z.stride(0), at(t), t.stride(0),
-                             (const uint32_t*)at(mask), row_stride(mask), (const float*)at(v), (const float*)at(r),
-                             (float*)at(loss), s, nullptr, cols, nullptr, 1., s + 4 * rows, work, (void*)stream));
+    const auto [loss, stats] = loss_of(logits, or_none(value), target, or_none(reward), or_none(legal), Tensor(), Tensor(), 1.,
+                                       stream);
     ctx->save_for_backward({logits, or_none(value), target, or_none(reward), or_none(legal), stats});
     ctx->saved_data["stream"] = stream;
     return loss;
@@ -86,21 +106,16 @@ struct AdjustLogits : torch::autograd::Function<AdjustLogits> {
   static Tensor forward(AutogradContext* ctx, const Tensor& logits, const MaybeTensor& bias, const MaybeTensor& legal,
                         const MaybeTensor& actions, const MaybeTensor& lengths, const MaybeTensor& per_row,
                         double repetition, double frequency, double presence, bool bends, int64_t stream) {
-    const Tensor x = unit(logits), b = unit(or_none(bias)), mask = unit(or_none(legal)), a = or_none(actions),
-                 n = or_none(lengths), p = or_none(per_row);
+    const Tensor a = or_none(actions), n = or_none(lengths), p = or_none(per_row);
     const double penalties[3] = {repetition, frequency, presence};
-    const Tensor y = fresh(x);
-    checked(mtaz_adjust_logits(x.get_device(), x.size(0), x.size(1), type_of(x), at(x), x.stride(0), at(y), x.size(1),
-                               (const uint32_t*)at(mask), row_stride(mask), (const float*)at(b), row_stride(b),
-                               (const int32_t*)at(a), a.defined() ? a.stride(0) : 0, a.defined() ? (int)a.size(1) : 0,
-                               (const int32_t*)at(n), penalties, (const float*)at(p), (void*)stream));
+    const Tensor y = adjusted(logits, or_none(bias), or_none(legal), a, n, p, penalties, stream);
     // where the penalties do not bend the logits their gradient is 1, and neither these nor the actions are needed
     ctx->save_for_backward(bends ? variable_list{logits, or_none(legal), a, n, p}
                                  : variable_list{Tensor(), or_none(legal), Tensor(), Tensor(), Tensor()});
     ctx->saved_data["stream"] = stream;
-    ctx->saved_data["type"] = (int64_t)type_of(x);
+    ctx->saved_data["type"] = (int64_t)type_of(logits);
     ctx->saved_data["repetition"] = repetition;
-    if (b.defined()) ctx->saved_data["bias"] = b.sizes().vec();
+    if (bias && bias->defined()) ctx->saved_data["bias"] = bias->sizes().vec();
     return y;
   }
   static variable_list backward(AutogradContext* ctx, const variable_list& grads) {
@@ -137,11 +152,24 @@ struct AdjustLogits : torch::autograd::Function<AdjustLogits> {
 
 Tensor policy_loss(const Tensor& logits, const MaybeTensor& value, const Tensor& target, const MaybeTensor& reward,
                    const MaybeTensor& legal, int64_t stream) {
-  return PolicyLoss::apply(logits, value, target, reward, legal, stream);
+  if (wanted(logits, value)) return PolicyLoss::apply(logits, value, target, reward, legal, stream);
+  return loss_of(logits, or_none(value), target, or_none(reward), or_none(legal), Tensor(), Tensor(), 1., stream).first;
+}
+std::tuple<Tensor, Tensor, Tensor> policy_loss_grad(const Tensor& logits, const MaybeTensor& value, const Tensor& target,
+                                                    const MaybeTensor& reward, const MaybeTensor& legal, double scale,
+                                                    int64_t stream) {
+  const at::NoGradGuard off;
+  const Tensor v = or_none(value), dz = fresh(logits), dv = v.defined() ? fresh(v) : Tensor();
+  return {loss_of(logits, v, target, or_none(reward), or_none(legal), dz, dv, scale, stream).first, dz, dv};
 }
 Tensor adjust_logits(const Tensor& logits, const MaybeTensor& bias, const MaybeTensor& legal, const MaybeTensor& actions,
                      const MaybeTensor& lengths, const MaybeTensor& per_row, double repetition, double frequency,
                      double presence, bool bends, int64_t stream) {
+  if (!wanted(logits, bias)) {
+    const double penalties[3] = {repetition, frequency, presence};
+    return adjusted(logits, or_none(bias), or_none(legal), or_none(actions), or_none(lengths), or_none(per_row), penalties,
+                    stream);
+  }
   return AdjustLogits::apply(logits, bias, legal, actions, lengths, per_row, repetition, frequency, presence, bends, stream);
 }
 std::string built_from() { return MTAZ_AUTOGRAD_SHA256; }
@@ -150,6 +178,7 @@ std::string built_from() { return MTAZ_AUTOGRAD_SHA256; }
 
 TORCH_LIBRARY(mtaz, m) {
   m.def("policy_loss", &policy_loss);
+  m.def("policy_loss_grad", &policy_loss_grad);
   m.def("adjust_logits", &adjust_logits);
   m.def("built_from", &built_from);
 }

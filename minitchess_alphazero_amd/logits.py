@@ -41,8 +41,15 @@ def _check_rows(t, what, like, shapes, dtypes):
         raise ValueError(f'{what} has shape {tuple(t.shape)}, expected {" or ".join(str(s) for s in shapes)}')
 
 
-def _fresh(like):
-    return torch.empty_like(like) if like.is_contiguous() else torch.empty(like.shape, dtype=like.dtype, device=like.device)
+def _call(op, *args):
+    try:
+        return op(*args)
+    except RuntimeError as e:
+        text = str(e)
+        if not text.startswith('mtaz error '):
+            raise
+        code, why = text[len('mtaz error '):].split(': ', 1)
+        raise _lib.MtazError(int(code), why) from None
 
 
 def _check_logits(logits):
@@ -81,32 +88,26 @@ def legal_masks(positions, device, rules_flags=RULES_FLAGS, move_cap=MOVE_CAP):
 
 # ---- penalties, bias and mask ----------------------------------------------------------------------------
 class _Taken:
-    """The actions taken and their penalties, as the C entries take them (args); keep: the tensors behind them."""
-    __slots__ = ('args', 'keep', 'host', 'bends')
+    """The actions taken and their penalties: tensors = (actions, lengths, penalties per row), host = the penalties that
+    are numbers, bends = whether the slope is other than 1 somewhere."""
+    __slots__ = ('tensors', 'host', 'bends')
 
     def __init__(self, logits, actions, lengths, repetition, frequency, presence):
         rows = logits.shape[0]
         given = (repetition, frequency, presence)
-        per_row = None
         tensors = [t for t in given if isinstance(t, torch.Tensor)]
         for t in tensors:
             _check_rows(t, 'a penalty', logits, ((rows,),), (torch.float32,))
             if t.requires_grad and torch.is_grad_enabled():
                 raise ValueError('penalties have no gradient')
-        if tensors:
-            host, self.host = None, (1.0, 0.0, 0.0)
-            if not isinstance(repetition, torch.Tensor) and not repetition > 0:
-                raise ValueError(f'repetition must be positive, got {repetition}')
-        else:
-            self.host = (float(repetition), float(frequency), float(presence))
-            host = _doubles(*self.host)
-            if not repetition > 0:
-                raise ValueError(f'repetition must be positive, got {repetition}')
-        self.bends = (isinstance(repetition, torch.Tensor) or repetition != 1.0)   # slope not 1
+        per_row_repetition = isinstance(repetition, torch.Tensor)
+        if not per_row_repetition and not repetition > 0:
+            raise ValueError(f'repetition must be positive, got {repetition}')
+        self.host = (1.0, 0.0, 0.0) if tensors else (float(repetition), float(frequency), float(presence))
         if actions is None:
             if lengths is not None:
                 raise ValueError('lengths without actions')
-            self.args, self.keep, self.bends = (None, 0, 0, None, host, None), (None, None, None), False
+            self.tensors, self.bends = (None, None, None), False
             return
         if actions.dim() != 2:
             raise ValueError(f'actions must be [rows, history], got {tuple(actions.shape)}')
@@ -115,19 +116,22 @@ class _Taken:
             _check_rows(lengths, 'lengths', logits, ((rows,),), (torch.int32,))
             lengths = lengths.contiguous()
         actions = _unit(actions)
+        per_row = None
         if tensors:
             per_row = torch.stack([t if isinstance(t, torch.Tensor) else torch.full((rows,), float(t), device=logits.device)
                                    for t in given], 1)
-        self.keep = (actions, lengths, per_row)
-        self.args = (actions.data_ptr(), actions.stride(0), actions.shape[1], _ptr(lengths), host, _ptr(per_row))
+        self.tensors, self.bends = (actions, lengths, per_row), per_row_repetition or repetition != 1.0
 
 
 def _adjust(x, legal, bias, taken, out):
     x, legal, bias = _unit(x), _unit(legal), _unit(bias)
     rows, cols = x.shape
+    actions, lengths, per_row = taken.tensors
+    stride, history = (0, 0) if actions is None else (actions.stride(0), actions.shape[1])
     _lib.check(_lib.lib().mtaz_adjust_logits(
         x.device.index, rows, cols, TYPES[x.dtype], x.data_ptr(), x.stride(0), out.data_ptr(), out.stride(0),
-        _ptr(legal), _row_stride(legal), _ptr(bias), _row_stride(bias), *taken.args, _stream(x.device)))
+        _ptr(legal), _row_stride(legal), _ptr(bias), _row_stride(bias), _ptr(actions), stride,
+        history, _ptr(lengths), _doubles(*taken.host), _ptr(per_row), _stream(x.device)))
     return out
 
 
@@ -149,13 +153,11 @@ def adjust_logits(logits, legal=None, bias=None, actions=None, lengths=None, rep
     if bias is not None:
         _check_rows(bias, 'bias', logits, ((cols,), (1, cols), (rows, cols)), (torch.float32,))
     taken = _Taken(logits, actions, lengths, repetition, frequency, presence)
-    if torch.is_grad_enabled() and (logits.requires_grad or (bias is not None and bias.requires_grad)):
-        if out is not None:
-            raise ValueError('out is not supported where a gradient is required')
-        return _lib.nodes().adjust_logits.default(logits, bias, legal, *taken.keep, *taken.host, taken.bends,
-                                                  _stream(logits.device))
     if out is None:
-        return _adjust(logits, legal, bias, taken, _fresh(logits))
+        return _call(_lib.nodes().adjust_logits.default, logits, bias, legal, *taken.tensors, *taken.host, taken.bends,
+                     _stream(logits.device))
+    if torch.is_grad_enabled() and (logits.requires_grad or (bias is not None and bias.requires_grad)):
+        raise ValueError('out is not supported where a gradient is required')
     if out.shape != logits.shape or out.dtype != logits.dtype or out.device != logits.device:
         raise ValueError('out must have the shape, type and device of logits')
     if (cols > 1 and out.stride(1) != 1) or (rows > 1 and out.stride(0) < cols):
@@ -185,25 +187,6 @@ def _check_loss(logits, target, value, reward, legal):
         raise ValueError('target and reward have no gradient')
 
 
-def _loss(logits, target, value, reward, legal, grad, value_grad, scale):
-    """(loss, the rows' statistics with the call's scratch memory behind them)"""
-    z, t, legal = _unit(logits), _unit(target), _unit(legal)
-    rows, cols = z.shape
-    dev = z.device
-    if value is not None:
-        value, reward = value.contiguous(), reward.contiguous()
-    entries = _lib.lib()
-    work = _lib.check(entries.mtaz_policy_loss_workspace(rows, cols))
-    stats = torch.empty(4 * rows + work // 4, dtype=torch.float32, device=dev)
-    loss = stats.new_empty(())
-    at = stats.data_ptr()
-    _lib.check(entries.mtaz_policy_loss(
-        dev.index, rows, cols, TYPES[z.dtype], TYPES[t.dtype], z.data_ptr(), z.stride(0), t.data_ptr(), t.stride(0),
-        _ptr(legal), _row_stride(legal), _ptr(value), _ptr(reward), loss.data_ptr(), at, _ptr(grad), cols,
-        _ptr(value_grad), scale, at + 16 * rows, work, _stream(dev)))
-    return loss, stats
-
-
 def policy_value_loss(logits, target, value=None, reward=None, legal=None):
     """The mean over the rows of (value - reward)^2 - sum over the legal v of target_v log softmax(logits)_v
     (exp/learner.py:86-87, where every action counts as legal), a float32 scalar.
@@ -213,9 +196,7 @@ def policy_value_loss(logits, target, value=None, reward=None, legal=None):
     a target of 0 adds nothing, and a row with nothing legal, or with every legal logit at -inf, adds its value term
     alone.  Differentiable in logits and value."""
     _check_loss(logits, target, value, reward, legal)
-    if torch.is_grad_enabled() and (logits.requires_grad or (value is not None and value.requires_grad)):
-        return _lib.nodes().policy_loss.default(logits, value, target, reward, legal, _stream(logits.device))
-    return _loss(logits, target, value, reward, legal, None, None, 1.0)[0]
+    return _call(_lib.nodes().policy_loss.default, logits, value, target, reward, legal, _stream(logits.device))
 
 
 def policy_value_loss_grad(logits, target, value=None, reward=None, legal=None, scale=1.0):
@@ -223,6 +204,5 @@ def policy_value_loss_grad(logits, target, value=None, reward=None, legal=None, 
     for torch.autograd.backward((logits, value), (d logits, d value)); the three are cut off from autograd's graph.
     With 16-bit logits a scale keeps small gradients in range."""
     _check_loss(logits, target, value, reward, legal)
-    dz = _fresh(logits)
-    dv = None if value is None else _fresh(value)
-    return _loss(logits, target, value, reward, legal, dz, dv, float(scale))[0], dz, dv
+    return _call(_lib.nodes().policy_loss_grad.default, logits, value, target, reward, legal, float(scale),
+                 _stream(logits.device))
