@@ -438,7 +438,7 @@ template <int DT, int DP, int THREADS, int REP, bool KEEP = true> struct Held {
 };
 
 // Rows of up to WAVE_COLS columns: a wave each, and everything stays in its registers.  4096 x 554 f32 with targets:
-// 9 us (18 MB).  ONE: a single workgroup takes all rows and their mean (32 x 554 with the gradient 8.6 us).
+// 8 us (18 MB).  ONE: a single workgroup takes all rows and their mean (32 x 554 with the gradient 8.6 us).
 template <int DT, int DP, bool ONE>
 __global__ __launch_bounds__(ONE ? 1024 : 256) void k_loss_wave(const typename Elem<DT>::T* z, int64_t z_stride,
                                                                 const typename Elem<DP>::T* pi, int64_t pi_stride,
