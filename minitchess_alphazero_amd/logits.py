@@ -27,9 +27,9 @@ def _unit(t):
     return t if t is None or t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
 
 
-def _row_stride(t, shared=False):
+def _row_stride(t):
     """Elements from one row to the next; 0 where one row serves all."""
-    return 0 if t is None or shared or t.dim() == 1 or t.shape[0] == 1 else t.stride(0)
+    return 0 if t is None or t.dim() == 1 or t.shape[0] == 1 else t.stride(0)
 
 
 def _check_rows(t, what, like, shapes, dtypes):
