@@ -230,6 +230,27 @@ def parity_stamp(engine, sims, weights_kind, seed_base):
             'plies': plies, 'first_mismatch': first, 'ok': ident == plies}
 
 
+def traffic_of(path, engine, games, sims, kernel):
+    """(HBM/fabric bytes per launch, where they come from) of the PMC passes in `path` (tools/gpu.sh pmc ->
+    tools/pmc_summary.py -> profiles/conv_traffic.json), attached only when those passes ran THIS engine (the file's
+    engine_sha256 stamp equals build.engine_hash() of the sources, which the loaded library was built from) on this
+    workload; else null with the reason: a change of the engine without a new PMC pass must not carry a stale
+    figure, and a change of the learner's operators beside it leaves the figure valid."""
+    name = os.path.relpath(path, HERE)
+    if not os.path.exists(path):
+        return None, f'no {name}'
+    try:
+        with open(path) as f:
+            tj = json.load(f)
+        if tj.get('engine_sha256') != engine:
+            return None, f'stale: PMC passes of engine {str(tj.get("engine_sha256"))[:16]}, running {engine[:16]}'
+        if not (tj.get('games') == games and tj.get('sims') == sims and kernel.startswith(tj.get('kernel', '?'))):
+            return None, f'PMC passes of another workload ({tj.get("games")} games, {tj.get("sims")} sims, {tj.get("kernel")})'
+        return tj.get('hbm_bytes_per_launch'), f'{name}: PMC passes of this engine ({engine[:16]}) on this workload'
+    except Exception as e:
+        return None, f'unreadable: {e}'
+
+
 def kernel_roofline(tot, prec):
     """Roofline of the dominant kernel from the engine's HIP events (one record per network launch).
       f16x3 (default): k_net_y, the fused network with all three split products on f16 MFMA (16x16x32);
@@ -634,29 +655,11 @@ def main():
         return
 
     roof = kernel_roofline(tot, prec)
-    # traffic: HBM/fabric bytes per launch from the PMC passes (tools/gpu.sh pmc -> tools/pmc_summary.py
-    # -> profiles/conv_traffic.json), attached only when those passes ran THIS library (the file's
-    # mtaz_src_sha256 stamp equals the loaded library's source hash) on this workload; else null, with
-    # the reason in traffic_source (a kernel change without a new PMC pass must not
-    # carry a stale figure)
     from minitchess_alphazero_amd import _lib
+    from minitchess_alphazero_amd.build import engine_hash
     lib_hash = _lib.lib().mtaz_version().decode().rsplit('mtaz-src-sha256=', 1)[-1]
-    traffic, why = None, f'no {os.path.relpath(args.traffic_json, HERE)}'
-    if os.path.exists(args.traffic_json):
-        try:
-            tj = json.load(open(args.traffic_json))
-            if tj.get('mtaz_src_sha256') != lib_hash:
-                why = (f'stale: PMC passes of library {str(tj.get("mtaz_src_sha256"))[:16]}, running '
-                       f'{lib_hash[:16]}')
-            elif not (tj.get('games') == args.games and tj.get('sims') == args.sims
-                      and roof['kernel'].startswith(tj.get('kernel', '?'))):
-                why = f'PMC passes of another workload ({tj.get("games")} games, {tj.get("sims")} sims, {tj.get("kernel")})'
-            else:
-                traffic = tj.get('hbm_bytes_per_launch')
-                why = (f'{os.path.relpath(args.traffic_json, HERE)}: PMC passes of this library '
-                       f'({lib_hash[:16]}) on this workload')
-        except Exception as e:
-            why = f'unreadable: {e}'
+    engine = engine_hash()
+    traffic, why = traffic_of(args.traffic_json, engine, args.games, args.sims, roof['kernel'])
     roof['traffic'] = traffic
     roof['traffic_source'] = why
     line = {
@@ -712,6 +715,7 @@ def main():
         'sync_mode': sync_mode,
         'defer': args.defer,
         'mtaz_src_sha256': lib_hash,
+        'engine_sha256': engine,
     }
     if parity is not None:
         line['parity'] = parity

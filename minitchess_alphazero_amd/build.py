@@ -17,6 +17,7 @@ _lib.lib() refuses a library whose hash differs from the sources next to it.
 import hashlib
 import importlib.util
 import os
+import re
 import subprocess
 import sys
 
@@ -73,6 +74,26 @@ def source_hash():
     with open(os.path.join(INCLUDE, 'mtaz.h'), 'rb') as f:
         h.update(b'include/mtaz.h\0' + f.read())
     h.update(repr((SOURCES, ARCH)).encode())
+    return h.hexdigest()
+
+
+# what the learner's operators alone are built from: no engine code is in it
+OPERATOR_FILES = ('mtaz_muon.hip', 'mtaz_logits.hip', 'mtaz_autograd.cpp', 'ops.h')
+
+
+def engine_hash():
+    """sha256 over what the engine (tree and network kernels, host driver) is built from: source_hash() without the
+    learner operators' files and their part of include/mtaz.h.  Measurements of the engine carry it, so that they
+    stay attached while only the operators change."""
+    h = hashlib.sha256()
+    for name in sorted(os.listdir(CSRC)):
+        path = os.path.join(CSRC, name)
+        if os.path.isfile(path) and name not in OPERATOR_FILES:
+            with open(path, 'rb') as f:
+                h.update(b'csrc/' + name.encode() + b'\0' + f.read())
+    with open(os.path.join(INCLUDE, 'mtaz.h'), 'rb') as f:
+        h.update(b'include/mtaz.h\0' + re.sub(rb'/\* -+ learner operators .*?(?=/\* ----)', b'', f.read(), flags=re.S))
+    h.update(repr(([s for s in SOURCES if s[0] not in OPERATOR_FILES], ARCH)).encode())
     return h.hexdigest()
 
 

@@ -100,8 +100,9 @@ def main():
     }
     if line is not None:
         out['boards_per_launch'] = line['roofline']['flop_per_launch'] / 638245892
-        # the library the passes ran (bench.py attaches this file's traffic only to a run of the same one)
+        # the library the passes ran, and its engine (bench.py attaches this file's traffic only to a run of the same engine)
         out['mtaz_src_sha256'] = line.get('mtaz_src_sha256')
+        out['engine_sha256'] = line.get('engine_sha256')
     hashes = bench_hashes(args.root)
     if len(hashes) > 1:
         raise SystemExit(f'PMC passes ran different libraries: {sorted(hashes)}')
