@@ -118,6 +118,10 @@ def _tu_key(src, cmd):
     return h.hexdigest()
 
 
+def _rocm():
+    return os.environ.get('ROCM_PATH', '/opt/rocm')
+
+
 def _torch_dir():
     return list(importlib.util.find_spec('torch').submodule_search_locations)[0]
 
@@ -136,12 +140,13 @@ def build_autograd(force=False, verbose=True):
     if not force and embedded_hash(OUT_AUTOGRAD, b'mtaz-autograd-sha256=') == autograd_hash():
         return OUT_AUTOGRAD
     torch_dir, tmp = _torch_dir(), OUT_AUTOGRAD + '.tmp'
-    cmd = ['g++', '-shared', '-fPIC', '-std=c++17', '-O2', '-Wall',
+    cmd = ['g++', '-shared', '-fPIC', '-std=c++17', '-O2', '-Wall', '-D__HIP_PLATFORM_AMD__',
            f'-DMTAZ_AUTOGRAD_SHA256="mtaz-autograd-sha256={autograd_hash()}"', f'-I{INCLUDE}',
            '-isystem', os.path.join(torch_dir, 'include'),
            '-isystem', os.path.join(torch_dir, 'include', 'torch', 'csrc', 'api', 'include'),
+           '-isystem', os.path.join(_rocm(), 'include'),
            os.path.join(CSRC, 'mtaz_autograd.cpp'), '-o', tmp, '-L' + os.path.join(torch_dir, 'lib'), '-ltorch',
-           '-ltorch_cpu', '-lc10', '-L' + HERE, '-lmtaz', '-Wl,-rpath,$ORIGIN']
+           '-ltorch_cpu', '-lc10', '-lc10_hip', '-L' + HERE, '-lmtaz', '-Wl,-rpath,$ORIGIN']
     if verbose:
         print(' '.join(cmd), flush=True)
     subprocess.check_call(cmd)

@@ -1,8 +1,16 @@
 // The logits operators for torch, over the C entries of libmtaz.so: nodes of its autograd graph where a gradient is
 // required, plain calls elsewhere.
 //
+// Each operator is one of torch's dispatcher: an implementation on the GPU that calls the C entry, one that knows the
+// results' shapes alone (Meta), and one for autograd where it has a gradient.  What records torch's operators (a tracer,
+// tensors without data) so sees the operator itself, its backward pass likewise.  The stream is the current one of
+// the moment of the call.
+//
 // A node written in Python has the engine's own thread wait for the interpreter: forward and backward of a loss of 64 x
 // 554 took the host 105 us that way and takes 72 here.  A call without gradients costs it 3 us less than through ctypes.
+#include <ATen/core/LegacyTypeDispatch.h>
+#include <ATen/core/dispatch/Dispatcher.h>
+#include <c10/hip/HIPStream.h>
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/library.h>
@@ -15,6 +23,8 @@ using at::Tensor;
 using torch::autograd::AutogradContext;
 using torch::autograd::variable_list;
 using MaybeTensor = std::optional<Tensor>;
+using Two = std::tuple<Tensor, Tensor>;
+using Three = std::tuple<Tensor, Tensor, Tensor>;
 
 int type_of(const Tensor& t) {
   return t.scalar_type() == at::kFloat ? MTAZ_F32 : t.scalar_type() == at::kHalf ? MTAZ_F16 : MTAZ_BF16;
@@ -22,8 +32,9 @@ int type_of(const Tensor& t) {
 // t with its last dimension dense (a copy where it is not)
 Tensor unit(const Tensor& t) { return !t.defined() || t.size(-1) == 1 || t.stride(-1) == 1 ? t : t.contiguous(); }
 Tensor dense(const Tensor& t) { return t.defined() ? t.contiguous() : t; }
-Tensor fresh(const Tensor& like) { return at::empty(like.sizes(), like.options()); }
+Tensor fresh(const Tensor& like) { return at::empty_symint(like.sym_sizes(), like.options()); }
 Tensor or_none(const MaybeTensor& t) { return t ? *t : Tensor(); }
+bool there(const MaybeTensor& t) { return t && t->defined(); }
 void* at(const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
 // elements from one row to the next; 0 where one row serves all
 int64_t row_stride(const Tensor& t) { return !t.defined() || t.dim() == 1 || t.size(0) == 1 ? 0 : t.stride(0); }
@@ -31,7 +42,121 @@ int64_t checked(int64_t rc) {
   TORCH_CHECK(rc >= 0, "mtaz error ", rc, ": ", mtaz_last_error());
   return rc;
 }
-void* stream_of(AutogradContext* ctx) { return (void*)ctx->saved_data["stream"].toInt(); }   // a node runs where it was made
+// the current stream of t's device; autograd's engine runs a backward pass on that of its forward pass
+void* stream_of(const Tensor& t) { return (void*)c10::hip::getCurrentHIPStream(t.get_device()).stream(); }
+
+// ---- the operators on the GPU -----------------------------------------------------------------------------------
+// The loss and the rows' statistics; with gradients of scale * loss where dz or dv is defined.
+Two loss_of(const Tensor& logits, const MaybeTensor& value, const Tensor& target, const MaybeTensor& reward,
+            const MaybeTensor& legal, const Tensor& dz, const Tensor& dv, double scale) {
+  const Tensor z = unit(logits), t = unit(target), mask = unit(or_none(legal)), v = dense(or_none(value)),
+               r = dense(or_none(reward));
+  const int64_t rows = z.size(0), cols = z.size(1), size = checked(mtaz_policy_loss_workspace(rows, cols));
+  const auto floats = z.options().dtype(at::kFloat);
+  Tensor loss = at::empty({}, floats), stats = at::empty({rows, 4}, floats), work = at::empty({(size + 3) / 4}, floats);
+  checked(mtaz_policy_loss(z.get_device(), rows, cols, type_of(z), type_of(t), at(z), z.stride(0), at(t), t.stride(0),
+                           (const uint32_t*)at(mask), row_stride(mask), (const float*)at(v), (const float*)at(r),
+                           (float*)at(loss), (float*)at(stats), at(dz), cols, (float*)at(dv), scale, at(work), size,
+                           stream_of(z)));
+  return {loss, stats};
+}
+Two loss_gpu(const Tensor& logits, const MaybeTensor& value, const Tensor& target, const MaybeTensor& reward,
+             const MaybeTensor& legal) {
+  return loss_of(logits, value, target, reward, legal, Tensor(), Tensor(), 1.);
+}
+Three loss_grad_gpu(const Tensor& logits, const MaybeTensor& value, const Tensor& target, const MaybeTensor& reward,
+                    const MaybeTensor& legal, double scale) {
+  const Tensor dz = fresh(logits), dv = there(value) ? fresh(*value) : Tensor();
+  return {std::get<0>(loss_of(logits, value, target, reward, legal, dz, dv, scale)), dz, dv};
+}
+Two loss_back_gpu(const Tensor& grad, const Tensor& logits, const MaybeTensor& value, const Tensor& target,
+                  const MaybeTensor& reward, const MaybeTensor& legal, const Tensor& stats, bool want_z, bool want_v) {
+  const Tensor g = dense(grad), z = unit(logits), v = dense(or_none(value)), t = unit(target), r = dense(or_none(reward)),
+               mask = unit(or_none(legal)), dz = want_z ? fresh(z) : Tensor(), dv = want_v ? fresh(v) : Tensor();
+  checked(mtaz_policy_loss_grad(z.get_device(), z.size(0), z.size(1), type_of(z), type_of(t), at(z), z.stride(0), at(t),
+                                t.stride(0), (const uint32_t*)at(mask), row_stride(mask), (const float*)at(v),
+                                (const float*)at(r), (const float*)at(stats), (const float*)at(g), at(dz), z.size(1),
+                                (float*)at(dv), stream_of(z)));
+  return {dz, dv};
+}
+Tensor adjust_gpu(const Tensor& logits, const MaybeTensor& bias, const MaybeTensor& legal, const MaybeTensor& actions,
+                  const MaybeTensor& lengths, const MaybeTensor& per_row, double repetition, double frequency,
+                  double presence, bool) {
+  const Tensor x = unit(logits), b = unit(or_none(bias)), mask = unit(or_none(legal)), a = or_none(actions), y = fresh(x);
+  const double penalties[3] = {repetition, frequency, presence};
+  checked(mtaz_adjust_logits(x.get_device(), x.size(0), x.size(1), type_of(x), at(x), x.stride(0), at(y), x.size(1),
+                             (const uint32_t*)at(mask), row_stride(mask), (const float*)at(b), row_stride(b),
+                             (const int32_t*)at(a), a.defined() ? a.stride(0) : 0, a.defined() ? (int)a.size(1) : 0,
+                             (const int32_t*)at(or_none(lengths)), penalties, (const float*)at(or_none(per_row)),
+                             stream_of(x)));
+  return y;
+}
+// bias: the shape of the bias whose gradient is wanted
+Two adjust_back_gpu(const Tensor& grad, const MaybeTensor& logits, const MaybeTensor& legal, const MaybeTensor& actions,
+                    const MaybeTensor& lengths, const MaybeTensor& per_row, double repetition, bool want_x,
+                    at::OptionalIntArrayRef bias) {
+  const Tensor g = unit(grad), x = unit(or_none(logits)), mask = unit(or_none(legal)), a = or_none(actions);
+  const int64_t rows = g.size(0), cols = g.size(1);
+  const Tensor dx = want_x ? fresh(g) : Tensor();
+  const bool shared = bias && (bias->size() == 1 || (*bias)[0] == 1);
+  const int64_t size = shared ? checked(mtaz_adjust_logits_grad_workspace(rows, cols)) : 0;
+  const auto floats = g.options().dtype(at::kFloat);
+  const Tensor db = bias ? at::empty(*bias, floats) : Tensor(),
+               work = shared ? at::empty({std::max<int64_t>(size, 4) / 4}, floats) : Tensor();
+  const double penalties[3] = {repetition, 0., 0.};     // the others are constants
+  checked(mtaz_adjust_logits_grad(g.get_device(), rows, cols, type_of(g), at(g), g.stride(0), at(x),
+                                  x.defined() ? x.stride(0) : 0, at(dx), cols, (float*)at(db), shared ? 0 : cols,
+                                  (const uint32_t*)at(mask), row_stride(mask), (const int32_t*)at(a),
+                                  a.defined() ? a.stride(0) : 0, a.defined() ? (int)a.size(1) : 0,
+                                  (const int32_t*)at(or_none(lengths)), penalties, (const float*)at(or_none(per_row)),
+                                  at(work), size, stream_of(g)));
+  return {dx, db};
+}
+
+// ---- their shapes -----------------------------------------------------------------------------------------------
+Tensor floats_like(const Tensor& t, c10::SymIntArrayRef size) { return at::empty_symint(size, t.options().dtype(at::kFloat)); }
+
+Two loss_meta(const Tensor& logits, const MaybeTensor&, const Tensor&, const MaybeTensor&, const MaybeTensor&) {
+  return {floats_like(logits, {}), floats_like(logits, {logits.sym_size(0), 4})};
+}
+Three loss_grad_meta(const Tensor& logits, const MaybeTensor& value, const Tensor&, const MaybeTensor&, const MaybeTensor&,
+                     double) {
+  return {floats_like(logits, {}), fresh(logits), there(value) ? fresh(*value) : Tensor()};
+}
+Two loss_back_meta(const Tensor&, const Tensor& logits, const MaybeTensor& value, const Tensor&, const MaybeTensor&,
+                   const MaybeTensor&, const Tensor&, bool want_z, bool want_v) {
+  return {want_z ? fresh(logits) : Tensor(), want_v ? fresh(*value) : Tensor()};
+}
+Tensor adjust_meta(const Tensor& logits, const MaybeTensor&, const MaybeTensor&, const MaybeTensor&, const MaybeTensor&,
+                   const MaybeTensor&, double, double, double, bool) {
+  return fresh(logits);
+}
+Two adjust_back_meta(const Tensor& grad, const MaybeTensor&, const MaybeTensor&, const MaybeTensor&, const MaybeTensor&,
+                     const MaybeTensor&, double, bool want_x, at::OptionalIntArrayRef bias) {
+  return {want_x ? fresh(grad) : Tensor(), bias ? at::empty(*bias, grad.options().dtype(at::kFloat)) : Tensor()};
+}
+
+// ---- autograd ---------------------------------------------------------------------------------------------------
+// The operator `name` of F's type below autograd
+template <typename F> auto operator_of(const char* name) {
+  return c10::Dispatcher::singleton().findSchemaOrThrow(name, "").typed<F>();
+}
+Two loss_below(const Tensor& logits, const MaybeTensor& value, const Tensor& target, const MaybeTensor& reward,
+               const MaybeTensor& legal) {
+  static const auto op = operator_of<decltype(loss_gpu)>("mtaz::policy_loss");
+  const at::AutoDispatchBelowADInplaceOrView below;
+  return op.call(logits, value, target, reward, legal);
+}
+Tensor adjust_below(const Tensor& logits, const MaybeTensor& bias, const MaybeTensor& legal, const MaybeTensor& actions,
+                    const MaybeTensor& lengths, const MaybeTensor& per_row, double repetition, double frequency,
+                    double presence, bool bends) {
+  static const auto op = operator_of<decltype(adjust_gpu)>("mtaz::adjust_logits");
+  const at::AutoDispatchBelowADInplaceOrView below;
+  return op.call(logits, bias, legal, actions, lengths, per_row, repetition, frequency, presence, bends);
+}
+bool wanted(const Tensor& a, const MaybeTensor& b) {
+  return at::GradMode::is_enabled() && (a.requires_grad() || (there(b) && b->requires_grad()));
+}
 
 // Gradients that cannot be differentiated once more: with create_graph they say so, and are no constants.
 variable_list once(variable_list grads) {
@@ -49,136 +174,109 @@ variable_list once(variable_list grads) {
   return grads;
 }
 
-// The loss and the rows' statistics; with gradients of scale * loss where dz or dv is defined.
-std::pair<Tensor, Tensor> loss_of(const Tensor& logits, const Tensor& value, const Tensor& target, const Tensor& reward,
-                                  const Tensor& legal, const Tensor& dz, const Tensor& dv, double scale, int64_t stream) {
-  const Tensor z = unit(logits), t = unit(target), mask = unit(legal), v = dense(value), r = dense(reward);
-  const int64_t rows = z.size(0), cols = z.size(1), work = checked(mtaz_policy_loss_workspace(rows, cols));
-  const auto floats = z.options().dtype(at::kFloat);
-  Tensor loss = at::empty({}, floats), stats = at::empty({4 * rows + work / 4}, floats);   // scratch memory behind them
-  float* const s = (float*)stats.data_ptr();
-  checked(mtaz_policy_loss(z.get_device(), rows, cols, type_of(z), type_of(t), at(z), z.stride(0), at(t), t.stride(0),
-                           (const uint32_t*)at(mask), row_stride(mask), (const float*)at(v), (const float*)at(r),
-                           (float*)at(loss), s, at(dz), cols, (float*)at(dv), scale, s + 4 * rows, work, (void*)stream));
-  return {loss, stats};
-}
-Tensor adjusted(const Tensor& logits, const Tensor& bias, const Tensor& legal, const Tensor& a, const Tensor& n,
-                const Tensor& p, const double* penalties, int64_t stream) {
-  const Tensor x = unit(logits), b = unit(bias), mask = unit(legal), y = fresh(x);
-  checked(mtaz_adjust_logits(x.get_device(), x.size(0), x.size(1), type_of(x), at(x), x.stride(0), at(y), x.size(1),
-                             (const uint32_t*)at(mask), row_stride(mask), (const float*)at(b), row_stride(b),
-                             (const int32_t*)at(a), a.defined() ? a.stride(0) : 0, a.defined() ? (int)a.size(1) : 0,
-                             (const int32_t*)at(n), penalties, (const float*)at(p), (void*)stream));
-  return y;
-}
-bool wanted(const Tensor& a, const MaybeTensor& b) {
-  return at::GradMode::is_enabled() && (a.requires_grad() || (b && b->defined() && b->requires_grad()));
-}
-
 struct PolicyLoss : torch::autograd::Function<PolicyLoss> {
-  static Tensor forward(AutogradContext* ctx, const Tensor& logits, const MaybeTensor& value, const Tensor& target,
-                        const MaybeTensor& reward, const MaybeTensor& legal, int64_t stream) {
-    const auto [loss, stats] = loss_of(logits, or_none(value), target, or_none(reward), or_none(legal), Tensor(), Tensor(), 1.,
-                                       stream);
+  static variable_list forward(AutogradContext* ctx, const Tensor& logits, const MaybeTensor& value, const Tensor& target,
+                               const MaybeTensor& reward, const MaybeTensor& legal) {
+    const auto [loss, stats] = loss_below(logits, value, target, reward, legal);
     ctx->save_for_backward({logits, or_none(value), target, or_none(reward), or_none(legal), stats});
-    ctx->saved_data["stream"] = stream;
-    return loss;
+    ctx->mark_non_differentiable({stats});
+    ctx->set_materialize_grads(false);
+    return {loss, stats};
   }
   static variable_list backward(AutogradContext* ctx, const variable_list& grads) {
+    static const auto op = operator_of<decltype(loss_back_gpu)>("mtaz::policy_loss_back");
     const variable_list saved = ctx->get_saved_variables();
-    const Tensor g = dense(grads[0]), z = unit(saved[0]), v = dense(saved[1]), t = unit(saved[2]), r = dense(saved[3]),
-                 mask = unit(saved[4]);
     Tensor dz, dv;
-    if (g.defined()) {
-      if (ctx->needs_input_grad(0)) dz = fresh(z);
-      if (v.defined() && ctx->needs_input_grad(1)) dv = fresh(v);
-      const int64_t rows = z.size(0), cols = z.size(1);
-      checked(mtaz_policy_loss_grad(z.get_device(), rows, cols, type_of(z), type_of(t), at(z), z.stride(0), at(t), t.stride(0),
-                                    (const uint32_t*)at(mask), row_stride(mask), (const float*)at(v), (const float*)at(r),
-                                    (const float*)at(saved[5]), (const float*)at(g), at(dz), cols, (float*)at(dv),
-                                    stream_of(ctx)));
+    if (grads[0].defined()) {
+      const at::AutoDispatchBelowADInplaceOrView below;
+      std::tie(dz, dv) = op.call(grads[0], saved[0], saved[1], saved[2], saved[3], saved[4], saved[5],
+                                 ctx->needs_input_grad(0), saved[1].defined() && ctx->needs_input_grad(1));
     }
-    return once({dz, dv, Tensor(), Tensor(), Tensor(), Tensor()});
+    return once({dz, dv, Tensor(), Tensor(), Tensor()});
   }
 };
 
 struct AdjustLogits : torch::autograd::Function<AdjustLogits> {
   static Tensor forward(AutogradContext* ctx, const Tensor& logits, const MaybeTensor& bias, const MaybeTensor& legal,
                         const MaybeTensor& actions, const MaybeTensor& lengths, const MaybeTensor& per_row,
-                        double repetition, double frequency, double presence, bool bends, int64_t stream) {
-    const Tensor a = or_none(actions), n = or_none(lengths), p = or_none(per_row);
-    const double penalties[3] = {repetition, frequency, presence};
-    const Tensor y = adjusted(logits, or_none(bias), or_none(legal), a, n, p, penalties, stream);
+                        double repetition, double frequency, double presence, bool bends) {
+    const Tensor y = adjust_below(logits, bias, legal, actions, lengths, per_row, repetition, frequency, presence, bends);
     // where the penalties do not bend the logits their gradient is 1, and neither these nor the actions are needed
-    ctx->save_for_backward(bends ? variable_list{logits, or_none(legal), a, n, p}
+    ctx->save_for_backward(bends ? variable_list{logits, or_none(legal), or_none(actions), or_none(lengths), or_none(per_row)}
                                  : variable_list{Tensor(), or_none(legal), Tensor(), Tensor(), Tensor()});
-    ctx->saved_data["stream"] = stream;
-    ctx->saved_data["type"] = (int64_t)type_of(logits);
     ctx->saved_data["repetition"] = repetition;
-    if (bias && bias->defined()) ctx->saved_data["bias"] = bias->sizes().vec();
+    if (there(bias)) ctx->saved_data["bias"] = bias->sizes().vec();
     return y;
   }
   static variable_list backward(AutogradContext* ctx, const variable_list& grads) {
+    static const auto op = operator_of<decltype(adjust_back_gpu)>("mtaz::adjust_logits_back");
     const variable_list saved = ctx->get_saved_variables();
-    const Tensor g = unit(grads[0]), x = unit(saved[0]), mask = unit(saved[1]), a = saved[2], n = saved[3], p = saved[4];
-    Tensor dx, db, work;
-    if (g.defined()) {
-      const int64_t rows = g.size(0), cols = g.size(1);
-      int64_t size = 0;
-      bool shared = false;
-      if (ctx->needs_input_grad(0)) dx = fresh(g);
+    variable_list out(10);
+    if (grads[0].defined()) {
       const auto bias = ctx->saved_data.find("bias");
-      if (bias != ctx->saved_data.end() && ctx->needs_input_grad(1)) {
-        const std::vector<int64_t> shape = bias->second.toIntVector();
-        db = at::empty(shape, g.options().dtype(at::kFloat));
-        shared = shape.size() == 1 || shape[0] == 1;
-        if (shared) {
-          size = checked(mtaz_adjust_logits_grad_workspace(rows, cols));
-          work = at::empty({size > 0 ? size : 1}, g.options().dtype(at::kByte));
-        }
-      }
-      const double penalties[3] = {ctx->saved_data["repetition"].toDouble(), 0., 0.};   // the others are constants
-      checked(mtaz_adjust_logits_grad(g.get_device(), rows, cols, (int)ctx->saved_data["type"].toInt(), at(g), g.stride(0),
-                                      at(x), x.defined() ? x.stride(0) : 0, at(dx), cols, (float*)at(db), shared ? 0 : cols,
-                                      (const uint32_t*)at(mask), row_stride(mask), (const int32_t*)at(a),
-                                      a.defined() ? a.stride(0) : 0, a.defined() ? (int)a.size(1) : 0, (const int32_t*)at(n),
-                                      penalties, (const float*)at(p), at(work), size, stream_of(ctx)));
+      std::vector<int64_t> shape;
+      at::OptionalIntArrayRef sizes;
+      if (bias != ctx->saved_data.end() && ctx->needs_input_grad(1)) shape = bias->second.toIntVector(), sizes = shape;
+      const at::AutoDispatchBelowADInplaceOrView below;
+      std::tie(out[0], out[1]) = op.call(grads[0], saved[0], saved[1], saved[2], saved[3], saved[4],
+                                         ctx->saved_data["repetition"].toDouble(), ctx->needs_input_grad(0), sizes);
     }
-    variable_list out(11);
-    out[0] = dx, out[1] = db;
     return once(std::move(out));
   }
 };
 
-Tensor policy_loss(const Tensor& logits, const MaybeTensor& value, const Tensor& target, const MaybeTensor& reward,
-                   const MaybeTensor& legal, int64_t stream) {
-  if (wanted(logits, value)) return PolicyLoss::apply(logits, value, target, reward, legal, stream);
-  return loss_of(logits, or_none(value), target, or_none(reward), or_none(legal), Tensor(), Tensor(), 1., stream).first;
+Two loss_autograd(const Tensor& logits, const MaybeTensor& value, const Tensor& target, const MaybeTensor& reward,
+                  const MaybeTensor& legal) {
+  if (!wanted(logits, value)) return loss_below(logits, value, target, reward, legal);
+  const variable_list out = PolicyLoss::apply(logits, value, target, reward, legal);
+  return {out[0], out[1]};
 }
-std::tuple<Tensor, Tensor, Tensor> policy_loss_grad(const Tensor& logits, const MaybeTensor& value, const Tensor& target,
-                                                    const MaybeTensor& reward, const MaybeTensor& legal, double scale,
-                                                    int64_t stream) {
-  const at::NoGradGuard off;
-  const Tensor v = or_none(value), dz = fresh(logits), dv = v.defined() ? fresh(v) : Tensor();
-  return {loss_of(logits, v, target, or_none(reward), or_none(legal), dz, dv, scale, stream).first, dz, dv};
+// cut off from the graph
+Three loss_grad_autograd(const Tensor& logits, const MaybeTensor& value, const Tensor& target, const MaybeTensor& reward,
+                         const MaybeTensor& legal, double scale) {
+  static const auto op = operator_of<decltype(loss_grad_gpu)>("mtaz::policy_loss_grad");
+  const at::AutoDispatchBelowADInplaceOrView below;
+  return op.call(logits, value, target, reward, legal, scale);
 }
-Tensor adjust_logits(const Tensor& logits, const MaybeTensor& bias, const MaybeTensor& legal, const MaybeTensor& actions,
-                     const MaybeTensor& lengths, const MaybeTensor& per_row, double repetition, double frequency,
-                     double presence, bool bends, int64_t stream) {
-  if (!wanted(logits, bias)) {
-    const double penalties[3] = {repetition, frequency, presence};
-    return adjusted(logits, or_none(bias), or_none(legal), or_none(actions), or_none(lengths), or_none(per_row), penalties,
-                    stream);
-  }
-  return AdjustLogits::apply(logits, bias, legal, actions, lengths, per_row, repetition, frequency, presence, bends, stream);
+Tensor adjust_autograd(const Tensor& logits, const MaybeTensor& bias, const MaybeTensor& legal, const MaybeTensor& actions,
+                       const MaybeTensor& lengths, const MaybeTensor& per_row, double repetition, double frequency,
+                       double presence, bool bends) {
+  if (!wanted(logits, bias))
+    return adjust_below(logits, bias, legal, actions, lengths, per_row, repetition, frequency, presence, bends);
+  return AdjustLogits::apply(logits, bias, legal, actions, lengths, per_row, repetition, frequency, presence, bends);
 }
 std::string built_from() { return MTAZ_AUTOGRAD_SHA256; }
 
 }  // namespace
 
 TORCH_LIBRARY(mtaz, m) {
-  m.def("policy_loss", &policy_loss);
-  m.def("policy_loss_grad", &policy_loss_grad);
-  m.def("adjust_logits", &adjust_logits);
-  m.def("built_from", &built_from);
+  m.def("policy_loss(Tensor logits, Tensor? value, Tensor target, Tensor? reward, Tensor? legal) -> (Tensor, Tensor)");
+  m.def("policy_loss_grad(Tensor logits, Tensor? value, Tensor target, Tensor? reward, Tensor? legal, float scale) -> "
+        "(Tensor, Tensor, Tensor)");
+  m.def("policy_loss_back(Tensor grad, Tensor logits, Tensor? value, Tensor target, Tensor? reward, Tensor? legal, "
+        "Tensor stats, bool want_z, bool want_v) -> (Tensor, Tensor)");
+  m.def("adjust_logits(Tensor logits, Tensor? bias, Tensor? legal, Tensor? actions, Tensor? lengths, Tensor? per_row, "
+        "float repetition, float frequency, float presence, bool bends) -> Tensor");
+  m.def("adjust_logits_back(Tensor grad, Tensor? logits, Tensor? legal, Tensor? actions, Tensor? lengths, "
+        "Tensor? per_row, float repetition, bool want_x, int[]? bias) -> (Tensor, Tensor)");
+  m.def("built_from() -> str", &built_from);
+}
+TORCH_LIBRARY_IMPL(mtaz, CUDA, m) {
+  m.impl("policy_loss", &loss_gpu);
+  m.impl("policy_loss_grad", &loss_grad_gpu);
+  m.impl("policy_loss_back", &loss_back_gpu);
+  m.impl("adjust_logits", &adjust_gpu);
+  m.impl("adjust_logits_back", &adjust_back_gpu);
+}
+TORCH_LIBRARY_IMPL(mtaz, Meta, m) {
+  m.impl("policy_loss", &loss_meta);
+  m.impl("policy_loss_grad", &loss_grad_meta);
+  m.impl("policy_loss_back", &loss_back_meta);
+  m.impl("adjust_logits", &adjust_meta);
+  m.impl("adjust_logits_back", &adjust_back_meta);
+}
+TORCH_LIBRARY_IMPL(mtaz, Autograd, m) {
+  m.impl("policy_loss", &loss_autograd);
+  m.impl("policy_loss_grad", &loss_grad_autograd);
+  m.impl("adjust_logits", &adjust_autograd);
 }

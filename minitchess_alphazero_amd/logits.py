@@ -154,8 +154,7 @@ def adjust_logits(logits, legal=None, bias=None, actions=None, lengths=None, rep
         _check_rows(bias, 'bias', logits, ((cols,), (1, cols), (rows, cols)), (torch.float32,))
     taken = _Taken(logits, actions, lengths, repetition, frequency, presence)
     if out is None:
-        return _call(_lib.nodes().adjust_logits.default, logits, bias, legal, *taken.tensors, *taken.host, taken.bends,
-                     _stream(logits.device))
+        return _call(_lib.nodes().adjust_logits.default, logits, bias, legal, *taken.tensors, *taken.host, taken.bends)
     if torch.is_grad_enabled() and (logits.requires_grad or (bias is not None and bias.requires_grad)):
         raise ValueError('out is not supported where a gradient is required')
     if out.shape != logits.shape or out.dtype != logits.dtype or out.device != logits.device:
@@ -196,7 +195,7 @@ def policy_value_loss(logits, target, value=None, reward=None, legal=None):
     a target of 0 adds nothing, and a row with nothing legal, or with every legal logit at -inf, adds its value term
     alone.  Differentiable in logits and value."""
     _check_loss(logits, target, value, reward, legal)
-    return _call(_lib.nodes().policy_loss.default, logits, value, target, reward, legal, _stream(logits.device))
+    return _call(_lib.nodes().policy_loss.default, logits, value, target, reward, legal)[0]
 
 
 def policy_value_loss_grad(logits, target, value=None, reward=None, legal=None, scale=1.0):
@@ -204,5 +203,4 @@ def policy_value_loss_grad(logits, target, value=None, reward=None, legal=None, 
     for torch.autograd.backward((logits, value), (d logits, d value)); the three are cut off from autograd's graph.
     With 16-bit logits a scale keeps small gradients in range."""
     _check_loss(logits, target, value, reward, legal)
-    return _call(_lib.nodes().policy_loss_grad.default, logits, value, target, reward, legal, float(scale),
-                 _stream(logits.device))
+    return _call(_lib.nodes().policy_loss_grad.default, logits, value, target, reward, legal, float(scale))

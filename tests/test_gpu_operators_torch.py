@@ -1,0 +1,43 @@
+"""GPU: the learner operators under what torch does with operators: tracing, streams, derivatives that they lack."""
+import pytest
+import torch
+from torch.fx.experimental.proxy_tensor import make_fx
+
+from minitchess_alphazero_amd import logits as ops
+from test_gpu_logits import gen, make, pack
+
+pytestmark = pytest.mark.gpu
+
+
+def inputs(seed, rows=6, cols=70):
+    x, legal, actions, lengths = make(rows, cols, 9, seed)
+    t = torch.rand(rows, cols, generator=gen(seed)) * legal
+    v = torch.rand(rows, 1, generator=gen(seed + 1))
+    return [a.cuda() for a in (x, torch.randn(cols, generator=gen(seed + 2)), v, pack(legal), actions, lengths, t)]
+
+
+def step(x, b, v, mask, actions, lengths, t):
+    """Adjusted logits into the loss, and back to logits, bias and value."""
+    leaves = [a.detach().requires_grad_() for a in (x, b, v)]
+    y = ops.adjust_logits(leaves[0], mask, leaves[1], actions, lengths, 1.2, 0.1, 0.3)
+    loss = ops.policy_value_loss(y, t, leaves[2], torch.ones_like(v))
+    return (y.detach(), loss.detach(), *torch.autograd.grad(loss, leaves), *ops.policy_value_loss_grad(x, t, legal=mask)[:2])
+
+
+def test_traced_graph_computes():
+    """The trace holds the operators, their backward passes too, and computes what the call does, for other inputs and on
+    another stream than the one it was recorded on."""
+    graph = make_fx(step)(*inputs(1))
+    names = [str(n.target) for n in graph.graph.nodes if str(n.target).startswith('mtaz.')]
+    assert sorted(set(names)) == ['mtaz.adjust_logits.default', 'mtaz.adjust_logits_back.default', 'mtaz.policy_loss.default',
+                                  'mtaz.policy_loss_back.default', 'mtaz.policy_loss_grad.default']
+    side = torch.cuda.Stream()
+    for seed in (1, 2, 3):
+        args = inputs(seed)
+        want = step(*args)
+        assert all(torch.equal(a, b) for a, b in zip(graph(*args), want))
+        torch.cuda.synchronize()
+        with torch.cuda.stream(side):
+            got = graph(*[a * 1 for a in args])   # a wrong stream would read these before they are there
+        side.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
