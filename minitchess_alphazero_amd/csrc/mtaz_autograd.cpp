@@ -158,6 +158,13 @@ bool wanted(const Tensor& a, const MaybeTensor& b) {
   return at::GradMode::is_enabled() && (a.requires_grad() || (there(b) && b->requires_grad()));
 }
 
+// An input that carries a tangent (forward-mode differentiation) is refused: without this the result would have none,
+// which says that its derivative is 0.
+template <typename... T> void no_tangent(const char* what, const T&... inputs) {
+  auto has = [](const MaybeTensor& t) { return there(t) && t->_fw_grad(0).defined(); };
+  TORCH_CHECK_VALUE(!(has(inputs) || ...), what, " has no forward-mode derivative");
+}
+
 // Gradients that cannot be differentiated once more: with create_graph they say so, and are no constants.
 variable_list once(variable_list grads) {
   if (!at::GradMode::is_enabled()) return grads;
@@ -188,6 +195,7 @@ struct PolicyLoss : torch::autograd::Function<PolicyLoss> {
     const variable_list saved = ctx->get_saved_variables();
     Tensor dz, dv;
     if (grads[0].defined()) {
+      no_tangent("policy_value_loss's backward pass", grads[0], saved[0], saved[1]);
       const at::AutoDispatchBelowADInplaceOrView below;
       std::tie(dz, dv) = op.call(grads[0], saved[0], saved[1], saved[2], saved[3], saved[4], saved[5],
                                  ctx->needs_input_grad(0), saved[1].defined() && ctx->needs_input_grad(1));
@@ -213,6 +221,7 @@ struct AdjustLogits : torch::autograd::Function<AdjustLogits> {
     const variable_list saved = ctx->get_saved_variables();
     variable_list out(10);
     if (grads[0].defined()) {
+      no_tangent("adjust_logits' backward pass", grads[0]);
       const auto bias = ctx->saved_data.find("bias");
       std::vector<int64_t> shape;
       at::OptionalIntArrayRef sizes;
@@ -227,6 +236,7 @@ struct AdjustLogits : torch::autograd::Function<AdjustLogits> {
 
 Two loss_autograd(const Tensor& logits, const MaybeTensor& value, const Tensor& target, const MaybeTensor& reward,
                   const MaybeTensor& legal) {
+  no_tangent("policy_value_loss", logits, value, target, reward);
   if (!wanted(logits, value)) return loss_below(logits, value, target, reward, legal);
   const variable_list out = PolicyLoss::apply(logits, value, target, reward, legal);
   return {out[0], out[1]};
@@ -235,12 +245,14 @@ Two loss_autograd(const Tensor& logits, const MaybeTensor& value, const Tensor& 
 Three loss_grad_autograd(const Tensor& logits, const MaybeTensor& value, const Tensor& target, const MaybeTensor& reward,
                          const MaybeTensor& legal, double scale) {
   static const auto op = operator_of<decltype(loss_grad_gpu)>("mtaz::policy_loss_grad");
+  no_tangent("policy_value_loss_grad", logits, value, target, reward);
   const at::AutoDispatchBelowADInplaceOrView below;
   return op.call(logits, value, target, reward, legal, scale);
 }
 Tensor adjust_autograd(const Tensor& logits, const MaybeTensor& bias, const MaybeTensor& legal, const MaybeTensor& actions,
                        const MaybeTensor& lengths, const MaybeTensor& per_row, double repetition, double frequency,
                        double presence, bool bends) {
+  no_tangent("adjust_logits", logits, bias, per_row);
   if (!wanted(logits, bias))
     return adjust_below(logits, bias, legal, actions, lengths, per_row, repetition, frequency, presence, bends);
   return AdjustLogits::apply(logits, bias, legal, actions, lengths, per_row, repetition, frequency, presence, bends);

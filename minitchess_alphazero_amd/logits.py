@@ -9,13 +9,14 @@ A mask is packed 32 actions a word: action v is legal where bit v & 31 of word v
 [rows, ceil(cols / 32)], or [1, words] / [words] for one mask that all rows share.  Logits are float32,
 float16 or bfloat16, sums are float32, and the operators enqueue on the current stream without a
 synchronization; they may be captured in a HIP graph (a backward pass like any of torch's: with no eager graph of the
-same leaves alive).  There is no CPU form: tensors elsewhere are refused.
+same leaves alive).  There is no CPU form: tensors elsewhere are refused, and so are tensors that carry a tangent of
+forward-mode differentiation.
 """
 import torch
 
 from . import _lib
 from .environment import MOVE_CAP, RULES_FLAGS
-from .optim import TYPES, _check_type, _doubles, _stream
+from .optim import TYPES, _check_type, _doubles, _no_tangent, _stream
 
 
 def _ptr(t):
@@ -163,6 +164,7 @@ def adjust_logits(logits, legal=None, bias=None, actions=None, lengths=None, rep
         raise ValueError('out must have dense rows that do not overlap')
     if torch.is_grad_enabled() and out.requires_grad:
         raise ValueError('out must not require a gradient')
+    _no_tangent('adjust_logits', logits, bias, taken.tensors[2], out)
     _adjust(logits, legal, bias, taken, out)
     torch.autograd.graph.increment_version(out)
     return out

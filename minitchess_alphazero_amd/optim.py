@@ -17,6 +17,7 @@ import functools
 import math
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 
@@ -53,6 +54,15 @@ def _check_type(t, what):
         raise ValueError(f'{what} must be float32, float16 or bfloat16, not {t.dtype}')
 
 
+def _no_tangent(what, *tensors):
+    """Refuses tensors that carry a tangent (forward-mode differentiation): the result would have none, which says
+    that its derivative is 0."""
+    if getattr(forward_ad, '_current_level', 0) < 0:   # no dual level is open
+        return
+    if any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        raise ValueError(f'{what} has no forward-mode derivative')
+
+
 def _span(t):
     """The addresses of a contiguous tensor: (first, behind the last)."""
     at = t.data_ptr()
@@ -68,7 +78,7 @@ def orthogonalize(grad, steps=5, coefficients=COEFFICIENTS, eps=1e-7, out=None):
     """Each matrix of grad [..., rows, cols] (float32, float16 or bfloat16) divided by its Frobenius
     norm + eps and taken through `steps` Newton-Schulz steps over its shorter side.  The result has
     grad's type and shape; the products keep 32-bit accuracy whatever the type.  out: a contiguous tensor
-    for the result (grad itself is allowed).  There is no backward pass.
+    for the result (grad itself is allowed).  There is no backward pass and no forward-mode derivative.
 
     Accuracy is relative to the largest singular value: entries below 2^-38 of the norm are taken as 0."""
     _check_type(grad, 'grad')
@@ -76,6 +86,7 @@ def orthogonalize(grad, steps=5, coefficients=COEFFICIENTS, eps=1e-7, out=None):
         raise ValueError(f'grad must have at least two dimensions, got {tuple(grad.shape)}')
     if torch.is_grad_enabled() and grad.requires_grad:
         raise ValueError('orthogonalize has no backward pass: detach grad')
+    _no_tangent('orthogonalize', grad, out)
     if out is None:
         out = torch.empty(grad.shape, dtype=grad.dtype, device=grad.device)
     elif out.shape != grad.shape or out.dtype != grad.dtype or out.device != grad.device or not out.is_contiguous():
@@ -115,6 +126,7 @@ def muon_step(params, grads, momenta, *, lr, momentum=0.95, nesterov=True, weigh
     params, grads, momenta = list(params), list(grads), list(momenta)
     if not len(params) == len(grads) == len(momenta):
         raise ValueError(f'{len(params)} parameters, {len(grads)} gradients and {len(momenta)} momenta')
+    _no_tangent('muon_step', *params, *grads, *momenta)
     groups, written, read = {}, [], []
     for w, g, m in zip(params, grads, momenta):
         _check_type(w, 'a parameter')

@@ -1,6 +1,7 @@
 """GPU: the learner operators under what torch does with operators: tracing, streams, derivatives that they lack."""
 import pytest
 import torch
+from torch.autograd import forward_ad
 from torch.fx.experimental.proxy_tensor import make_fx
 
 from minitchess_alphazero_amd import logits as ops
@@ -41,3 +42,16 @@ def test_traced_graph_computes():
             got = graph(*[a * 1 for a in args])   # a wrong stream would read these before they are there
         side.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def test_tangents_are_refused_in_backward_too():
+    x, b, v, mask, actions, lengths, t = inputs(4)
+    y, loss = ops.adjust_logits(x.requires_grad_(), mask), ops.policy_value_loss(x, t)
+    with forward_ad.dual_level():
+        for out in (y, loss):
+            g = torch.ones_like(out)
+            with pytest.raises(ValueError, match='no forward-mode derivative'):
+                torch.autograd.grad(out, x, forward_ad.make_dual(g, g), retain_graph=True)
+        with pytest.raises(ValueError, match='no forward-mode derivative'):
+            ops.adjust_logits(forward_ad.make_dual(x.detach(), x.detach()))
+    torch.autograd.grad(loss, x)

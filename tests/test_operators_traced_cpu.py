@@ -2,10 +2,12 @@
 them), with the shapes, types and devices that they return."""
 import pytest
 import torch
+from torch.autograd import forward_ad
 from torch._subclasses.fake_tensor import FakeTensorMode
 from torch.fx.experimental.proxy_tensor import make_fx
 
 from minitchess_alphazero_amd import logits as ops
+from minitchess_alphazero_amd import optim
 
 
 def called(graph):
@@ -43,3 +45,26 @@ def test_shapes_without_data(fake):
     loss, dz, dv = ops.policy_value_loss_grad(z, t, v, v)
     assert (loss.shape, dz.shape, dz.dtype, dv.shape, dv.dtype) == ((), (5, 40), torch.bfloat16, (5, 1), torch.float32)
     assert ops.policy_value_loss_grad(z, t)[2] is None
+
+
+def test_tangents_are_refused(fake):
+    """No operator has a forward-mode derivative: a result without a tangent would say that it is 0."""
+    z, t, v, mask, actions = tensors(5, 40, torch.float32)
+    per_row = torch.ones(5, device='cuda')
+    with forward_ad.dual_level():
+        d, dv, dp = (forward_ad.make_dual(a, torch.ones_like(a)) for a in (z, v, per_row))
+        for call in (lambda: ops.adjust_logits(d), lambda: ops.adjust_logits(z, bias=forward_ad.make_dual(z[0].clone(), z[1])),
+                     lambda: ops.adjust_logits(z, actions=actions, repetition=dp), lambda: ops.adjust_logits(d, out=z),
+                     lambda: ops.adjust_logits(z, out=d), lambda: ops.policy_value_loss(d, t),
+                     lambda: ops.policy_value_loss(z, t, dv, v), lambda: ops.policy_value_loss(z, t, v, dv),
+                     lambda: ops.policy_value_loss(z, d), lambda: ops.policy_value_loss_grad(d, t),
+                     lambda: optim.orthogonalize(d), lambda: optim.orthogonalize(z, out=d),
+                     lambda: optim.muon_step([d], [z], [t], lr=0.1), lambda: optim.muon_step([z], [d], [t], lr=0.1),
+                     lambda: optim.muon_step([z], [t], [d], lr=0.1)):
+            with pytest.raises(ValueError, match='no forward-mode derivative'):
+                call()
+        for call in (lambda: ops.adjust_logits(d.clone().requires_grad_()), lambda: ops.policy_value_loss(d.clone().requires_grad_(), t)):
+            with pytest.raises(ValueError, match='no forward-mode derivative'):
+                call()
+        assert ops.policy_value_loss(z, t).shape == ()
+    assert ops.adjust_logits(z).shape == (5, 40)
