@@ -46,28 +46,35 @@ int64_t checked(int64_t rc) {
 void* stream_of(const Tensor& t) { return (void*)c10::hip::getCurrentHIPStream(t.get_device()).stream(); }
 
 // ---- the operators on the GPU -----------------------------------------------------------------------------------
-// The loss and the rows' statistics; with gradients of scale * loss where dz or dv is defined.
-Two loss_of(const Tensor& logits, const MaybeTensor& value, const Tensor& target, const MaybeTensor& reward,
-            const MaybeTensor& legal, const Tensor& dz, const Tensor& dv, double scale) {
+// The loss, with the rows' statistics where stats is, and with gradients of scale * loss where dz or dv is defined
+Tensor loss_of(const Tensor& logits, const MaybeTensor& value, const Tensor& target, const MaybeTensor& reward,
+               const MaybeTensor& legal, const Tensor& dz, const Tensor& dv, double scale, Tensor* stats) {
   const Tensor z = unit(logits), t = unit(target), mask = unit(or_none(legal)), v = dense(or_none(value)),
                r = dense(or_none(reward));
   const int64_t rows = z.size(0), cols = z.size(1), size = checked(mtaz_policy_loss_workspace(rows, cols));
   const auto floats = z.options().dtype(at::kFloat);
-  Tensor loss = at::empty({}, floats), stats = at::empty({rows, 4}, floats), work = at::empty({(size + 3) / 4}, floats);
+  const Tensor loss = at::empty({}, floats);
+  if (stats) *stats = at::empty({rows, 4}, floats);
+  // scratch memory, and the statistics behind it where nobody else wants them (on a boundary of 256 bytes)
+  const int64_t floats_each = (size + 255) / 256 * 64;
+  const Tensor work = at::empty({floats_each + (stats ? 0 : 4 * rows)}, floats);
+  float* const w = (float*)work.data_ptr();
   checked(mtaz_policy_loss(z.get_device(), rows, cols, type_of(z), type_of(t), at(z), z.stride(0), at(t), t.stride(0),
                            (const uint32_t*)at(mask), row_stride(mask), (const float*)at(v), (const float*)at(r),
-                           (float*)at(loss), (float*)at(stats), at(dz), cols, (float*)at(dv), scale, at(work), size,
-                           stream_of(z)));
-  return {loss, stats};
+                           (float*)at(loss), stats ? (float*)at(*stats) : w + floats_each, at(dz), cols, (float*)at(dv),
+                           scale, w, size, stream_of(z)));
+  return loss;
 }
 Two loss_gpu(const Tensor& logits, const MaybeTensor& value, const Tensor& target, const MaybeTensor& reward,
              const MaybeTensor& legal) {
-  return loss_of(logits, value, target, reward, legal, Tensor(), Tensor(), 1.);
+  Tensor stats;
+  const Tensor loss = loss_of(logits, value, target, reward, legal, Tensor(), Tensor(), 1., &stats);
+  return {loss, stats};
 }
 Three loss_grad_gpu(const Tensor& logits, const MaybeTensor& value, const Tensor& target, const MaybeTensor& reward,
                     const MaybeTensor& legal, double scale) {
   const Tensor dz = fresh(logits), dv = there(value) ? fresh(*value) : Tensor();
-  return {std::get<0>(loss_of(logits, value, target, reward, legal, dz, dv, scale)), dz, dv};
+  return {loss_of(logits, value, target, reward, legal, dz, dv, scale, nullptr), dz, dv};
 }
 Two loss_back_gpu(const Tensor& grad, const Tensor& logits, const MaybeTensor& value, const Tensor& target,
                   const MaybeTensor& reward, const MaybeTensor& legal, const Tensor& stats, bool want_z, bool want_v) {
@@ -182,13 +189,12 @@ variable_list once(variable_list grads) {
 }
 
 struct PolicyLoss : torch::autograd::Function<PolicyLoss> {
-  static variable_list forward(AutogradContext* ctx, const Tensor& logits, const MaybeTensor& value, const Tensor& target,
-                               const MaybeTensor& reward, const MaybeTensor& legal) {
-    const auto [loss, stats] = loss_below(logits, value, target, reward, legal);
-    ctx->save_for_backward({logits, or_none(value), target, or_none(reward), or_none(legal), stats});
-    ctx->mark_non_differentiable({stats});
-    ctx->set_materialize_grads(false);
-    return {loss, stats};
+  static Tensor forward(AutogradContext* ctx, const Tensor& logits, const MaybeTensor& value, const Tensor& target,
+                        const MaybeTensor& reward, const MaybeTensor& legal, Tensor* stats) {
+    Tensor loss;
+    std::tie(loss, *stats) = loss_below(logits, value, target, reward, legal);
+    ctx->save_for_backward({logits, or_none(value), target, or_none(reward), or_none(legal), *stats});
+    return loss;
   }
   static variable_list backward(AutogradContext* ctx, const variable_list& grads) {
     static const auto op = operator_of<decltype(loss_back_gpu)>("mtaz::policy_loss_back");
@@ -200,7 +206,7 @@ struct PolicyLoss : torch::autograd::Function<PolicyLoss> {
       std::tie(dz, dv) = op.call(grads[0], saved[0], saved[1], saved[2], saved[3], saved[4], saved[5],
                                  ctx->needs_input_grad(0), saved[1].defined() && ctx->needs_input_grad(1));
     }
-    return once({dz, dv, Tensor(), Tensor(), Tensor()});
+    return once({dz, dv, Tensor(), Tensor(), Tensor(), Tensor()});
   }
 };
 
@@ -238,8 +244,9 @@ Two loss_autograd(const Tensor& logits, const MaybeTensor& value, const Tensor& 
                   const MaybeTensor& legal) {
   no_tangent("policy_value_loss", logits, value, target, reward);
   if (!wanted(logits, value)) return loss_below(logits, value, target, reward, legal);
-  const variable_list out = PolicyLoss::apply(logits, value, target, reward, legal);
-  return {out[0], out[1]};
+  Tensor stats;
+  const Tensor loss = PolicyLoss::apply(logits, value, target, reward, legal, &stats);
+  return {loss, stats};
 }
 // cut off from the graph
 Three loss_grad_autograd(const Tensor& logits, const MaybeTensor& value, const Tensor& target, const MaybeTensor& reward,
