@@ -16,7 +16,7 @@ import torch
 
 from . import _lib
 from .environment import MOVE_CAP, RULES_FLAGS
-from .optim import TYPES, _check_type, _doubles, _no_tangent, _stream
+from .optim import TYPES, _check_type, _doubles, _no_tangent, _not_traced, _stream
 
 
 def _ptr(t):
@@ -70,6 +70,7 @@ def legal_masks(positions, device, rules_flags=RULES_FLAGS, move_cap=MOVE_CAP):
     mtaz_legal_batch finds (it waits for the stream, unlike the other functions here).  A position with no
     legal move has an empty mask."""
     import numpy as np
+    _not_traced('legal_masks')
     dev = torch.device(device)
     if not torch.is_tensor(positions):
         positions = torch.from_numpy(np.ascontiguousarray(positions, np.uint32).view(np.int32)).to(dev)
@@ -165,6 +166,7 @@ def adjust_logits(logits, legal=None, bias=None, actions=None, lengths=None, rep
     if torch.is_grad_enabled() and out.requires_grad:
         raise ValueError('out must not require a gradient')
     _no_tangent('adjust_logits', logits, bias, taken.tensors[2], out)
+    _not_traced('adjust_logits with out')
     _adjust(logits, legal, bias, taken, out)
     torch.autograd.graph.increment_version(out)
     return out

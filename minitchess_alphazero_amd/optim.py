@@ -9,7 +9,7 @@ the matrix [out, in * kh * kw].
     Muon(params, lr)                      the same as a torch.optim.Optimizer
 
 Every function enqueues on the current stream of its tensors' device, synchronizes nothing, and may be
-captured in a HIP graph.  There is no CPU form: tensors elsewhere are refused.
+captured in a HIP graph (not traced by make_fx: that is refused).  There is no CPU form: tensors elsewhere are refused.
 """
 import bisect
 import ctypes
@@ -18,6 +18,7 @@ import math
 
 import torch
 from torch.autograd import forward_ad
+from torch.fx.experimental.proxy_tensor import get_proxy_mode
 
 from . import _lib
 
@@ -63,6 +64,12 @@ def _no_tangent(what, *tensors):
         raise ValueError(f'{what} has no forward-mode derivative')
 
 
+def _not_traced(what):
+    """Refuses a call that a tracer (make_fx) would not record: it goes straight to the C entry."""
+    if torch._C._len_torch_dispatch_stack() and get_proxy_mode() is not None:
+        raise RuntimeError(f'{what} cannot be traced into a graph of torch operators')
+
+
 def _span(t):
     """The addresses of a contiguous tensor: (first, behind the last)."""
     at = t.data_ptr()
@@ -87,6 +94,7 @@ def orthogonalize(grad, steps=5, coefficients=COEFFICIENTS, eps=1e-7, out=None):
     if torch.is_grad_enabled() and grad.requires_grad:
         raise ValueError('orthogonalize has no backward pass: detach grad')
     _no_tangent('orthogonalize', grad, out)
+    _not_traced('orthogonalize')
     if out is None:
         out = torch.empty(grad.shape, dtype=grad.dtype, device=grad.device)
     elif out.shape != grad.shape or out.dtype != grad.dtype or out.device != grad.device or not out.is_contiguous():
@@ -127,6 +135,7 @@ def muon_step(params, grads, momenta, *, lr, momentum=0.95, nesterov=True, weigh
     if not len(params) == len(grads) == len(momenta):
         raise ValueError(f'{len(params)} parameters, {len(grads)} gradients and {len(momenta)} momenta')
     _no_tangent('muon_step', *params, *grads, *momenta)
+    _not_traced('muon_step')
     groups, written, read = {}, [], []
     for w, g, m in zip(params, grads, momenta):
         _check_type(w, 'a parameter')

@@ -68,3 +68,15 @@ def test_tangents_are_refused(fake):
                 call()
         assert ops.policy_value_loss(z, t).shape == ()
     assert ops.adjust_logits(z).shape == (5, 40)
+
+
+def test_calls_that_a_tracer_would_lose_are_refused(fake):
+    z, t, v, mask, actions = tensors(5, 40, torch.float32)
+    pos = torch.zeros(5, 5, dtype=torch.int32, device='cuda')
+
+    def step(z):
+        optim.muon_step([z], [t], [t.clone()], lr=0.1)
+        return z
+    for call in (lambda z: optim.orthogonalize(z), step, lambda z: ops.adjust_logits(z, out=z), lambda z: ops.legal_masks(pos, 'cuda')):
+        with pytest.raises(RuntimeError, match='cannot be traced'):
+            make_fx(call)(z)
