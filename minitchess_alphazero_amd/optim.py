@@ -175,7 +175,8 @@ def muon_step(params, grads, momenta, *, lr, momentum=0.95, nesterov=True, weigh
 class Muon(torch.optim.Optimizer):
     """muon_step as an optimizer.  Give it the weights that are matrices (hidden layers); embeddings,
     heads, biases and norms train better with AdamW (learner.muon_split divides a network).  The
-    momenta are float32 whatever the parameters' type, in the state as 'momentum_buffer'."""
+    momenta are float32 whatever the parameters' type, in the state as 'momentum_buffer'; the first step makes
+    them, so it is not one to capture in a graph.  A captured step keeps the lr and the other numbers of its capture."""
 
     def __init__(self, params, lr=0.02, momentum=0.95, nesterov=True, weight_decay=0.0, steps=5,
                  coefficients=COEFFICIENTS, eps=1e-7, scale=None):
@@ -198,6 +199,8 @@ class Muon(torch.optim.Optimizer):
             params = [p for p in group['params'] if p.grad is not None]
             for p in params:
                 if not self.state[p]:
+                    if torch.cuda.is_current_stream_capturing():   # a replay would set the momentum to 0 again
+                        raise RuntimeError('the first step of a parameter cannot be captured: run one before the capture')
                     self.state[p]['momentum_buffer'] = torch.zeros(p.shape, dtype=torch.float32, device=p.device)
             muon_step(params, [p.grad for p in params], [self.state[p]['momentum_buffer'] for p in params],
                       **{k: group[k] for k in ('lr', 'momentum', 'nesterov', 'weight_decay', 'steps', 'coefficients',
