@@ -120,8 +120,8 @@ class _Taken:
         actions = _unit(actions)
         per_row = None
         if tensors:
-            per_row = torch.stack([t if isinstance(t, torch.Tensor) else torch.full((rows,), float(t), device=logits.device)
-                                   for t in given], 1)
+            like = dict(dtype=torch.float32, device=logits.device)
+            per_row = torch.stack([t if isinstance(t, torch.Tensor) else torch.full((rows,), float(t), **like) for t in given], 1)
         self.tensors, self.bends = (actions, lengths, per_row), per_row_repetition or repetition != 1.0
 
 
