@@ -674,6 +674,17 @@ bool tangled(const Place& a, const Place& b, int64_t rows, bool same) {
   const int64_t off = ((b.at - a.at) % a.step + a.step) % a.step;   // from a row of a to the next of b
   return off < a.width || a.step - off < b.width;
 }
+// Whether an output lies over what is read for other places than the one that is written: a mask, or the actions taken,
+// their lengths and penalties
+bool over_inputs(const Place& out, int64_t rows, int64_t cols, const uint32_t* legal, int64_t legal_stride,
+                 const int32_t* actions = nullptr, int64_t actions_stride = 0, int history = 0,
+                 const int32_t* lengths = nullptr, const float* per_row = nullptr) {
+  auto over = [&](const void* p, int64_t stride, int64_t width) {
+    return tangled({p, stride, width, MTAZ_F32}, out, rows, false);
+  };
+  return over(legal, legal_stride, (cols + 31) / 32) ||
+         (actions && history && (over(actions, actions_stride, history) || over(lengths, 1, 1) || over(per_row, 3, 3)));
+}
 const char* bad_taken(const int32_t* actions, int64_t stride, int history, const double* penalties,
                       const float* per_row) {
   if (history < 0) return "history must not be negative";
@@ -737,6 +748,10 @@ extern "C" int mtaz_adjust_logits(int device, int64_t rows, int64_t cols, int dt
   if (!bad && out_stride < cols && rows > 1) bad = "rows of the output overlap";
   if (!bad && tangled({d_logits, logits_stride, cols, dtype}, {d_out, out_stride, cols, dtype}, rows, true))
     bad = "the output overlaps the logits and is not in place";
+  const Place to(d_out, out_stride, cols, dtype);
+  if (!bad && (over_inputs(to, rows, cols, d_legal, legal_stride, d_actions, actions_stride, history, d_lengths, d_penalties) ||
+               tangled({d_bias, bias_stride, cols, MTAZ_F32}, to, rows, true)))
+    bad = "the output overlaps the mask, the bias or the actions";
   if (bad) return ops_error(MTAZ_E_FAIL, "adjust_logits", bad);
   if (rows == 0) return 0;
   DeviceScope on(device);
@@ -793,6 +808,9 @@ extern "C" int mtaz_adjust_logits_grad(int device, int64_t rows, int64_t cols, i
     bad = "the gradient overlaps the incoming one (in place is allowed without penalties)";
   if (!bad && t.actions && tangled({d_logits, logits_stride, cols, dtype}, {d_grad, grad_stride, cols, dtype}, rows, false))
     bad = "the gradient overlaps the logits";
+  for (const Place& to : {Place(d_grad, grad_stride, cols, dtype), Place(d_bias_grad, bias_grad_stride, cols, MTAZ_F32)})
+    if (!bad && over_inputs(to, rows, cols, d_legal, legal_stride, d_actions, actions_stride, history, d_lengths, d_penalties))
+      bad = "a gradient overlaps the mask or the actions";
   if (bad) return ops_error(MTAZ_E_FAIL, what, bad);
   DeviceScope on(device);
   if (on.status != hipSuccess) return ops_error(MTAZ_E_DEVICE, what, hipGetErrorString(on.status));
@@ -840,9 +858,10 @@ static const char* bad_loss(int64_t rows, int64_t cols, int dtype, int target_dt
 }
 // A gradient over its own logits is written where a thread has read them; over the targets likewise.
 static const char* bad_place(int64_t rows, int64_t cols, int dtype, int target_dtype, const void* logits,
-                             int64_t logits_stride, const void* target, int64_t target_stride, const void* grad,
-                             int64_t grad_stride) {
+                             int64_t logits_stride, const void* target, int64_t target_stride, const uint32_t* legal,
+                             int64_t legal_stride, const void* grad, int64_t grad_stride) {
   const Place g(grad, grad_stride, cols, dtype);
+  if (over_inputs(g, rows, cols, legal, legal_stride)) return "the gradient overlaps the mask";
   if (tangled({logits, logits_stride, cols, dtype}, g, rows, true) ||
       tangled({target, target_stride, cols, target_dtype}, g, rows, true))
     return "the gradient overlaps the logits or the targets and is not in place";
@@ -860,7 +879,8 @@ extern "C" int mtaz_policy_loss(int device, int64_t rows, int64_t cols, int dtyp
                              grad_stride, d_value_grad);
   if (!bad && !d_loss) bad = "no place for the loss";
   if (!bad && (!d_work || work_bytes < loss_workspace(rows, cols))) bad = "workspace too small";
-  if (!bad) bad = bad_place(rows, cols, dtype, target_dtype, d_logits, logits_stride, d_target, target_stride, d_grad, grad_stride);
+  if (!bad) bad = bad_place(rows, cols, dtype, target_dtype, d_logits, logits_stride, d_target, target_stride, d_legal, legal_stride,
+                             d_grad, grad_stride);
   if (bad) return ops_error(MTAZ_E_FAIL, what, bad);
   DeviceScope on(device);
   if (on.status != hipSuccess) return ops_error(MTAZ_E_DEVICE, what, hipGetErrorString(on.status));
@@ -917,7 +937,8 @@ extern "C" int mtaz_policy_loss_grad(int device, int64_t rows, int64_t cols, int
   const char* bad = bad_loss(rows, cols, dtype, target_dtype, d_logits, d_target, d_value, d_reward, d_stats, d_grad,
                              grad_stride, d_value_grad);
   if (!bad && !d_grad_out) bad = "no incoming gradient";
-  if (!bad) bad = bad_place(rows, cols, dtype, target_dtype, d_logits, logits_stride, d_target, target_stride, d_grad, grad_stride);
+  if (!bad) bad = bad_place(rows, cols, dtype, target_dtype, d_logits, logits_stride, d_target, target_stride, d_legal, legal_stride,
+                             d_grad, grad_stride);
   if (bad) return ops_error(MTAZ_E_FAIL, what, bad);
   if (!d_grad && !d_value_grad) return 0;
   DeviceScope on(device);

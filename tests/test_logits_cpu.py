@@ -1,7 +1,10 @@
 """CPU: what the logits operators make of their arguments before they call a kernel."""
+import ctypes
+
 import pytest
 import torch
 
+from minitchess_alphazero_amd import _lib
 from minitchess_alphazero_amd import logits as ops
 
 
@@ -17,3 +20,37 @@ def test_penalties_are_float32_under_another_default_type():
             torch.set_default_dtype(before)
         assert taken.tensors[2].dtype == torch.float32
         assert torch.equal(taken.tensors[2], torch.tensor([[1.5, 0.25, 0.5]] * 2))
+
+
+BUF = ctypes.create_string_buffer(8192)
+P = (ctypes.addressof(BUF) + 255) // 256 * 256
+PEN = (ctypes.c_double * 3)(1.2, 0.1, 0.1)
+
+
+def refused(rc, why):
+    assert rc == _lib.E_FAIL
+    assert why in _lib.lib().mtaz_last_error().decode()
+
+
+# [2][40] float32 at P: 320 bytes
+@pytest.mark.parametrize('legal,bias,bias_stride,actions,lengths,per_row', [
+    (P + 316, None, 0, None, None, None),                       # its first word is the output's last element
+    (P + 1024, P, 0, None, None, None),                         # one bias for both rows, where the first row is written
+    (P + 1024, P, 41, None, None, None),
+    (P + 1024, P + 4, 40, None, None, None),
+    (None, None, 0, P + 304, None, None), (None, None, 0, P - 16, None, None), (None, None, 0, P + 1024, P + 160, None),
+    (None, None, 0, P + 1024, None, P + 300)])
+def test_output_over_what_other_rows_read_is_refused(legal, bias, bias_stride, actions, lengths, per_row):
+    L = _lib.lib()
+    refused(L.mtaz_adjust_logits(0, 2, 40, 0, P + 2048, 40, P, 40, legal, 2, bias, bias_stride, actions, 4, 4 if actions else 0,
+                                 lengths, PEN, per_row, None), 'overlaps the mask, the bias or the actions')
+    if bias is None:
+        for grads in ((P, 40, None, 0), (None, 0, P, 40), (None, 0, P, 0)):
+            hit = grads[3] != 0 or grads[0] is not None or (P <= (actions or 0) < P + 160)
+            if hit:
+                refused(L.mtaz_adjust_logits_grad(0, 2, 40, 0, P + 2048, 40, P + 3072, 40, *grads, legal, 2, actions, 4,
+                                                  4 if actions else 0, lengths, PEN, per_row, P + 4096, 1024, None),
+                        'overlaps the mask or the actions')
+    if legal is not None and bias is None:
+        refused(L.mtaz_policy_loss(0, 2, 40, 0, 0, P + 2048, 40, P + 3072, 40, legal, 2, None, None, P + 4096, P + 4352, P, 40,
+                                   None, 1.0, P + 4608, 256, None), 'overlaps the mask')
