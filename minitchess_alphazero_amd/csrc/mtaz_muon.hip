@@ -55,7 +55,7 @@ struct Shape {
   int parts;                  // workgroups for the sum of squares
 };
 struct Update {
-  float momentum, keep, step;   // m <- momentum m + (1 - momentum) g;  w <- keep w - step O
+  float momentum, fresh, keep, step;   // m <- momentum m + fresh g, fresh = 1 - momentum;  w <- keep w - step O
   int nesterov;
 };
 // n matrices of pairs, one after the other
@@ -72,7 +72,7 @@ struct Pairs {
 // ---- the matrix to orthogonalise: sum of squares, then the pairs of X -----------------------------------------
 template <int DT, bool MUON>
 __device__ __forceinline__ float update_of(float g, float m, const Update& u) {
-  return MUON ? (u.nesterov ? fmaf(u.momentum, m, (1.f - u.momentum) * g) : m) : g;
+  return MUON ? (u.nesterov ? fmaf(u.momentum, m, u.fresh * g) : m) : g;
 }
 
 // Partial sums of squares in 64 bits: neither large nor tiny gradients leave the range.  With momentum, the
@@ -101,7 +101,7 @@ __global__ __launch_bounds__(NT) void k_squares(Matrices ms, int64_t count, Upda
 #pragma unroll
     for (int j = 0; j < N; ++j) {
       const float x = E::get(gv.v[j]);
-      if (MUON) mv.v[j] = fmaf(u.momentum, mv.v[j], (1.f - u.momentum) * x);
+      if (MUON) mv.v[j] = fmaf(u.momentum, mv.v[j], u.fresh * x);
       const double y = (double)update_of<DT, MUON>(x, mv.v[j], u);
       s = fma(y, y, s);
     }
@@ -649,7 +649,7 @@ __global__ __launch_bounds__(64 * SMALL_WAVES) void k_small(Matrices ms, Shape s
       const float x = E::get(gv[c].v[j]);
       float m = mv[c].v[j];
       if (MUON) {
-        m = fmaf(u.momentum, m, (1.f - u.momentum) * x);
+        m = fmaf(u.momentum, m, u.fresh * x);
         if (j < n) mom[k + j] = m;
       }
       mv[c].v[j] = update_of<DT, MUON>(x, m, u);
@@ -1057,7 +1057,7 @@ extern "C" int mtaz_muon_step(int device, int n, int64_t rows, int64_t cols, int
   if (!(momentum >= 0. && momentum < 1.)) return ops_error(MTAZ_E_FAIL, "muon_step", "momentum must be in [0, 1)");
   if (!isfinite(lr) || !isfinite(weight_decay) || !isfinite(scale))
     return ops_error(MTAZ_E_FAIL, "muon_step", "lr, weight_decay and scale must be finite");
-  const Update u = {(float)momentum, (float)(1. - lr * weight_decay), (float)(lr * scale), nesterov};
+  const Update u = {(float)momentum, (float)(1. - momentum), (float)(1. - lr * weight_decay), (float)(lr * scale), nesterov};
   return run<true>("muon_step", device, n, rows, cols, dtype, d_grads, d_params, d_momenta, u, steps, coefficients,
                    eps, d_work, work_bytes, stream);
 }

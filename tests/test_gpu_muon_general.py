@@ -76,3 +76,15 @@ def test_small_singular_values(kind, shape, dtype):
     g = left @ randn(rank, shape[1], seed=2)
     g = (g + 1e-2 * randn(*shape, seed=4) if rank == 5 else g).to(dtype)
     assert off(optim.orthogonalize(g), reference(g)) <= LOOSE + HALF[dtype]
+
+
+@pytest.mark.parametrize('momentum', [0.9, 0.95, 0.999, 0.9999])
+@pytest.mark.parametrize('shape', [(20, 60), (256, 2304)], ids=str)
+def test_share_of_the_gradient_is_rounded_once(shape, momentum):
+    """1 - momentum is taken in 64 bits: a momentum that starts at 0 is that share of the gradient, the share rounded to
+    float and the product once more."""
+    for nesterov in (True, False):
+        w, g, m = randn(*shape, seed=1), randn(*shape, seed=2), torch.zeros(*shape, device='cuda')
+        optim.muon_step([w], [g], [m], lr=0.1, momentum=momentum, nesterov=nesterov)
+        want = (1 - momentum) * g.double()
+        assert bool(((m.double() - want).abs() <= 2.0 * 2.0 ** -24 * want.abs() * (1 + 2.0 ** -20)).all())
