@@ -142,8 +142,9 @@ int mtaz_adjust_logits(int device, int64_t rows, int64_t cols, int dtype, const 
                        void* stream);
 /* Its backward pass: d_grad (NULL: not wanted) = d y / d x of the logits times d_grad_out, 0 where
  * not legal; d_bias_grad (NULL: not wanted) float32, per row, or summed over the rows in a fixed order
- * when bias_grad_stride is 0.  d_logits is read only where a repetition penalty applies.
- * d_grad may be d_grad_out (same stride) where no penalty applies. */
+ * when bias_grad_stride is 0.  d_logits is read only where a repetition penalty applies (one other
+ * than 1, or one per row); it may be NULL where none does.
+ * d_grad may be d_grad_out (same stride) where none does. */
 int64_t mtaz_adjust_logits_grad_workspace(int64_t rows, int64_t cols);
 int mtaz_adjust_logits_grad(int device, int64_t rows, int64_t cols, int dtype, const void* d_grad_out,
                             int64_t grad_out_stride, const void* d_logits, int64_t logits_stride, void* d_grad,

@@ -796,7 +796,9 @@ extern "C" int mtaz_adjust_logits_grad(int device, int64_t rows, int64_t cols, i
   const char* what = "adjust_logits_grad";
   const char* bad = bad_shape(rows, cols, dtype);
   if (!bad) bad = bad_taken(d_actions, actions_stride, history, penalties, d_penalties);
-  const Taken t = bad ? Taken{} : taken_of(d_actions, actions_stride, history, d_lengths, penalties, d_penalties);
+  // the frequency and presence penalties are constants: without a repetition penalty the slope is 1 everywhere
+  const bool bends = !bad && (d_penalties || (penalties && penalties[0] != 1.));
+  const Taken t = bends ? taken_of(d_actions, actions_stride, history, d_lengths, penalties, d_penalties) : Taken{};
   const bool shared = d_bias_grad && bias_grad_stride == 0;
   if (!bad && rows && !d_grad_out) bad = "no incoming gradient";
   if (!bad && rows && t.actions && d_grad && !d_logits) bad = "the penalties' gradient needs the logits";
@@ -805,7 +807,7 @@ extern "C" int mtaz_adjust_logits_grad(int device, int64_t rows, int64_t cols, i
     bad = "rows of an output overlap";
   if (!bad && shared && rows && (!d_work || work_bytes < 4 * cols * bias_chunks(rows, cols))) bad = "workspace too small";
   if (!bad && tangled({d_grad_out, grad_out_stride, cols, dtype}, {d_grad, grad_stride, cols, dtype}, rows, !t.actions))
-    bad = "the gradient overlaps the incoming one (in place is allowed without penalties)";
+    bad = "the gradient overlaps the incoming one (in place is allowed without a repetition penalty)";
   if (!bad && t.actions && tangled({d_logits, logits_stride, cols, dtype}, {d_grad, grad_stride, cols, dtype}, rows, false))
     bad = "the gradient overlaps the logits";
   for (const Place& to : {Place(d_grad, grad_stride, cols, dtype), Place(d_bias_grad, bias_grad_stride, cols, MTAZ_F32)})

@@ -5,6 +5,7 @@ log2(e), and by 2 * 2^-24 for exp.  A row's sum has up to 64 own terms of a thre
 after the other; rows in tiles join these over up to 6 levels and as many steps as a lane has tiles (2 below), and each
 join moves a sum by exp(-d) (off by (d + 2) 2^-24; all the d of a path together are at most the spread) and adds d pi to
 the dot product: in all less than (4 spread + 160) 2^-24 of the sum of magnitudes.  A 16-bit gradient is rounded once."""
+import ctypes
 import math
 
 import pytest
@@ -90,3 +91,18 @@ def test_outputs_over_their_inputs():
     words = place[:rows * mask.shape[1]].view(rows, -1)
     with pytest.raises(_lib.MtazError, match='overlaps the mask'):
         ops.adjust_logits(x, words, out=place.view(torch.float32).view(rows, cols))
+
+
+def test_gradient_without_a_repetition_penalty_needs_no_logits():
+    """Frequency and presence are constants: d x = d y where legal, also over the incoming gradient itself."""
+    rows, cols = 3, 70
+    _, legal, actions, _ = make(rows, cols, 6, 1, density=0.7)
+    dy = torch.randn(rows, cols, generator=gen(1)).cuda()
+    want = dy * legal.cuda()
+    mask, actions = pack(legal).cuda(), actions.cuda()
+    host = (ctypes.c_double * 3)(1.0, 0.25, 0.5)
+    for dx in (torch.empty_like(dy), dy):
+        _lib.check(_lib.lib().mtaz_adjust_logits_grad(
+            0, rows, cols, 0, dy.data_ptr(), cols, None, 0, dx.data_ptr(), cols, None, 0, mask.data_ptr(), mask.stride(0),
+            actions.data_ptr(), 6, 6, None, host, None, None, 0, torch.cuda.current_stream().cuda_stream))
+        assert torch.equal(dx, want)
