@@ -708,6 +708,9 @@ constexpr int BLOCK_COLS = 32768;
 int64_t loss_workspace(int64_t rows, int64_t cols) {
   return cols <= BLOCK_COLS ? 256 : (int64_t)sizeof(Soft) * rows * tiles_of(cols, LOSS_TILE<MTAZ_F32>);
 }
+const char* bad_work(const void* work, int64_t bytes, int64_t needed) {
+  return !work || ((uintptr_t)work & 255) || bytes < needed ? "workspace too small or not aligned to 256 bytes" : nullptr;
+}
 int launched(const char* what) {
   const hipError_t e = hipGetLastError();
   return e == hipSuccess ? 0 : ops_error(MTAZ_E_DEVICE, what, hipGetErrorString(e));
@@ -805,7 +808,7 @@ extern "C" int mtaz_adjust_logits_grad(int device, int64_t rows, int64_t cols, i
   if (!bad && rows * ((history + 63) / 64) >= 1 << 26) bad = "too many rows for one call";
   if (!bad && rows > 1 && ((d_grad && grad_stride < cols) || (d_bias_grad && !shared && bias_grad_stride < cols)))
     bad = "rows of an output overlap";
-  if (!bad && shared && rows && (!d_work || work_bytes < 4 * cols * bias_chunks(rows, cols))) bad = "workspace too small";
+  if (!bad && shared && rows) bad = bad_work(d_work, work_bytes, 4 * cols * bias_chunks(rows, cols));
   if (!bad && tangled({d_grad_out, grad_out_stride, cols, dtype}, {d_grad, grad_stride, cols, dtype}, rows, !t.actions))
     bad = "the gradient overlaps the incoming one (in place is allowed without a repetition penalty)";
   if (!bad && t.actions && tangled({d_logits, logits_stride, cols, dtype}, {d_grad, grad_stride, cols, dtype}, rows, false))
@@ -880,7 +883,7 @@ extern "C" int mtaz_policy_loss(int device, int64_t rows, int64_t cols, int dtyp
   const char* bad = bad_loss(rows, cols, dtype, target_dtype, d_logits, d_target, d_value, d_reward, d_stats, d_grad,
                              grad_stride, d_value_grad);
   if (!bad && !d_loss) bad = "no place for the loss";
-  if (!bad && (!d_work || work_bytes < loss_workspace(rows, cols))) bad = "workspace too small";
+  if (!bad) bad = bad_work(d_work, work_bytes, loss_workspace(rows, cols));
   if (!bad) bad = bad_place(rows, cols, dtype, target_dtype, d_logits, logits_stride, d_target, target_stride, d_legal, legal_stride,
                              d_grad, grad_stride);
   if (bad) return ops_error(MTAZ_E_FAIL, what, bad);

@@ -54,3 +54,12 @@ def test_output_over_what_other_rows_read_is_refused(legal, bias, bias_stride, a
     if legal is not None and bias is None:
         refused(L.mtaz_policy_loss(0, 2, 40, 0, 0, P + 2048, 40, P + 3072, 40, legal, 2, None, None, P + 4096, P + 4352, P, 40,
                                    None, 1.0, P + 4608, 256, None), 'overlaps the mask')
+
+
+def test_workspaces_off_their_boundary_are_refused():
+    L = _lib.lib()
+    for off in (4, 16, 128):
+        refused(L.mtaz_policy_loss(0, 2, 40, 0, 0, P, 40, P + 1024, 40, None, 0, None, None, P + 2048, P + 2304, None, 0, None, 1.0,
+                                   P + 4096 + off, 1024, None), 'aligned')
+        refused(L.mtaz_adjust_logits_grad(0, 2, 40, 0, P, 40, None, 0, P + 1024, 40, P + 2048, 0, None, 0, None, 0, 0, None, None,
+                                          None, P + 4096 + off, 1024, None), 'aligned')
