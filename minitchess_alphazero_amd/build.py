@@ -126,9 +126,15 @@ def _torch_dir():
     return list(importlib.util.find_spec('torch').submodule_search_locations)[0]
 
 
+AUTOGRAD_FLAGS = ['-shared', '-fPIC', '-std=c++17', '-O2', '-Wall', '-D__HIP_PLATFORM_AMD__']
+AUTOGRAD_LIBS = ['-ltorch', '-ltorch_cpu', '-lc10', '-lc10_hip', '-lmtaz', '-Wl,-rpath,$ORIGIN']
+AUTOGRAD_MARK = b'mtaz-autograd-sha256='
+
+
 def autograd_hash():
-    """sha256 over what libmtaz_autograd.so is built from: its source, include/mtaz.h and torch's version."""
-    h = hashlib.sha256()
+    """sha256 over what libmtaz_autograd.so is built from: its source, include/mtaz.h, torch's version and the compile
+    command (without the folders, which may differ where the library is only loaded)."""
+    h = hashlib.sha256(repr((AUTOGRAD_FLAGS, AUTOGRAD_LIBS)).encode())
     for path in (os.path.join(CSRC, 'mtaz_autograd.cpp'), os.path.join(INCLUDE, 'mtaz.h'),
                  os.path.join(_torch_dir(), 'version.py')):
         with open(path, 'rb') as f:
@@ -137,16 +143,15 @@ def autograd_hash():
 
 
 def build_autograd(force=False, verbose=True):
-    if not force and embedded_hash(OUT_AUTOGRAD, b'mtaz-autograd-sha256=') == autograd_hash():
+    if not force and embedded_hash(OUT_AUTOGRAD, AUTOGRAD_MARK) == autograd_hash():
         return OUT_AUTOGRAD
     torch_dir, tmp = _torch_dir(), OUT_AUTOGRAD + '.tmp'
-    cmd = ['g++', '-shared', '-fPIC', '-std=c++17', '-O2', '-Wall', '-D__HIP_PLATFORM_AMD__',
-           f'-DMTAZ_AUTOGRAD_SHA256="mtaz-autograd-sha256={autograd_hash()}"', f'-I{INCLUDE}',
-           '-isystem', os.path.join(torch_dir, 'include'),
-           '-isystem', os.path.join(torch_dir, 'include', 'torch', 'csrc', 'api', 'include'),
-           '-isystem', os.path.join(_rocm(), 'include'),
-           os.path.join(CSRC, 'mtaz_autograd.cpp'), '-o', tmp, '-L' + os.path.join(torch_dir, 'lib'), '-ltorch',
-           '-ltorch_cpu', '-lc10', '-lc10_hip', '-L' + HERE, '-lmtaz', '-Wl,-rpath,$ORIGIN']
+    cmd = ['g++'] + AUTOGRAD_FLAGS + [
+        f'-DMTAZ_AUTOGRAD_SHA256="{AUTOGRAD_MARK.decode()}{autograd_hash()}"', f'-I{INCLUDE}',
+        '-isystem', os.path.join(torch_dir, 'include'),
+        '-isystem', os.path.join(torch_dir, 'include', 'torch', 'csrc', 'api', 'include'),
+        '-isystem', os.path.join(_rocm(), 'include'), os.path.join(CSRC, 'mtaz_autograd.cpp'), '-o', tmp,
+        '-L' + os.path.join(torch_dir, 'lib'), '-L' + HERE] + AUTOGRAD_LIBS
     if verbose:
         print(' '.join(cmd), flush=True)
     subprocess.check_call(cmd)

@@ -17,6 +17,9 @@
 
 #include "mtaz.h"
 
+// In one piece in the library, where build.py looks for it: what only a function returns, the compiler may store in parts.
+extern "C" const char mtaz_autograd_built_from[] = MTAZ_AUTOGRAD_SHA256;
+
 namespace {
 
 using at::Tensor;
@@ -264,7 +267,7 @@ Tensor adjust_autograd(const Tensor& logits, const MaybeTensor& bias, const Mayb
     return adjust_below(logits, bias, legal, actions, lengths, per_row, repetition, frequency, presence, bends);
   return AdjustLogits::apply(logits, bias, legal, actions, lengths, per_row, repetition, frequency, presence, bends);
 }
-std::string built_from() { return MTAZ_AUTOGRAD_SHA256; }
+std::string built_from() { return mtaz_autograd_built_from; }
 
 }  // namespace
 

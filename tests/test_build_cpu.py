@@ -51,3 +51,20 @@ def test_traffic_stays_attached_while_only_operators_change(tree):
     traffic, why = bench.traffic_of(path, build.engine_hash(), 4096, 64, 'k_net_y (fused)')
     assert traffic is None and why.startswith('stale')
     assert bench.traffic_of(os.path.join(str(tree), 'none.json'), '', 4096, 64, 'k_net_y')[0] is None
+
+
+def test_built_libraries_are_not_built_again(monkeypatch):
+    """Both libraries carry the fingerprint of what they are built from where it is looked for."""
+    assert build.embedded_hash(build.OUT_AUTOGRAD, b'mtaz-autograd-sha256=') == build.autograd_hash()
+
+    def command(*args, **kwargs):
+        raise AssertionError(f'a compiler was called: {args}')
+    monkeypatch.setattr(build.subprocess, 'check_call', command)
+    monkeypatch.setattr(build.subprocess, 'Popen', command)
+    assert build.build(verbose=False) == build.OUT
+
+
+def test_autograd_hash_covers_the_compile_command(monkeypatch):
+    first = build.autograd_hash()
+    monkeypatch.setattr(build, 'AUTOGRAD_FLAGS', build.AUTOGRAD_FLAGS + ['-DX'])
+    assert build.autograd_hash() != first
