@@ -52,6 +52,9 @@ SOURCES = [
     ('mtaz_host.cpp', ['-O2', '-ffp-contract=off', '-fno-fast-math']),
     ('mtaz_wire.cpp', ['-O2']),
 ]
+# One name whatever the file is called: where MTAZ_LIB names another build of the library, libmtaz_autograd.so (which asks
+# for libmtaz.so) then finds the one that is loaded, and no second one beside it comes in.
+LINK_FLAGS = ['-lpthread', '-Wl,-soname,libmtaz.so']
 HEADERS = ['rules.h', 'engine.h', 'ops.h', 'net_common.h', 'glibc_math.h', 'glibc_math_tables.h']
 
 
@@ -73,7 +76,7 @@ def source_hash():
                 h.update(f.read())
     with open(os.path.join(INCLUDE, 'mtaz.h'), 'rb') as f:
         h.update(b'include/mtaz.h\0' + f.read())
-    h.update(repr((SOURCES, ARCH)).encode())
+    h.update(repr((SOURCES, ARCH, LINK_FLAGS)).encode())
     return h.hexdigest()
 
 
@@ -212,7 +215,7 @@ def build(force=False, verbose=True, diag=False):
         with open(obj + '.key', 'w') as f:
             f.write(key)
     tmp = out + '.tmp'
-    cmd = [hipcc, '-shared', f'--offload-arch={ARCH}', '-o', tmp] + objs + ['-lpthread']
+    cmd = [hipcc, '-shared', f'--offload-arch={ARCH}', '-o', tmp] + objs + LINK_FLAGS
     if verbose:
         print(' '.join(cmd), flush=True)
     subprocess.check_call(cmd)

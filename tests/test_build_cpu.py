@@ -2,10 +2,13 @@
 import json
 import os
 import shutil
+import subprocess
+import sys
 
 import pytest
 
 import bench
+from conftest import REPO
 from minitchess_alphazero_amd import build
 
 
@@ -68,3 +71,15 @@ def test_autograd_hash_covers_the_compile_command(monkeypatch):
     first = build.autograd_hash()
     monkeypatch.setattr(build, 'AUTOGRAD_FLAGS', build.AUTOGRAD_FLAGS + ['-DX'])
     assert build.autograd_hash() != first
+
+
+def test_another_library_is_the_only_one_loaded(tmp_path):
+    """MTAZ_LIB names another file: the operators of libmtaz_autograd.so call that one too."""
+    other = tmp_path / 'another_build.so'
+    shutil.copy(build.OUT, other)
+    code = ('from minitchess_alphazero_amd import _lib\n'
+            '_lib.nodes()\n'
+            'print(sorted({l.split()[-1] for l in open("/proc/self/maps") if "libmtaz.so" in l or "another_build" in l}))')
+    out = subprocess.run([sys.executable, '-c', code], env={**os.environ, 'MTAZ_LIB': str(other)}, cwd=REPO, check=True,
+                         capture_output=True, text=True).stdout
+    assert out.strip().splitlines()[-1] == str([str(other)])

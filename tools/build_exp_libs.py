@@ -46,7 +46,7 @@ def main():
             raise SystemExit('hipcc failed')
     for name, obj in nets.items():
         out = os.path.join(B.HERE, f'libmtaz_{name}.so')
-        subprocess.check_call([hipcc, '-shared', f'--offload-arch={B.ARCH}', '-o', out, obj] + shared + ['-lpthread'])
+        subprocess.check_call([hipcc, '-shared', f'--offload-arch={B.ARCH}', '-o', out, obj] + shared + B.LINK_FLAGS)
         print('built', out)
 
 
