@@ -126,7 +126,7 @@ class _Taken:
 
 
 def _adjust(x, legal, bias, taken, out):
-    x, legal, bias = _unit(x), _unit(legal), _unit(bias)
+    x, legal, bias = _unit(x.resolve_neg()), _unit(legal), _unit(bias if bias is None else bias.resolve_neg())
     rows, cols = x.shape
     actions, lengths, per_row = taken.tensors
     stride, history = (0, 0) if actions is None else (actions.stride(0), actions.shape[1])
@@ -163,6 +163,8 @@ def adjust_logits(logits, legal=None, bias=None, actions=None, lengths=None, rep
         raise ValueError('out must have the shape, type and device of logits')
     if (cols > 1 and out.stride(1) != 1) or (rows > 1 and out.stride(0) < cols):
         raise ValueError('out must have dense rows that do not overlap')
+    if out.is_neg():
+        raise ValueError('out must not be a negated view')
     if torch.is_grad_enabled() and out.requires_grad:
         raise ValueError('out must not require a gradient')
     _no_tangent('adjust_logits', logits, bias, taken.tensors[2], out)

@@ -99,11 +99,13 @@ def orthogonalize(grad, steps=5, coefficients=COEFFICIENTS, eps=1e-7, out=None):
         out = torch.empty(grad.shape, dtype=grad.dtype, device=grad.device)
     elif out.shape != grad.shape or out.dtype != grad.dtype or out.device != grad.device or not out.is_contiguous():
         raise ValueError('out must be contiguous and have the shape, type and device of grad')
+    elif out.is_neg():
+        raise ValueError('out must not be a negated view')
     elif torch.is_grad_enabled() and out.requires_grad:
         raise ValueError('out must not require a gradient')
     rows, cols = grad.shape[-2:]
     n = math.prod(grad.shape[:-2])
-    src = grad.detach().contiguous()
+    src = grad.detach().resolve_neg().contiguous()   # as it is: torch may hold a negated view of other numbers
     (a, b), (c, d) = _span(src), _span(out)
     if a != c and a < d and c < b:
         raise ValueError('out overlaps grad and is not grad')
@@ -147,7 +149,9 @@ def muon_step(params, grads, momenta, *, lr, momentum=0.95, nesterov=True, weigh
             raise ValueError('a momentum must be float32 and have its parameter\'s shape and device')
         if not (w.is_contiguous() and m.is_contiguous()):
             raise ValueError('parameters and momenta must be contiguous')
-        g = g.contiguous()
+        if w.is_neg() or m.is_neg():
+            raise ValueError('parameters and momenta must not be negated views')
+        g = g.resolve_neg().contiguous()
         written += _span(w), _span(m)
         if _span(g) != _span(w):   # a gradient in its own parameter's place has been read when that is written
             read.append(_span(g))

@@ -5,6 +5,7 @@ from torch.autograd import forward_ad
 from torch.fx.experimental.proxy_tensor import make_fx
 
 from minitchess_alphazero_amd import logits as ops
+from minitchess_alphazero_amd import optim
 from test_gpu_logits import gen, make, pack
 
 pytestmark = pytest.mark.gpu
@@ -55,3 +56,31 @@ def test_tangents_are_refused_in_backward_too():
         with pytest.raises(ValueError, match='no forward-mode derivative'):
             ops.adjust_logits(forward_ad.make_dual(x.detach(), x.detach()))
     torch.autograd.grad(loss, x)
+
+
+def test_negated_views_are_the_numbers_they_show():
+    """torch holds the imaginary part of a conjugate as a view that is negated when it is read."""
+    def negated(*shape, seed):
+        c = torch.randn(*shape, dtype=torch.complex64, generator=gen(seed)).cuda().conj()
+        view = torch._neg_view(c.imag.neg().clone())      # contiguous, so that no copy resolves it on the way
+        assert view.is_neg() and c.imag.is_neg() and torch.equal(view, c.imag)
+        return view
+    x, b = negated(6, 40, seed=1), negated(40, seed=2)
+    t = torch.rand(6, 40, generator=gen(3)).cuda()
+    plain = [a.clone() for a in (x, b)]
+    want = ops.adjust_logits(plain[0], bias=plain[1])
+    assert torch.equal(ops.adjust_logits(x, bias=b), want)
+    assert torch.equal(ops.adjust_logits(x, bias=b, out=torch.empty_like(want)), want)
+    for got, w in zip(ops.policy_value_loss_grad(x, t)[:2], ops.policy_value_loss_grad(plain[0], t)):
+        assert torch.equal(got, w)
+    assert torch.equal(optim.orthogonalize(x), optim.orthogonalize(plain[0]))
+    ws, ms = [t.clone() for _ in range(2)], [torch.zeros_like(t) for _ in range(2)]
+    optim.muon_step(ws, [x, plain[0]], ms, lr=0.1)
+    assert torch.equal(ws[0], ws[1]) and torch.equal(ms[0], ms[1])
+    with pytest.raises(ValueError, match='negated'):
+        ops.adjust_logits(t, out=x)
+    with pytest.raises(ValueError, match='negated'):
+        optim.orthogonalize(t, out=x)
+    for w, m in ((x, t), (t, x)):
+        with pytest.raises(ValueError, match='negated'):
+            optim.muon_step([w], [t.clone()], [m], lr=0.1)
