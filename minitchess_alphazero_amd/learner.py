@@ -69,6 +69,12 @@ def dense_pi(rows):
     return out
 
 
+def _lists_of(rows):
+    """The rows' legal lists: (lengths, codes one list after the other)."""
+    lists = [np.asarray(r['legal_moves'], np.int64) for r in rows]
+    return np.asarray([len(v) for v in lists], np.int64), np.concatenate(lists) if lists else np.zeros(0, np.int64)
+
+
 def collate_fn(batch):
     """exp/learner.py:23-41: (pi [B,554] f32, tokens [B,2,6,5] i64, clock [B,1] f32, reward [B,1] f32)."""
     toks, clocks = [], []
@@ -95,31 +101,46 @@ def encode_positions(pos, device):
     return tok.long().reshape(n, 2, 6, 5), clk.reshape(n, 1)
 
 
-def _masks_of(pos, device):
-    """Packed legal masks [n, 18] int32 of packed positions (host or device)."""
-    from .logits import legal_masks
-    return legal_masks(pos, device)
+def _masks_of(k, codes):
+    """Packed masks [n, 18] int32 of the rows' own legal lists: k [n] lengths, codes the lists one after the other (a code
+    may repeat).  They are the moves that the row's targets are over, whatever rules its games followed."""
+    n, dev, words = k.shape[0], k.device, (NUM_ACTIONS + 31) // 32
+    out = torch.zeros((n, words), dtype=torch.int32, device=dev)
+    row = torch.repeat_interleave(torch.arange(n, device=dev), k.long())
+    bit = torch.arange(32, device=dev)
+    first = torch.cumsum(k.long(), 0) - k.long()
+    for a in range(0, n, 1 << 15):                     # 19 MB of truth values at a time
+        b = min(n, a + (1 << 15))
+        e0, e1 = int(first[a]), int(first[b]) if b < n else row.shape[0]
+        legal = torch.zeros((b - a, words * 32), dtype=torch.bool, device=dev)
+        legal[row[e0:e1] - a, codes[e0:e1].long()] = True
+        out[a:b] = (legal.view(b - a, words, 32).long() << bit).sum(-1).to(torch.int32)   # the low 32 bits
+    return out
 
 
 class ResidentBatches:
-    """A dataset encoded once and kept on the device; batches are index gathers.  legal_masks (GPU
-    only): keep the positions' packed legal masks too."""
+    """A dataset encoded once and kept on the device; batches are index gathers.  legal_masks:
+    keep the packed masks of the rows' legal lists too."""
 
     def __init__(self, rows, device, legal_masks=False):
         self.device = torch.device(device)
         if isinstance(rows, EpisodeRecords):
             pos, pi, reward = rows.pos, rows.pi_dense(), rows.reward
+            k, codes = rows.k, rows.codes
         else:
             pos = np.stack([pos_from_fen(r['observation']) for r in rows]) if rows else np.zeros((0, 5), np.uint32)
             pi = dense_pi(rows)
             reward = np.asarray([float(r['reward']) for r in rows], np.float32)
+            k, codes = _lists_of(rows)
         if self.device.type == 'cuda':
             self.tokens, self.clock = encode_positions(pos, self.device)
         else:   # host encoder (CPU tests; the product learner runs on the GPU)
             enc = [pos_encode(p) for p in pos]
             self.tokens = torch.from_numpy(np.stack([t for t, _ in enc])).reshape(-1, 2, 6, 5)
             self.clock = torch.tensor(np.asarray([c for _, c in enc], np.float32)).reshape(-1, 1)
-        self.legal = _masks_of(pos, self.device) if legal_masks else None
+        self.legal = None
+        if legal_masks:
+            self.legal = _masks_of(*(torch.from_numpy(a.astype(np.int64)).to(self.device) for a in (k, codes)))
         self.pi = torch.from_numpy(pi).to(self.device)
         self.reward = torch.from_numpy(np.ascontiguousarray(reward, np.float32)).reshape(-1, 1).to(self.device)
 
@@ -153,7 +174,7 @@ class ReplayBuffer:
     ROW_BYTES = 60 + 4 + 4 * NUM_ACTIONS + 4
 
     def __init__(self, max_length, device, initial=1 << 16, legal_masks=False):
-        """legal_masks: keep each row's packed legal mask as well (72 B a row)."""
+        """legal_masks: keep the packed mask of each row's legal list as well (72 B a row)."""
         self.max_length = int(max_length)
         self.device = torch.device(device)
         self.legal_masks = bool(legal_masks)
@@ -215,7 +236,7 @@ class ReplayBuffer:
             self._alloc(min(self.max_length, max(2 * self.cap, self.size + n)))
         tail = (self.head + self.size) % self.cap
         if self.legal_masks:
-            self._legal[(torch.arange(n, device=self.device) + tail) % self.cap] = _masks_of(pos, self.device)
+            self._legal[(torch.arange(n, device=self.device) + tail) % self.cap] = _masks_of(k, codes[int(e0[0]):])
         args = [c.contiguous() for c in (pos, k, e0, codes, visits, reward)]
         _lib.check(_lib.lib().mtaz_replay_put(
             self.device.index or 0, n, *[a.data_ptr() for a in args], self.cap, tail,
@@ -246,7 +267,7 @@ class ReplayBuffer:
         self._clock[slots] = clk.reshape(n)
         self._pi[slots] = pi
         if self.legal_masks:
-            self._legal[slots] = _masks_of(pos, dev)
+            self._legal[slots] = _masks_of(*(torch.from_numpy(a).to(dev) for a in _lists_of(rows)))
         self._reward[slots] = rew
         over = max(0, self.size + n - self.cap)
         self.size = min(self.cap, self.size + n)
