@@ -43,8 +43,12 @@ def _pointers(tensors):
     return (ctypes.c_void_p * len(tensors))(*[t.data_ptr() for t in tensors])
 
 
-def _workspace(n, rows, cols, dtype, device):
-    size = _lib.check(_lib.lib().mtaz_orthogonalize_workspace(n, rows, cols, TYPES[dtype]))
+def _workspace_size(n, rows, cols, dtype):
+    """Bytes of scratch memory; refuses shapes that the kernels do not take."""
+    return _lib.check(_lib.lib().mtaz_orthogonalize_workspace(n, rows, cols, TYPES[dtype]))
+
+
+def _workspace(size, device):
     return torch.empty(size, dtype=torch.uint8, device=device)
 
 
@@ -113,7 +117,7 @@ def orthogonalize(grad, steps=5, coefficients=COEFFICIENTS, eps=1e-7, out=None):
     ptrs, outs = (ctypes.c_void_p * n)(), (ctypes.c_void_p * n)()
     for i in range(n):
         ptrs[i], outs[i] = src.data_ptr() + i * step, out.data_ptr() + i * step
-    work = _workspace(n, rows, cols, grad.dtype, grad.device)
+    work = _workspace(_workspace_size(n, rows, cols, grad.dtype), grad.device)
     _lib.check(_lib.lib().mtaz_orthogonalize(
         grad.device.index, n, rows, cols, TYPES[grad.dtype], ptrs, outs, int(steps), _coefficients(coefficients),
         float(eps), work.data_ptr(), work.numel(), _stream(grad.device)))
@@ -165,9 +169,11 @@ def muon_step(params, grads, momenta, *, lr, momentum=0.95, nesterov=True, weigh
         if at and written[at - 1][1] > start:
             raise ValueError('a gradient overlaps a parameter or a momentum')
     co = _coefficients(coefficients)
-    for (device, dtype, rows, cols), group in groups.items():
+    # all shapes are looked at before the first group's step
+    sizes = [_workspace_size(len(group), rows, cols, dtype) for (_, dtype, rows, cols), group in groups.items()]
+    for ((device, dtype, rows, cols), group), size in zip(groups.items(), sizes):
         ws, gs, ms = zip(*group)
-        work = _workspace(len(ws), rows, cols, dtype, device)
+        work = _workspace(size, device)
         factor = math.sqrt(max(1.0, rows / cols)) if scale is None else float(scale)
         _lib.check(_lib.lib().mtaz_muon_step(
             device.index, len(ws), rows, cols, TYPES[dtype], _pointers(ws), _pointers(gs), _pointers(ms), float(lr),
