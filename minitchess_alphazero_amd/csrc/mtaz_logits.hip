@@ -647,13 +647,15 @@ __global__ __launch_bounds__(1024) void k_loss_mean(const float* stats, int64_t 
 
 // ---- host ----------------------------------------------------------------------------------------------------
 constexpr int64_t MOST_COLS = 1 << 24;
+constexpr int64_t MOST_WAVES = (1 << 26) - 4;
 
 int64_t tiles_of(int64_t cols, int tile) { return (cols + tile - 1) / tile; }
 const char* bad_shape(int64_t rows, int64_t cols, int dtype) {
   if (rows < 0) return "rows must not be negative";
   if (cols < 1 || cols > MOST_COLS) return "cols must be in [1, 2^24]";
   // a launch has fewer than 2^32 threads: 64 a row in the kernels for short rows, 512 a tile in the others
-  if (rows >= 1 << 26 || (cols > WAVE_COLS && rows * tiles_of(cols, 512 * 4) >= 1 << 23)) return "too many rows for one call";
+  // (rounded up to four rows, or four times 64 entries, a workgroup)
+  if (rows > MOST_WAVES || (cols > WAVE_COLS && rows * tiles_of(cols, 512 * 4) >= 1 << 23)) return "too many rows for one call";
   if (dtype < MTAZ_F32 || dtype > MTAZ_BF16) return "unknown element type";
   return nullptr;
 }
@@ -805,7 +807,7 @@ extern "C" int mtaz_adjust_logits_grad(int device, int64_t rows, int64_t cols, i
   const bool shared = d_bias_grad && bias_grad_stride == 0;
   if (!bad && rows && !d_grad_out) bad = "no incoming gradient";
   if (!bad && rows && t.actions && d_grad && !d_logits) bad = "the penalties' gradient needs the logits";
-  if (!bad && rows * ((history + 63) / 64) >= 1 << 26) bad = "too many rows for one call";
+  if (!bad && rows * ((history + 63) / 64) > MOST_WAVES) bad = "too many rows for one call";
   if (!bad && rows > 1 && ((d_grad && grad_stride < cols) || (d_bias_grad && !shared && bias_grad_stride < cols)))
     bad = "rows of an output overlap";
   if (!bad && shared && rows) bad = bad_work(d_work, work_bytes, 4 * cols * bias_chunks(rows, cols));

@@ -63,3 +63,15 @@ def test_workspaces_off_their_boundary_are_refused():
                                    P + 4096 + off, 1024, None), 'aligned')
         refused(L.mtaz_adjust_logits_grad(0, 2, 40, 0, P, 40, None, 0, P + 1024, 40, P + 2048, 0, None, 0, None, 0, 0, None, None,
                                           None, P + 4096 + off, 1024, None), 'aligned')
+
+
+def test_rows_that_a_launch_does_not_hold_are_refused():
+    """2^26 - 4 waves of 64 threads, four a workgroup, are the most below 2^32 threads."""
+    L, most = _lib.lib(), (1 << 26) - 4
+    assert L.mtaz_policy_loss_workspace(most, 40) == 256
+    for rows in (most + 1, most + 3, most + 4):
+        refused(L.mtaz_policy_loss_workspace(rows, 40), 'too many rows')
+    assert L.mtaz_adjust_logits_grad_workspace(most, 40) > 0
+    for rows, history in ((most // 2 + 1, 65), (most // 4 + 1, 256)):
+        refused(L.mtaz_adjust_logits_grad(0, rows, 1, 0, P, 1, P + 1024, 1, P + 2048, 1, None, 0, None, 0, P + 4096, 0, history, None,
+                                          PEN, None, None, 0, None), 'too many rows')
