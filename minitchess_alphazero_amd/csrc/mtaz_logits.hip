@@ -689,7 +689,7 @@ bool over_inputs(const Place& out, int64_t rows, int64_t cols, const uint32_t* l
 }
 const char* bad_taken(const int32_t* actions, int64_t stride, int history, const double* penalties,
                       const float* per_row) {
-  if (history < 0) return "history must not be negative";
+  if (history < 0 || history > 1 << 30) return "history must be in [0, 2^30]";
   if (!actions || history == 0) return nullptr;
   if (stride < 0) return "actions_stride must not be negative";
   if (!penalties && !per_row) return "actions without penalties";

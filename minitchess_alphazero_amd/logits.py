@@ -114,6 +114,8 @@ class _Taken:
         if actions.dim() != 2:
             raise ValueError(f'actions must be [rows, history], got {tuple(actions.shape)}')
         _check_rows(actions, 'actions', logits, ((rows, actions.shape[1]),), (torch.int32,))
+        if actions.shape[1] > 1 << 30:
+            raise ValueError(f'actions hold at most 2^30 entries a row, got {actions.shape[1]}')
         if lengths is not None:
             _check_rows(lengths, 'lengths', logits, ((rows,),), (torch.int32,))
             lengths = lengths.contiguous()

@@ -75,3 +75,13 @@ def test_rows_that_a_launch_does_not_hold_are_refused():
     for rows, history in ((most // 2 + 1, 65), (most // 4 + 1, 256)):
         refused(L.mtaz_adjust_logits_grad(0, rows, 1, 0, P, 1, P + 1024, 1, P + 2048, 1, None, 0, None, 0, P + 4096, 0, history, None,
                                           PEN, None, None, 0, None), 'too many rows')
+
+
+def test_histories_past_an_int_are_refused():
+    """2^32 + 5 entries a row (one entry, expanded) would be 5 where they are counted in 32 bits."""
+    x = torch.zeros(2, 40)
+    for entries in (1 << 32) + 5, (1 << 31) + 1, (1 << 30) + 1:
+        with pytest.raises(ValueError, match='at most 2'):
+            ops._Taken(x, torch.zeros(1, 1, dtype=torch.int32).expand(2, entries), None, 1.2, 0.0, 0.0)
+    refused(_lib.lib().mtaz_adjust_logits(0, 2, 40, 0, P, 40, P + 1024, 40, None, 0, None, 0, P + 2048, 0, (1 << 30) + 1, None, PEN,
+                                          None, None), 'history')
