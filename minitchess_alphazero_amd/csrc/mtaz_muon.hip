@@ -949,11 +949,16 @@ void iterate(const Matrices& ms, int n, const Shape& sh, const Update& u, int st
   };
   // Two steps in one where the long side is long against the short one: with M = a I + b S + c S S the second step's S
   // is M S M, and X <- M' M X; three products r x r more, and one product over the long side and one with X less
-  // (2048 x 8192 bf16 1902 us without, 1577 with it).  S loses accuracy by that in its small eigenvalues, a^2 = 12 times
-  // the rounding of its large ones: not visible where the result is rounded to 16 bits, and in 32 bits not when it is
-  // done for the first two steps alone and r is not small (against 64 bits, 256 x 2304 Gaussian: 2.2e-6 either way, 3.8e-6
-  // when the next two are joined as well; 64 x 5000 of falling spectrum 8e-7 either way, 15 x 5000 4e-7 and 9e-7).
-  const bool joinable = sh.L >= 3 * sh.r || (sh.r >= 768 && 2 * sh.L >= 3 * sh.r);
+  // (2048 x 8192 bf16 1902 us without, 1577 with it).  That is a gain from L = 3 r on (16 bits, four and eighteen
+  // matrices: 4 x 512 x 1536 209 us without and 202 with it, 18 x 256 x 1024 190 and 178, 3 x 200 x 4000 230 and 199; the
+  // loss where it is none is small: 18 x 128 x 512 109 and 116), and from 1.5 r on where the square products fill the
+  // chip, which takes about three million elements in them (6 x 1000 x 1536 731 and 681, 1 x 2048 x 3200 865 and 802, 6 x
+  // 768 x 1152 399 and 395; but 1 x 768 x 1152 171 and 192, 6 x 640 x 960 296 and 309).
+  // S loses accuracy by that in its small eigenvalues, a^2 = 12 times the rounding of its large ones: not visible
+  // where the result is rounded to 16 bits, and in 32 bits not when it is done for the first two steps alone and r is not
+  // small (against 64 bits, gradients of few strong directions: 6 x 1000 x 1536 2.5e-6 without and 1.9e-6 with it, 18 x 256
+  // x 1024 1.4e-6 and 1.3e-6; 64 x 5000 of falling spectrum 8e-7 either way, but 15 x 5000 4e-7 and 9e-7).
+  const bool joinable = sh.L >= 3ll * sh.r || (2ll * sh.L >= 3ll * sh.r && (int64_t)n * sh.r * sh.r >= 3 << 20);
   int now = 0;
   for (int t = 0; t < steps;) {
     const bool join = joinable && t + 1 < steps && (DT != MTAZ_F32 || (t == 0 && sh.r >= 64));
