@@ -438,7 +438,7 @@ template <int DT, int DP, int THREADS, int REP, bool KEEP = true> struct Held {
 };
 
 // Rows of up to WAVE_COLS columns: a wave each, and everything stays in its registers.  4096 x 554 f32 with targets:
-// 8 us (18 MB).  ONE: a single workgroup takes all rows and their mean (32 x 554 with the gradient 8.6 us).
+// 8 us (18 MB).  ONE: a single workgroup takes all rows and their mean (32 x 554 with the gradient 8.3 us).
 template <int DT, int DP, bool ONE>
 __global__ __launch_bounds__(ONE ? 1024 : 256) void k_loss_wave(const typename Elem<DT>::T* z, int64_t z_stride,
                                                                 const typename Elem<DP>::T* pi, int64_t pi_stride,
@@ -630,8 +630,19 @@ __global__ __launch_bounds__(NT) void k_loss_grad(const typename Elem<DT>::T* z,
                     Row{0.f, st.x, st.y, st.z}, k);
 }
 
-// The mean of the rows' losses by one workgroup, in a fixed order and in 64 bits
+// The mean of the rows' losses by one workgroup, in a fixed order and in 64 bits.  A few rows are added like k_loss_wave's
+// one workgroup adds them, 16 waves' sums one after the other: a captured call, which takes this way, gives the same bits.
+constexpr int64_t FEW_ROWS = 32;
 __global__ __launch_bounds__(1024) void k_loss_mean(const float* stats, int64_t rows, float* loss) {
+  if (rows <= FEW_ROWS) {
+    if (threadIdx.x >= 64) return;
+    double s = 0.;
+    for (int64_t r = threadIdx.x; threadIdx.x < 16 && r < rows; r += 16) s += (double)stats[4 * r + 3];
+    double mean = __shfl(s, 0);
+    for (int w = 1; w < 16; ++w) mean += __shfl(s, w);
+    if (threadIdx.x == 0) *loss = (float)(mean / (double)rows);
+    return;
+  }
   double s = 0.;
 #pragma unroll 4
   for (int64_t r = threadIdx.x; r < rows; r += 1024) s += (double)stats[4 * r + 3];
@@ -712,6 +723,11 @@ int64_t loss_workspace(int64_t rows, int64_t cols) {
 }
 const char* bad_work(const void* work, int64_t bytes, int64_t needed) {
   return !work || ((uintptr_t)work & 255) || bytes < needed ? "workspace too small or not aligned to 256 bytes" : nullptr;
+}
+// Whether the stream records a graph.  (The stream of nullptr cannot, and asked beside another's capture it would end that.)
+bool capturing(hipStream_t s) {
+  hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+  return s && hipStreamIsCapturing(s, &status) == hipSuccess && status == hipStreamCaptureStatusActive;
 }
 int launched(const char* what) {
   const hipError_t e = hipGetLastError();
@@ -895,9 +911,11 @@ extern "C" int mtaz_policy_loss(int device, int64_t rows, int64_t cols, int dtyp
   const int nc = (int)cols;
   const Legal legal{d_legal, legal_stride};
   const float k = (float)(scale / (double)rows);
-  // A handful of short rows: one launch, mean included, which saves the host 4 us.  On the GPU it takes with 16, 32 and 64
-  // rows of 554 4.9, 7.4 and 12.9 us, the two launches 6.0 each time.
-  const bool one = cols <= WAVE_COLS && rows <= 32;
+  // A handful of short rows: one launch, mean included.  With 8, 16, 24, 32 and 64 rows of 554 it takes 4.3, 5.3, 7.0, 8.3 and
+  // 15.0 us in a graph, and the two launches 6.0 to 6.2 each time; called one by one, where the host's launches bound
+  // them, 7.4, 7.4, 7.5, 8.5 and 15.0 against 9.8.  So up to 16 rows, and up to 32 outside a capture: the means are
+  // added in the same order on both sides.
+  const bool one = cols <= WAVE_COLS && (rows <= FEW_ROWS / 2 || (rows <= FEW_ROWS && !capturing(s)));
   FOR_TYPES(dtype, target_dtype, {
     const auto* z = (const Elem<DT>::T*)d_logits;
     const auto* pi = (const Elem<DP>::T*)d_target;

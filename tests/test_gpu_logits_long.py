@@ -106,3 +106,28 @@ def test_gradient_without_a_repetition_penalty_needs_no_logits():
             0, rows, cols, 0, dy.data_ptr(), cols, None, 0, dx.data_ptr(), cols, None, 0, mask.data_ptr(), mask.stride(0),
             actions.data_ptr(), 6, 6, None, host, None, None, 0, torch.cuda.current_stream().cuda_stream))
         assert torch.equal(dx, want)
+
+
+@pytest.mark.parametrize('rows', [1, 15, 16, 17, 31, 32, 33])
+def test_small_batches_captured_and_called(rows):
+    """A captured call may take other launches than one that is made at once, and gives the same bits."""
+    z, legal, _, _ = make(rows, 554, 1, rows, density=0.5)
+    t = torch.rand(rows, 554, generator=gen(rows)) * legal
+    v, r = torch.rand(rows, 1, generator=gen(1)), torch.ones(rows, 1)
+    args = [a.cuda() for a in (z, t, v, r, pack(legal))]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        ops.policy_value_loss_grad(*args)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = ops.policy_value_loss_grad(*args)
+    for k in range(4):
+        args[0].mul_(0.75)
+        graph.replay()
+        want = ops.policy_value_loss_grad(*args)
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(out, want)), k
+        mean = loss64(args[0].cpu(), t, legal, v, r)[0]
+        assert abs(float(want[0]) - float(mean)) <= 1e-5 * abs(float(mean))
