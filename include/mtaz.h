@@ -108,8 +108,9 @@ int mtaz_replay_put(int device, int n, const uint32_t* d_pos, const int32_t* d_k
 /* Orthogonalisation of n matrices G [rows][cols] (contiguous, one pointer each in the host array
  * d_grad), rows, cols <= 65536 and rows * cols <= 2^30: X = G / (|G|_F + eps), then `steps` times
  * X <- a X + (b S + c S S) X with S = X X^T over the shorter side, coefficients = {a, b, c}.
- * Computed to 32 bits whatever the type, relative to the largest singular value; d_out[i] may be
- * d_grad[i], and no other two matrices of a call may overlap. */
+ * Whatever the type, products are of 22-bit factors with float32 sums, relative to the largest singular
+ * value, and the result is rounded once; d_out[i] may be d_grad[i], and no other two matrices of a
+ * call may overlap. */
 int64_t mtaz_orthogonalize_workspace(int n, int64_t rows, int64_t cols, int dtype);
 int mtaz_orthogonalize(int device, int n, int64_t rows, int64_t cols, int dtype, const void* const* d_grad,
                        void* const* d_out, int steps, const double* coefficients, double eps, void* d_work,
@@ -129,11 +130,11 @@ int mtaz_muon_step(int device, int n, int64_t rows, int64_t cols, int dtype, voi
  * everything is legal.  d_bias: float32, likewise (bias_stride 0 = shared).  d_actions: the actions
  * taken so far, row b's first d_lengths[b] (NULL: `history`) entries count, entries outside
  * [0, cols) do not.  Penalties {repetition, frequency, presence}: the host triple, or one triple per
- * row in d_penalties.  Strides are in elements (words for d_legal); cols <= 2^24.
+ * row in d_penalties.  Strides are in elements (words for d_legal); cols <= 2^24, history <= 2^30.  No output
+ * may overlap a mask, the actions, their lengths or penalties.
  *
- * Adjusted logits y (same type; d_out may be d_logits with the same stride, and may not overlap it
- * otherwise): with c = how often v
- * was taken in the row, x <- c ? (x > 0 ? x / repetition : x repetition) - c frequency - presence : x;
+ * Adjusted logits y (same type; d_out may be d_logits with the same stride, or row for row a float32 d_bias, and
+ * may not overlap them otherwise): with c = how often v was taken in the row, x <- c ? (x > 0 ? x / repetition : x repetition) - c frequency - presence : x;
  * y = x + bias where legal, -inf elsewhere whatever x holds there. */
 int mtaz_adjust_logits(int device, int64_t rows, int64_t cols, int dtype, const void* d_logits, int64_t logits_stride,
                        void* d_out, int64_t out_stride, const uint32_t* d_legal, int64_t legal_stride,
