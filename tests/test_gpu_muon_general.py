@@ -58,7 +58,7 @@ def test_muon_step(n, shape, nesterov, dtype):
 
 @pytest.mark.parametrize('dtype', list(HALF), ids=str)
 @pytest.mark.parametrize('shape,tight', [((3, 1021, 509), False), ((10, 896, 1000), False), ((1, 800, 1300), False),
-                                         ((1, 1000, 1536), False), ((1, 256, 300), False), ((4, 1101, 500), False),
+                                         ((1, 1000, 1536), False), ((4, 1000, 1536), False), ((1, 256, 300), False), ((4, 1101, 500), False),
                                          ((2, 768, 3100), True), ((1, 5000, 1100), True)], ids=str)
 def test_forms_of_the_products(shape, tight, dtype):
     g = randn(*shape, seed=sum(shape), dtype=dtype)
@@ -66,7 +66,7 @@ def test_forms_of_the_products(shape, tight, dtype):
 
 
 @pytest.mark.parametrize('dtype', list(HALF), ids=str)
-@pytest.mark.parametrize('shape', [(64, 3000), (150, 1100), (800, 1300), (1300, 800), (509, 1021)], ids=str)
+@pytest.mark.parametrize('shape', [(64, 3000), (150, 1100), (800, 1300), (1300, 800), (509, 1021), (1800, 2800)], ids=str)
 @pytest.mark.parametrize('kind', ['low rank', 'falling'])
 def test_small_singular_values(kind, shape, dtype):
     """A few strong directions and weak noise, or singular values falling over four decades: what two steps joined make of
