@@ -474,7 +474,7 @@ class SimpleAlphaZeroLearner:
                     pending.append(step(idx))
                     continue
                 for o in optimizers:
-                    o.zero_grad()
+                    o.zero_grad(set_to_none=step is None)   # the captured step goes on writing to these gradients
                 loss = self._backward(model, data, torch.as_tensor(idx, dtype=torch.long, device=self._device))
                 pending.append(loss.clone())
                 for o in optimizers:
