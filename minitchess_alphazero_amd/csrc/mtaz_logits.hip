@@ -138,7 +138,8 @@ template <int DT, int N> struct Words {
 template <int DT> constexpr uint32_t NEVER = DT == MTAZ_F32 ? 0xff800000u : DT == MTAZ_F16 ? 0xfc00fc00u : 0xff80ff80u;
 // One access: N logits, the counts of their actions (none: nullptr), their bias and legality.  Without a branch and
 // with the reciprocal of the repetition penalty, because a few taken actions among many others are enough to send
-// every wave through all branches.
+// every wave through all branches.  The reciprocal is a rounded float itself, so that x times it is off by up to 2^-23 of
+// the result, where x / repetition would be by 2^-24.
 template <int DT, int N>
 __device__ __forceinline__ void adjust(Words<DT, N>& q, const uint32_t* cnt, const Words<MTAZ_F32, N>& bias, uint32_t ok,
                                        const Penalty& p) {
@@ -164,7 +165,7 @@ __device__ __forceinline__ void adjust(Words<DT, N>& q, const uint32_t* cnt, con
 }
 
 // Rows of up to WAVE_COLS columns: a wave each, with the counts of its actions in its own piece of LDS.  4096 x 554 f32
-// with 60 actions a row, mask and bias: 6.7 us (19 MB, 2.9 TB/s, most of it from the caches).
+// with 60 actions a row and masks: 6.8 us (19 MB, 2.9 TB/s, most of it from the caches).
 constexpr int WAVE_COLS = 1024;
 template <int DT>
 __global__ __launch_bounds__(256) void k_adjust_wave(const typename Elem<DT>::T* x, int64_t x_stride,
@@ -208,9 +209,10 @@ __global__ __launch_bounds__(256) void k_adjust_wave(const typename Elem<DT>::T*
 
 // Longer rows in tiles, so that one long row fills the chip as well as many: a workgroup counts the actions in its
 // columns.  Integer adds, so their order does not matter.  One access a thread and four workgroups on a CU hide each
-// other's phases; two accesses take 84 registers and only two workgroups fit (1024 x 50021 f16 with everything 52 and
-// 62 us, 205 MB; f32 92 and 97).  A workgroup takes `per` rows one after the other, more than one only where they share
-// mask and bias, which it then reads once.
+// other's phases; two accesses take 84 registers, only two workgroups fit, and it took a fifth longer.  1024 x 50021 f16
+// with everything (205 MB): 60 us in a training step, where the logits come from memory, 43 call after call, where
+// the last-level cache has them; without actions 33.  A workgroup takes `per` rows one after the other, more than one
+// only where they share mask and bias, which it then reads once.
 constexpr int NT = 512;
 template <int DT, bool COUNTED>
 __global__ __launch_bounds__(NT) void k_adjust(const typename Elem<DT>::T* x, int64_t x_stride,
@@ -324,7 +326,8 @@ __global__ __launch_bounds__(256) void k_bias_join(const float* part, int chunks
 // With top the largest legal logit, total = sum exp(z - top), pi = sum of the targets, dot = sum pi (z - top):
 //   row = pi log(total) - dot,   d row / d z = exp(z - top) / total * pi - target.
 // exp by the instruction for 2^x: the product with log2(e) is off by 2^-24 of z - top, which a term e^(z - top) turns
-// into at most 0.37 * 2^-24 of the largest.
+// into at most 0.37 * 2^-24 of the largest; relative to the term itself it is |z - top| 2^-24, as much as the difference
+// z - top is off by its own rounding, so that a small term is off by twice what a float's exp of that difference is.
 __device__ __forceinline__ float soft_exp(float d) { return __builtin_amdgcn_exp2f(d * 1.44269504088896341f); }
 
 struct Row {
@@ -505,7 +508,10 @@ __global__ __launch_bounds__(THREADS, 4) void k_loss_block(const typename Elem<D
   if (threadIdx.x == 0) finish_row(r, row, value, reward, k, stats, value_grad);
 }
 
-// Longer rows in tiles: the statistics of a tile, then of the row from its tiles'.
+// Longer rows in tiles: the statistics of a tile, then of the row from its tiles'.  The gradient reads logits and targets
+// again, since a row does not fit into a workgroup's registers: 512 x 131072 bf16 takes 56 us for the statistics (268 MB,
+// 4.8 TB/s) and 67 for the gradient (403 MB, 6.0 TB/s, some of it from the last-level cache), 128 with the mean; one pass
+// over what has to move would take 78 at the rate of a copy.
 struct Soft {
   float top, total, pi, dot;
 };
@@ -594,7 +600,8 @@ __global__ __launch_bounds__(NT) void k_loss_row(const typename Elem<DT>::T* z, 
                     joined, k);
 }
 
-// The gradient from the statistics: rows of up to WAVE_COLS a wave each, longer ones in tiles
+// The gradient from the statistics: rows of up to WAVE_COLS a wave each, longer ones in tiles (2048 x 32003 bf16 73 us, 393
+// MB, 5.4 TB/s; 512 x 131072 59 us)
 template <int DT, int DP>
 __global__ __launch_bounds__(256) void k_loss_grad_wave(const typename Elem<DT>::T* z, int64_t z_stride,
                                                         const typename Elem<DP>::T* pi, int64_t pi_stride, int64_t rows,
@@ -790,7 +797,8 @@ extern "C" int mtaz_adjust_logits(int device, int64_t rows, int64_t cols, int dt
     } else {
       const int64_t tiles = tiles_of(cols, NT * PER<DT>);
       // Two rows a workgroup where they share what it would read again, a float's bias for each logit, and the chip is
-      // full twice over all the same (1024 x 50021 f16: 52 us, with one row 59, with four 52; f32 92, 97 and 95).
+      // full twice over all the same (call after call, 512 actions: 1024 x 50021 f16 43 us, with one row 48, f32 90 and 99,
+      // 4096 x 5000 f16 24 and 28; from memory 2 to 3 us less with two rows, and without actions as much more).
       const bool two = d_bias && bias_stride == 0 && (!d_legal || legal_stride == 0) && rows * tiles >= 4096;
       const unsigned grid = (unsigned)((two ? (rows + 1) / 2 : rows) * tiles);
       if (t.actions) k_adjust<DT, true><<<grid, NT, 0, s>>>(x, logits_stride, y, out_stride, rows, two ? 2 : 1, nc, (int)tiles,
