@@ -325,10 +325,18 @@ __global__ __launch_bounds__(256) void k_bias_join(const float* part, int chunks
 // ---- policy/value loss -------------------------------------------------------------------------------------
 // With top the largest legal logit, total = sum exp(z - top), pi = sum of the targets, dot = sum pi (z - top):
 //   row = pi log(total) - dot,   d row / d z = exp(z - top) / total * pi - target.
-// exp by the instruction for 2^x: the product with log2(e) is off by 2^-24 of z - top, which a term e^(z - top) turns
-// into at most 0.37 * 2^-24 of the largest; relative to the term itself it is |z - top| 2^-24, as much as the difference
-// z - top is off by its own rounding, so that a small term is off by twice what a float's exp of that difference is.
+// exp by the instruction for 2^x.  The product with log2(e) is off by 2^-24 of z - top (and the factor by a third of that),
+// which a term e^(z - top) turns into at most 0.5 * 2^-24 of the largest, but |z - top| 2^-24 of itself: for float
+// logits, whose small gradients would show it, the product's remainder goes into the term.  Five operations more a
+// logit, which 4096 x 554 do not show.  (0 stays 0: the remainder of a product past -FLT_MAX is no number.)
 __device__ __forceinline__ float soft_exp(float d) { return __builtin_amdgcn_exp2f(d * 1.44269504088896341f); }
+template <int DT> __device__ __forceinline__ float soft_exp_of(float d) {
+  if constexpr (DT != MTAZ_F32) return soft_exp(d);
+  constexpr double LOG2E = 1.44269504088896341;
+  constexpr float HIGH = (float)LOG2E, LOW = (float)(LOG2E - (double)HIGH);
+  const float p = d * HIGH, rest = fmaf(d, LOW, fmaf(d, HIGH, -p)), e = __builtin_amdgcn_exp2f(p);
+  return e > 0.f ? fmaf(e, rest * 0.693147180559945309f, e) : e;
+}
 
 struct Row {
   float loss;          // without the value term
@@ -412,7 +420,7 @@ template <int DT, int DP, int THREADS, int REP, bool KEEP = true> struct Held {
 #pragma unroll
       for (int j = 0; j < N; ++j) {
         const float d = z[k].get(j) - base, t = w[k].get(j);
-        const float x = soft_exp(d);
+        const float x = soft_exp_of<DT>(d);
         if (KEEP) e[k][j] = x;
         total += x;
         pi += t;
@@ -429,7 +437,7 @@ template <int DT, int DP, int THREADS, int REP, bool KEEP = true> struct Held {
       if (n <= 0) continue;
       Words<DT, N> o;
 #pragma unroll
-      for (int j = 0; j < N; ++j) o.put(j, Elem<DT>::put(fmaf(KEEP ? e[q][j] : soft_exp(z[q].get(j) - base), soft,
+      for (int j = 0; j < N; ++j) o.put(j, Elem<DT>::put(fmaf(KEEP ? e[q][j] : soft_exp_of<DT>(z[q].get(j) - base), soft,
                                       -kt * w[q].get(j))));
       if (ok[q] != (1u << N) - 1)                       // 0 there in a row of NaN too
 #pragma unroll

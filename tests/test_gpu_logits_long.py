@@ -131,3 +131,21 @@ def test_small_batches_captured_and_called(rows):
         assert all(torch.equal(a, b) for a, b in zip(out, want)), k
         mean = loss64(args[0].cpu(), t, legal, v, r)[0]
         assert abs(float(want[0]) - float(mean)) <= 1e-5 * abs(float(mean))
+
+
+@pytest.mark.parametrize('cols', [64, 2000, 20000, 40000])
+def test_gradients_of_small_terms(cols):
+    """float32 logits down to 80 below the top, which is 0, so that the differences are exact: each gradient k softmax is off
+    by exp (2 U, and U for its correction), the sum of what is near the top (a handful of terms over up to 6 + 16 + 8
+    additions, and 3 U of each), its reciprocal and four products, whatever its size: less than 45 U of itself."""
+    z = torch.full((2, cols), -200.0)
+    z[:, :64] = -torch.linspace(0, 80, 64)
+    z[1] = z[1].flip(0)                     # the same from the last column on
+    t = torch.zeros(2, cols)
+    t[0, 0] = t[1, -1] = 1.0
+    x = z.cuda().requires_grad_()
+    ops.policy_value_loss(x, t.cuda()).backward()
+    soft = z.double().softmax(1) / 2
+    for dz in (ops.policy_value_loss_grad(z.cuda(), t.cuda())[1].cpu().double(), x.grad.cpu().double()):
+        for row, there in ((0, slice(1, 64)), (1, slice(cols - 64, cols - 1))):
+            assert float((dz[row, there] / soft[row, there] - 1).abs().max()) <= 45 * U
