@@ -328,7 +328,7 @@ __global__ __launch_bounds__(256) void k_bias_join(const float* part, int chunks
 // exp by the instruction for 2^x.  The product with log2(e) is off by 2^-24 of z - top (and the factor by a third of that),
 // which a term e^(z - top) turns into at most 0.5 * 2^-24 of the largest, but |z - top| 2^-24 of itself: for float
 // logits, whose small gradients would show it, the product's remainder goes into the term.  Five operations more a
-// logit, which 4096 x 554 do not show.  (0 stays 0: the remainder of a product past -FLT_MAX is no number.)
+// logit: 4096 x 554 with targets 7.7 us in place of 7.2.  (0 stays 0: the remainder of a product past -FLT_MAX is no number.)
 __device__ __forceinline__ float soft_exp(float d) { return __builtin_amdgcn_exp2f(d * 1.44269504088896341f); }
 template <int DT> __device__ __forceinline__ float soft_exp_of(float d) {
   if constexpr (DT != MTAZ_F32) return soft_exp(d);
@@ -449,7 +449,7 @@ template <int DT, int DP, int THREADS, int REP, bool KEEP = true> struct Held {
 };
 
 // Rows of up to WAVE_COLS columns: a wave each, and everything stays in its registers.  4096 x 554 f32 with targets:
-// 8 us (18 MB).  ONE: a single workgroup takes all rows and their mean (32 x 554 with the gradient 8.3 us).
+// 8 us (18 MB).  ONE: a single workgroup takes all rows and their mean (32 x 554 with the gradient 9.2 us).
 template <int DT, int DP, bool ONE>
 __global__ __launch_bounds__(ONE ? 1024 : 256) void k_loss_wave(const typename Elem<DT>::T* z, int64_t z_stride,
                                                                 const typename Elem<DP>::T* pi, int64_t pi_stride,
@@ -927,10 +927,10 @@ extern "C" int mtaz_policy_loss(int device, int64_t rows, int64_t cols, int dtyp
   const int nc = (int)cols;
   const Legal legal{d_legal, legal_stride};
   const float k = (float)(scale / (double)rows);
-  // A handful of short rows: one launch, mean included.  With 8, 16, 24, 32 and 64 rows of 554 it takes 4.3, 5.3, 7.0, 8.3 and
-  // 15.0 us in a graph, and the two launches 6.0 to 6.2 each time; called one by one, where the host's launches bound
-  // them, 7.4, 7.4, 7.5, 8.5 and 15.0 against 9.8.  So up to 16 rows, and up to 32 outside a capture: the means are
-  // added in the same order on both sides.
+  // A handful of short rows: one launch, mean included.  With 8, 16, 24, 32 and 64 rows of 554 it takes 4.6, 5.7, 7.6, 9.0 and
+  // 16.3 us in a graph, and the two launches 5.9 to 6.5; called one by one, where the host's launches bound them, 7.8, 7.9,
+  // 8.2, 9.3 and 16.4 against 10.4.  So up to 16 rows, and up to 32 outside a capture: the means are added in the same
+  // order on both sides.
   const bool one = cols <= WAVE_COLS && (rows <= FEW_ROWS / 2 || (rows <= FEW_ROWS && !capturing(s)));
   FOR_TYPES(dtype, target_dtype, {
     const auto* z = (const Elem<DT>::T*)d_logits;

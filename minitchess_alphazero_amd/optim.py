@@ -88,8 +88,9 @@ def _stream(device):
 def orthogonalize(grad, steps=5, coefficients=COEFFICIENTS, eps=1e-7, out=None):
     """Each matrix of grad [..., rows, cols] (float32, float16 or bfloat16) divided by its Frobenius
     norm + eps and taken through `steps` Newton-Schulz steps over its shorter side.  The result has
-    grad's type and shape; the products keep 32-bit accuracy whatever the type.  out: a contiguous tensor
-    for the result (grad itself is allowed).  There is no backward pass and no forward-mode derivative.
+    grad's type and shape; whatever the type, the products have factors of 22 bits and float32 sums, and
+    the result is rounded once.  out: a contiguous tensor for the result (grad itself is allowed).  There is no
+    backward pass and no forward-mode derivative.
 
     Accuracy is relative to the largest singular value: entries below 2^-38 of the norm are taken as 0."""
     _check_type(grad, 'grad')

@@ -84,3 +84,17 @@ def test_negated_views_are_the_numbers_they_show():
     for w, m in ((x, t), (t, x)):
         with pytest.raises(ValueError, match='negated'):
             optim.muon_step([w], [t.clone()], [m], lr=0.1)
+
+
+@pytest.mark.parametrize('backend', ['eager', 'aot_eager'])
+def test_compiled_functions_compute_the_same(backend):
+    x, b, v, mask, actions, lengths, t = inputs(7)
+
+    def loss(x, b):
+        return ops.policy_value_loss(ops.adjust_logits(x, mask, b, actions, lengths, 1.2, 0.1, 0.3), t)
+    both = []
+    for f in (loss, torch.compile(loss, backend=backend)):
+        leaves = [a.clone().requires_grad_() for a in (x, b)]
+        out = f(*leaves)
+        both.append((out, *torch.autograd.grad(out, leaves)))
+    assert all(torch.equal(p, q) for p, q in zip(*both))
