@@ -4,6 +4,7 @@ import torch
 from torch.autograd import forward_ad
 from torch.fx.experimental.proxy_tensor import make_fx
 
+from minitchess_alphazero_amd import _lib
 from minitchess_alphazero_amd import logits as ops
 from minitchess_alphazero_amd import optim
 from test_gpu_logits import gen, make, pack
@@ -98,3 +99,16 @@ def test_compiled_functions_compute_the_same(backend):
         out = f(*leaves)
         both.append((out, *torch.autograd.grad(out, leaves)))
     assert all(torch.equal(p, q) for p, q in zip(*both))
+
+
+def test_operators_keep_what_their_schemas_say():
+    """Schemas (nothing written, no aliases), registrations and the results without data, by torch's own checks."""
+    x, b, v, mask, actions, lengths, t = inputs(9)
+    nodes = _lib.nodes()
+    leaf = [a.clone().requires_grad_() for a in (x, b, v)]
+    for op, args in ((nodes.adjust_logits, (leaf[0], leaf[1], mask, actions, lengths, None, 1.2, 0.1, 0.2, True)),
+                     (nodes.adjust_logits, (x, None, None, None, None, None, 1.0, 0.0, 0.0, False)),
+                     (nodes.policy_loss, (leaf[0], leaf[2], t, torch.ones_like(v), mask)),
+                     (nodes.policy_loss_grad, (x, v, t, torch.ones_like(v), mask, 2.0)),
+                     (nodes.policy_loss_grad, (x, None, t, None, None, 1.0))):
+        torch.library.opcheck(op.default, args)
